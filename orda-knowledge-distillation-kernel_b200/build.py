@@ -11,17 +11,19 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
-LIB = os.path.join(HERE, "orda_ce_kernel", "liborda_b200.so")
+LIB_NAME = "liborda_b200.so"
+LIB = os.path.join(HERE, "orda_ce_kernel", LIB_NAME)
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
 ]
 
@@ -48,12 +50,22 @@ def needs_build() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB
-    tmp = LIB + ".tmp"
-    cmd = [_nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-o", tmp, os.path.join(CSRC, "orda_abi.cu")]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, LIB)
+    nvcc = _nvcc()
+    with tempfile.TemporaryDirectory(dir=os.path.dirname(LIB)) as tmp:
+        # the translation units compile side by side
+        objects, running = [], []
+        for unit in sorted(glob.glob(os.path.join(CSRC, "*.cu"))):
+            objects.append(os.path.join(tmp, os.path.basename(unit) + ".o"))
+            cmd = [nvcc, *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c", unit, "-o", objects[-1]]
+            if verbose:
+                print(" ".join(cmd))
+            running.append((cmd, subprocess.Popen(cmd)))
+        failed = [cmd for cmd, p in running if p.wait() != 0]
+        if failed:
+            raise subprocess.CalledProcessError(1, failed[0])
+        lib = os.path.join(tmp, LIB_NAME)
+        subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", lib, *objects], check=True)
+        os.replace(lib, LIB)
     return LIB
 
 

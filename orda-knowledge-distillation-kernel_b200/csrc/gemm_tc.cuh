@@ -20,7 +20,11 @@
 
 namespace orda {
 
-enum EpiKind { EPI_FWD_STATS = 0, EPI_STORE = 1 };
+enum EpiKind {
+  EPI_FWD_STATS = 0,
+  EPI_STORE = 1,
+  EPI_GLU = 2,  // wide kernel: act(gate) * up of two weights' products (gated feed-forward block)
+};
 
 constexpr int kBK = 64;                       // k elements per stage (128 B of 16-bit data)
 constexpr uint32_t kATileBytes = kTileRows * kBK * 2;
@@ -65,6 +69,9 @@ struct TcGemmParams {
   int64_t split_bytes;
   int32_t prof_slot;  // >= 0: accumulate pipeline wait counters into g_tc2_prof[prof_slot] (testing hook)
   int32_t* status;
+  // EPI_GLU: b0 / b1 are the gate / up weights, out_map stores h, ws_s_map / ws_t_map the products before
+  // the activation (glu_save = 1)
+  int32_t glu_act, glu_save;
   FwdEpiParams fwd;
   StoreEpiParams st;
 };

@@ -20,6 +20,10 @@
 //
 // Row mapping of a tile (pair rows 0..511; CTA rank r, accumulator j, TMEM lane l):
 //   A_PLAIN      : row j*256 + r*128 + l
+// EPI_GLU (gated feed-forward block): the tile is 512 rows x 128 features. CTA 0 loads its 128-column
+// half of B from the gate weight and CTA 1 the same features of the up weight, so columns 0..127 of
+// every accumulator row hold x Wgate^T and columns 128..255 x Wup^T of the same features, and one
+// thread has both factors of its h.
 //   A_INTERLEAVE : token j*128 + r*64 + (l & 63); lanes 0..63 student (A0), 64..127 teacher (A1)
 #pragma once
 
@@ -27,6 +31,7 @@
 #include "fwd_epilogue.cuh"
 #include "gemm_tc.cuh"
 #include "gemm_tc2.cuh"
+#include "glu_math.cuh"
 #include "sm100_ptx.cuh"
 
 namespace orda {
@@ -243,6 +248,68 @@ __device__ __forceinline__ void wide_store_tma(const TcGemmParams& p, uint32_t t
   }
 }
 
+// One 32-row x 64-column piece, one row per lane, from registers through the warp's staging buffer to a
+// TMA store. w(q, e): words e = 0..3 of the row's 16-byte chunk q.
+template <typename Word>
+__device__ __forceinline__ void wide_stage_store(const CUtensorMap* map, uint32_t staging, int64_t y0, int64_t c0,
+                                                 int lane, Word&& w) {
+  // the previous TMA store of this warp must have read the staging buffer
+  if (lane == 0) bulk_wait_read_all();
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const uint32_t addr = staging + static_cast<uint32_t>(lane) * 128u +
+                          ((static_cast<uint32_t>(q) ^ static_cast<uint32_t>(lane & 7)) << 4);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w(q, 0)), "r"(w(q, 1)), "r"(w(q, 2)),
+                 "r"(w(q, 3))
+                 : "memory");
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(map, staging, static_cast<int32_t>(c0), static_cast<int32_t>(y0));
+    bulk_commit_group();
+  }
+}
+
+// Gated epilogue of the warp's 32 rows x 128 features: h = act(g) u, and g and u themselves where the
+// backward pass will want them, 64 features at a time through the staging buffer.
+template <typename T16>
+__device__ __forceinline__ void wide_glu_store(const TcGemmParams& p, uint32_t tbase, uint32_t staging, int64_t y0,
+                                               int64_t f0, int lane) {
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    const int64_t c0 = f0 + half * 64;
+    uint32_t g[2][32], u[2][32];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      tmem_ld32_async(tbase + half * 64 + c * 32, g[c]);
+      tmem_ld32_async(tbase + 128 + half * 64 + c * 32, u[c]);
+    }
+    tmem_wait_ld();
+    if (c0 >= p.st.N || y0 >= p.st.M) continue;  // warp-uniform
+    auto pair_of = [&](uint32_t (&v)[2][32], int q, int e) {
+      const int i = (q & 3) * 8 + 2 * e;
+      return pack2<T16>(__uint_as_float(v[q >> 2][i]), __uint_as_float(v[q >> 2][i + 1]));
+    };
+    if (p.glu_save) {
+      wide_stage_store(&p.ws_s_map, staging, y0, c0, lane, [&](int q, int e) { return pair_of(g, q, e); });
+      wide_stage_store(&p.ws_t_map, staging, y0, c0, lane, [&](int q, int e) { return pair_of(u, q, e); });
+    }
+    with_act(p.glu_act, [&](auto tag) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          float a, d;
+          glu_act<decltype(tag)::kAct, false>(__uint_as_float(g[c][j]), a, d);
+          u[c][j] = __float_as_uint(a * __uint_as_float(u[c][j]));
+        }
+    });
+    wide_stage_store(&p.out_map, staging, y0, c0, lane, [&](int q, int e) { return pair_of(u, q, e); });
+  }
+}
+
 template <bool A_MN, bool B_MN, int AMODE, bool TWO_SEG, int EPI, typename T16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThreads, 1)
     tc2w_gemm_kernel(const __grid_constant__ TcGemmParams p) {
@@ -292,7 +359,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThr
     tma_prefetch_desc(&p.a0);
     tma_prefetch_desc(&p.b0);
     if (AMODE == A_INTERLEAVE || TWO_SEG) tma_prefetch_desc(&p.a1);
-    if (TWO_SEG) tma_prefetch_desc(&p.b1);
+    if (TWO_SEG || EPI == EPI_GLU) tma_prefetch_desc(&p.b1);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, kTmemCols);
@@ -314,7 +381,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThr
       for (int32_t t = pair; t < num_tiles && ok; t += npairs) {
         int32_t mt, nt, ks, kb_begin, kb_count;
         decode(t, mt, nt, ks, kb_begin, kb_count);
-        const int32_t n_cta = nt * kPairBN + static_cast<int32_t>(rank) * 128;
+        const int32_t n_cta = EPI == EPI_GLU ? nt * 128 : nt * kPairBN + static_cast<int32_t>(rank) * 128;
         for (int32_t kbl = 0; kbl < kb_count; ++kbl) {
           const int32_t kb = kb_begin + kbl;
           const long long c0 = prof ? clk() : 0;
@@ -327,7 +394,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThr
           const bool seg1 = TWO_SEG && kb >= p.kb0;
           const int32_t k0 = (seg1 ? kb - p.kb0 : kb) * kBK;
           const CUtensorMap* amap = seg1 ? &p.a1 : &p.a0;
-          const CUtensorMap* bmap = seg1 ? &p.b1 : &p.b0;
+          const CUtensorMap* bmap = (EPI == EPI_GLU ? rank != 0 : seg1) ? &p.b1 : &p.b0;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t saj = sa + j * kATileBytes;
@@ -510,6 +577,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThr
                               (p.fwd.flags & (tdist ? F_WRITE_WS_T : F_WRITE_WS_S)) != 0, tbase, staging, y0 + lane,
                               y0, n0, !tdist, lane, j ? lab[1] : lab[0]);
           }
+        } else if constexpr (EPI == EPI_GLU) {
+          const int64_t y0 = static_cast<int64_t>(mt) * 512 + j * 256 + rank * 128 + quarter * 32;
+          wide_glu_store<T16>(p, tbase, staging, y0, static_cast<int64_t>(nt) * 128, lane);
         } else {
           const int64_t y0 = static_cast<int64_t>(mt) * 512 + j * 256 + rank * 128 + quarter * 32;
           if (p.st_tma) {
@@ -550,10 +620,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThr
       }
       if (prof) busy += clk() - c1;
     }
-    if (EPI == EPI_FWD_STATS || p.st_tma) {
+    if (EPI != EPI_STORE || p.st_tma) {
       if (lane == 0) bulk_wait_all();  // staged stores complete before the shared memory goes away
     }
-    if constexpr (EPI != EPI_FWD_STATS) {
+    if constexpr (EPI == EPI_STORE) {
       // stores routed to other GPUs are visible system-wide once this kernel has finished
       if (p.st.peers > 0) __threadfence_system();
     }

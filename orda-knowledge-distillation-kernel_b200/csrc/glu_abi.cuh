@@ -1,0 +1,268 @@
+// Host side of the gated feed-forward block (include/orda_b200_student.h). Included by orda_abi.cu, whose
+// tensor-map and GEMM launch helpers it uses.
+#pragma once
+
+#include "glu.cuh"
+#include "orda_b200_student.h"
+
+namespace {
+
+// Rows up to which the weight-streaming kernel runs instead of the pair GEMM.
+constexpr int64_t kGluRowsMax = 32;
+
+int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
+
+int check_glu(const orda_glu_args_t* a, bool backward) {
+  if (!a || a->abi_version != ORDA_ABI_VERSION) return ORDA_ERR_INVALID_ARGUMENT;
+  if (a->dtype != ORDA_F32 && a->dtype != ORDA_F16 && a->dtype != ORDA_BF16) return ORDA_ERR_INVALID_ARGUMENT;
+  if (a->activation < ORDA_ACT_SILU || a->activation > ORDA_ACT_RELU) return ORDA_ERR_INVALID_ARGUMENT;
+  if (a->rows < 0 || a->hidden <= 0 || a->ffn <= 0) return ORDA_ERR_INVALID_ARGUMENT;
+  if (a->rows > (int64_t(1) << 31) - 1024 || a->hidden > (int64_t(1) << 30) || a->ffn > (int64_t(1) << 30))
+    return ORDA_ERR_UNSUPPORTED;  // tile coordinates are 32-bit
+  if (a->rows == 0) return ORDA_OK;
+  if (!a->x || !a->gate || !a->up || !a->device_status) return ORDA_ERR_INVALID_ARGUMENT;
+  if (a->ld_x < a->hidden || a->ld_gate < a->hidden || a->ld_up < a->hidden || a->ld_h < a->ffn)
+    return ORDA_ERR_INVALID_ARGUMENT;
+  if (backward) {
+    if (!a->pre_gate || !a->pre_up || !a->dh) return ORDA_ERR_INVALID_ARGUMENT;
+  } else if (!a->h || (a->pre_gate == nullptr) != (a->pre_up == nullptr)) {
+    return ORDA_ERR_INVALID_ARGUMENT;
+  }
+  auto off = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };
+  const int64_t unit = a->dtype == ORDA_F32 ? 1 : 8;
+  if (a->hidden % unit || a->ld_x % unit || a->ld_gate % unit || a->ld_up % unit || a->ld_h % 8)
+    return ORDA_ERR_ALIGNMENT;
+  if (off(a->x) || off(a->gate) || off(a->up) || off(a->h) || off(a->pre_gate) || off(a->pre_up) || off(a->dh) ||
+      off(a->dx) || off(a->dweights))
+    return ORDA_ERR_ALIGNMENT;
+  if (a->dtype == ORDA_F32 && !backward && !a->pre_gate) return ORDA_ERR_INVALID_ARGUMENT;  // its products need a place
+  return ORDA_OK;
+}
+
+template <typename T16>
+int glu_rows_launch(const orda_glu_args_t* a, cudaStream_t s) {
+  GluRowsParams p{};
+  p.x = a->x; p.gate = a->gate; p.up = a->up;
+  p.h = a->h; p.pre_gate = a->pre_gate; p.pre_up = a->pre_up;
+  p.ld_x = a->ld_x; p.ld_gate = a->ld_gate; p.ld_up = a->ld_up; p.ld_h = a->ld_h;
+  p.ffn = a->ffn;
+  p.rows = static_cast<int32_t>(a->rows); p.hidden = static_cast<int32_t>(a->hidden); p.act = a->activation;
+  const int grid = static_cast<int>(cdiv(a->ffn, kGluFeatures));
+  count_launch();
+  if (a->rows <= 8) glu_rows_kernel<T16, 1><<<grid, 32 * kGluWarps, 0, s>>>(p);
+  else if (a->rows <= 16) glu_rows_kernel<T16, 2><<<grid, 32 * kGluWarps, 0, s>>>(p);
+  else glu_rows_kernel<T16, 4><<<grid, 32 * kGluWarps, 0, s>>>(p);
+  return launch_status();
+}
+
+template <typename T16>
+int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
+  if (a->rows <= kGluRowsMax) return glu_rows_launch<T16>(a, s);
+  TcGemmParams prm{};
+  prm.status = a->device_status;
+  int rc;
+  if ((rc = make_operand_map(&prm.a0, a->dtype, a->x, false, a->rows, a->hidden, a->ld_x, kTileRows))) return rc;
+  if ((rc = make_operand_map(&prm.b0, a->dtype, a->gate, false, a->ffn, a->hidden, a->ld_gate, 128))) return rc;
+  if ((rc = make_operand_map(&prm.b1, a->dtype, a->up, false, a->ffn, a->hidden, a->ld_up, 128))) return rc;
+  if ((rc = make_map(&prm.out_map, a->dtype, a->h, a->ffn, a->rows, a->ld_h, 64, 32))) return rc;
+  prm.glu_act = a->activation;
+  prm.glu_save = a->pre_gate != nullptr;
+  if (prm.glu_save) {
+    if ((rc = make_map(&prm.ws_s_map, a->dtype, a->pre_gate, a->ffn, a->rows, a->ld_h, 64, 32))) return rc;
+    if ((rc = make_map(&prm.ws_t_map, a->dtype, a->pre_up, a->ffn, a->rows, a->ld_h, 64, 32))) return rc;
+  }
+  prm.kb0 = static_cast<int32_t>(cdiv(a->hidden, kBK));
+  prm.st.M = a->rows;
+  prm.st.N = a->ffn;
+  return launch_tc2w<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 512), 2 * round8(a->ffn), s, 4);
+}
+
+// K split of a gradient GEMM with M x N outputs and `kb` k blocks on the wide kernel: the split whose
+// estimated time is smallest, from the time of a wave (every CTA pair one tile), a wave's fixed cost and
+// the traffic of the fp32 partials (written once, read once).
+int glu_split(int64_t M, int64_t N, int64_t kb) {
+  const int64_t tiles = cdiv(M, 512) * cdiv(N, kPairBN);
+  const int64_t pairs = std::max(1, num_sms() / 2);
+  int best = 1;
+  double best_us = 0;
+  for (int sp = 1; sp <= 8 && sp <= kb; ++sp) {
+    if (sp > 1 && cdiv(kb, sp) * (sp - 1) >= kb) continue;  // a range would be empty
+    double us = static_cast<double>(cdiv(tiles * sp, pairs)) * (0.75 * cdiv(kb, sp) + 2.0);
+    if (sp > 1) us += 3.0 + 8.0 * sp * M * N / 5.0e6;
+    if (sp == 1 || us < best_us) {
+      best = sp;
+      best_us = us;
+    }
+  }
+  return best;
+}
+
+struct GluPlan {
+  int64_t fp;             // columns of dg (du follows): ffn rounded up to 8
+  int split_dx, split_dw;
+  size_t off_part, total;  // dg | du at 0
+};
+
+GluPlan plan_glu_backward(const orda_glu_args_t* a) {
+  GluPlan p{};
+  p.fp = round8(a->ffn);
+  p.split_dx = p.split_dw = 1;
+  size_t off = align256(esize(a->dtype) * 2 * p.fp * a->rows);
+  p.off_part = off;
+  if (a->dtype != ORDA_F32) {
+    size_t part = 0;
+    if (a->dx) {
+      p.split_dx = glu_split(a->rows, a->hidden, 2 * cdiv(a->ffn, kBK));
+      if (p.split_dx > 1) part = std::max(part, sizeof(float) * p.split_dx * a->rows * a->hidden);
+    }
+    if (a->dweights) {
+      p.split_dw = glu_split(p.fp + a->ffn, a->hidden, cdiv(a->rows, kBK));
+      if (p.split_dw > 1) part = std::max(part, sizeof(float) * p.split_dw * (p.fp + a->ffn) * a->hidden);
+    }
+    off = align256(off + part);
+  }
+  p.total = off;
+  return p;
+}
+
+// Destination of a gradient GEMM: `out` itself (TMA store where its rows are whole 64-column pieces), or
+// fp32 partials added in a fixed order by sum_split_kernel.
+template <bool A_MN, bool TWO_SEG, typename T16>
+int glu_grad_gemm(TcGemmParams& prm, int dtype, int64_t M, int64_t N, int split, void* out, uint8_t* part,
+                  cudaStream_t s) {
+  int rc;
+  if (split <= 1) {
+    prm.st = StoreEpiParams{out, N, M, N, 0, 0};
+    if (N % 64 == 0) {
+      if ((rc = make_map(&prm.out_map, dtype, out, N, M, N, 64, 32))) return rc;
+      prm.st_tma = 1;
+    }
+    return launch_tc2w<A_MN, true, A_PLAIN, TWO_SEG, EPI_STORE, T16>(prm, cdiv(M, 512), N, s, 4);
+  }
+  prm.ksplit = split;
+  prm.kb_split = static_cast<int32_t>(cdiv(prm.kb0 + prm.kb1, split));
+  prm.split_bytes = static_cast<int64_t>(sizeof(float)) * M * N;
+  prm.st = StoreEpiParams{part, N, M, N, 1, 0};
+  if ((rc = launch_tc2w<A_MN, true, A_PLAIN, TWO_SEG, EPI_STORE, T16>(prm, cdiv(M, 512), N, s, 4))) return rc;
+  const int64_t count8 = M * N / 8;
+  count_launch();
+  sum_split_kernel<T16><<<static_cast<int>(std::min<int64_t>(cdiv(count8, 256), 8 * num_sms())), 256, 0, s>>>(
+      reinterpret_cast<const float*>(part), split, M * N, static_cast<T16*>(out), count8);
+  return launch_status();
+}
+
+template <typename T>
+int glu_grad_launch(const orda_glu_args_t* a, const GluPlan& P, T* out, cudaStream_t s) {
+  const int64_t vecs = a->rows * (P.fp / 8);
+  const int grid = static_cast<int>(std::min<int64_t>(cdiv(vecs, 256), 16 * num_sms()));
+  count_launch();
+  glu_grad_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(a->dh), static_cast<const T*>(a->pre_gate),
+                                          static_cast<const T*>(a->pre_up), out, a->rows, a->ffn, P.fp, a->ld_h,
+                                          a->activation);
+  return launch_status();
+}
+
+template <typename T16>
+int glu_backward_tc(const orda_glu_args_t* a, const GluPlan& P, uint8_t* ws, cudaStream_t s) {
+  T16* dgu = reinterpret_cast<T16*>(ws);
+  uint8_t* part = ws + P.off_part;
+  const int64_t ld = 2 * P.fp;
+  int rc;
+  if ((rc = glu_grad_launch<T16>(a, P, dgu, s))) return rc;
+  if (a->dx) {  // [dg | du] [Wgate; Wup]: two K segments
+    TcGemmParams prm{};
+    prm.status = a->device_status;
+    if ((rc = make_operand_map(&prm.a0, a->dtype, dgu, false, a->rows, a->ffn, ld, kTileRows))) return rc;
+    if ((rc = make_operand_map(&prm.a1, a->dtype, dgu + P.fp, false, a->rows, a->ffn, ld, kTileRows))) return rc;
+    if ((rc = make_operand_map(&prm.b0, a->dtype, a->gate, true, a->hidden, a->ffn, a->ld_gate, 128))) return rc;
+    if ((rc = make_operand_map(&prm.b1, a->dtype, a->up, true, a->hidden, a->ffn, a->ld_up, 128))) return rc;
+    prm.kb0 = prm.kb1 = static_cast<int32_t>(cdiv(a->ffn, kBK));
+    if ((rc = glu_grad_gemm<false, true, T16>(prm, a->dtype, a->rows, a->hidden, P.split_dx, a->dx, part, s)))
+      return rc;
+  }
+  if (a->dweights) {  // [dg | du]^T x: both weights' gradients are one product of fp + ffn rows
+    TcGemmParams prm{};
+    prm.status = a->device_status;
+    const int64_t m = P.fp + a->ffn;
+    if ((rc = make_operand_map(&prm.a0, a->dtype, dgu, true, m, a->rows, ld, kTileRows))) return rc;
+    if ((rc = make_operand_map(&prm.b0, a->dtype, a->x, true, a->hidden, a->rows, a->ld_x, 128))) return rc;
+    prm.kb0 = static_cast<int32_t>(cdiv(a->rows, kBK));
+    if ((rc = glu_grad_gemm<true, false, T16>(prm, a->dtype, m, a->hidden, P.split_dw, a->dweights, part, s)))
+      return rc;
+  }
+  return ORDA_OK;
+}
+
+int glu_forward_f32(const orda_glu_args_t* a, cudaStream_t s) {
+  float* g = static_cast<float*>(a->pre_gate);
+  float* u = static_cast<float*>(a->pre_up);
+  const float* x = static_cast<const float*>(a->x);
+  simt_gemm(x, a->ld_x, 1, static_cast<const float*>(a->gate), a->ld_gate, 1, g, a->ld_h, a->rows, a->ffn, a->hidden, 0, s);
+  simt_gemm(x, a->ld_x, 1, static_cast<const float*>(a->up), a->ld_up, 1, u, a->ld_h, a->rows, a->ffn, a->hidden, 0, s);
+  count_launch();
+  glu_act_kernel<<<static_cast<int>(std::min<int64_t>(cdiv(a->rows * a->ffn, 256), 16 * num_sms())), 256, 0, s>>>(
+      g, u, static_cast<float*>(a->h), a->rows, a->ffn, a->ld_h, a->activation);
+  return launch_status();
+}
+
+int glu_backward_f32(const orda_glu_args_t* a, const GluPlan& P, uint8_t* ws, cudaStream_t s) {
+  float* dgu = reinterpret_cast<float*>(ws);
+  const int64_t ld = 2 * P.fp;
+  const int rc = glu_grad_launch<float>(a, P, dgu, s);
+  if (rc) return rc;
+  const float* x = static_cast<const float*>(a->x);
+  if (a->dx) {
+    float* dx = static_cast<float*>(a->dx);
+    simt_gemm(dgu, ld, 1, static_cast<const float*>(a->gate), 1, a->ld_gate, dx, a->hidden, a->rows, a->hidden, a->ffn, 0, s);
+    simt_gemm(dgu + P.fp, ld, 1, static_cast<const float*>(a->up), 1, a->ld_up, dx, a->hidden, a->rows, a->hidden, a->ffn, 1, s);
+  }
+  if (a->dweights) {
+    float* dw = static_cast<float*>(a->dweights);
+    simt_gemm(dgu, 1, ld, x, 1, a->ld_x, dw, a->hidden, P.fp + a->ffn, a->hidden, a->rows, 0, s);
+  }
+  return launch_status();
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t orda_glu_forward(const orda_glu_args_t* args, void* stream) {
+  const int rc = check_glu(args, false);
+  if (rc || args->rows == 0) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (args->dtype) {
+    case ORDA_BF16: return glu_forward_tc<__nv_bfloat16>(args, s);
+    case ORDA_F16: return glu_forward_tc<__half>(args, s);
+    default: return glu_forward_f32(args, s);
+  }
+}
+
+size_t orda_glu_backward_workspace_bytes(const orda_glu_args_t* args) {
+  if (check_glu(args, true) != ORDA_OK || args->rows == 0) return 0;
+  return plan_glu_backward(args).total;
+}
+
+int32_t orda_glu_backward(const orda_glu_args_t* args, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_glu(args, true);
+  if (rc) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (args->rows == 0) {
+    if (args->dweights &&
+        cudaMemsetAsync(args->dweights, 0, esize(args->dtype) * (round8(args->ffn) + args->ffn) * args->hidden, s) !=
+            cudaSuccess)
+      return ORDA_ERR_CUDA;
+    return ORDA_OK;
+  }
+  const GluPlan P = plan_glu_backward(args);
+  if (!workspace || workspace_bytes < P.total) return ORDA_ERR_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return ORDA_ERR_ALIGNMENT;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  switch (args->dtype) {
+    case ORDA_BF16: return glu_backward_tc<__nv_bfloat16>(args, P, ws, s);
+    case ORDA_F16: return glu_backward_tc<__half>(args, P, ws, s);
+    default: return glu_backward_f32(args, P, ws, s);
+  }
+}
+
+}  // extern "C"

@@ -20,6 +20,7 @@
 #include "gemm_tc.cuh"
 #include "gemm_tc2.cuh"
 #include "gemm_tc2w.cuh"
+#include "host_common.cuh"
 #include "orda_b200.h"
 #include "orda_b200_testing.h"
 #include "row_kernels.cuh"
@@ -28,9 +29,6 @@
 using namespace orda;
 
 namespace {
-
-std::atomic<uint64_t> g_launches{0};
-inline void count_launch(uint64_t n = 1) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -72,18 +70,6 @@ int make_operand_map(CUtensorMap* m, int dtype, const void* base, bool mn_major,
   if (mn_major) return make_map(m, dtype, base, mn, k, ld, 64, 64);
   return make_map(m, dtype, base, k, mn, ld, 64, tile_mn);
 }
-
-int num_sms() {
-  int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
-}
-
-
-size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-size_t esize(int dtype) { return dtype == ORDA_F32 ? 4 : 2; }
 
 // Bound of the default chunk's logits buffers: 2 GiB, so the logits of a whole Llama-3-8B-head batch
 // (8192 tokens x 128256 x 2 distributions x 2 B = 4.2 GB) are never held at once; the chunk is 4096
@@ -1211,3 +1197,6 @@ extern "C" int32_t orda_debug_gemm_wide(int32_t dtype, int32_t a_mn, int32_t b_m
   ORDA_DBGW(__half, false, false);
 #undef ORDA_DBGW
 }
+
+// ---------------------------------------------------------------- gated feed-forward block
+#include "glu_abi.cuh"

@@ -96,7 +96,54 @@ class IpcHandle(ctypes.Structure):
     _fields_ = [("handle", ctypes.c_uint8 * 64), ("offset", ctypes.c_uint64)]
 
 
-# every symbol include/orda_b200.h and include/orda_b200_testing.h declare
+# ---- include/orda_b200_student.h
+ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU = 0, 1, 2, 3
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+ROTARY_MAX_DIM = 512
+
+
+class GluArgs(ctypes.Structure):
+    """Mirror of orda_glu_args_t (include/orda_b200_student.h)."""
+
+    _fields_ = [
+        ("abi_version", _i32), ("dtype", _i32), ("activation", _i32), ("reserved", _i32),
+        ("rows", _i64), ("hidden", _i64), ("ffn", _i64),
+        ("x", _vp), ("ld_x", _i64), ("gate", _vp), ("ld_gate", _i64), ("up", _vp), ("ld_up", _i64),
+        ("h", _vp), ("ld_h", _i64), ("pre_gate", _vp), ("pre_up", _vp),
+        ("dh", _vp), ("dx", _vp), ("dweights", _vp),
+        ("device_status", _vp),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of orda_rotary_args_t (include/orda_b200_student.h)."""
+
+    _fields_ = [
+        ("abi_version", _i32), ("dtype", _i32),
+        ("batch", _i64), ("seq", _i64),
+        ("heads", _i32 * 2), ("head_dim", _i32), ("rotary_dim", _i32), ("layout", _i32), ("inverse", _i32),
+        ("x", _vp * 2), ("x_stride", _i64 * 6),
+        ("out", _vp * 2), ("out_stride", _i64 * 6),
+        ("dy", _vp * 2), ("dy_stride", _i64 * 6),
+        ("positions", _vp), ("position_stride", _i64 * 2),
+        ("positions_int64", _i32), ("weight_dtype", _i32),
+        ("frequencies", _vp),
+        ("magnitude", _f32), ("eps", _f32),
+        ("weight", _vp * 2), ("dweight", _vp * 2),
+    ]
+
+
+class TensorList(ctypes.Structure):
+    """Mirror of orda_tensor_list_t (include/orda_b200_student.h)."""
+
+    _fields_ = [
+        ("abi_version", _i32), ("count", _i32),
+        ("src", ctypes.POINTER(_vp)), ("dst", ctypes.POINTER(_vp)),
+        ("numel", ctypes.POINTER(_i64)), ("dtype", ctypes.POINTER(_i32)),
+    ]
+
+
+# every symbol include/orda_b200.h, include/orda_b200_student.h and include/orda_b200_testing.h declare
 EXPORTED_SYMBOLS = (
     "orda_abi_version",
     "orda_args_struct_size",
@@ -116,6 +163,14 @@ EXPORTED_SYMBOLS = (
     "orda_merge_row_stats",
     "orda_shard_jsd_partials",
     "orda_shard_backward",
+    "orda_glu_forward",
+    "orda_glu_backward_workspace_bytes",
+    "orda_glu_backward",
+    "orda_rotary_forward",
+    "orda_qk_norm_rotary_backward_workspace_bytes",
+    "orda_qk_norm_rotary_backward",
+    "orda_clip_workspace_bytes",
+    "orda_clip_gradients",
     "orda_debug_gemm",
     "orda_debug_gemm_pair",
     "orda_debug_gemm_profile",
@@ -168,6 +223,23 @@ def _declare(lib):
     lib.orda_shard_jsd_partials.argtypes = [P, _vp, ctypes.c_size_t, _vp, _vp, _vp]
     lib.orda_shard_backward.restype = _i32
     lib.orda_shard_backward.argtypes = [P, _vp, ctypes.c_size_t, _vp, _vp, _vp]
+    PG, PR, PT = ctypes.POINTER(GluArgs), ctypes.POINTER(RotaryArgs), ctypes.POINTER(TensorList)
+    lib.orda_glu_forward.restype = _i32
+    lib.orda_glu_forward.argtypes = [PG, _vp]
+    lib.orda_glu_backward_workspace_bytes.restype = ctypes.c_size_t
+    lib.orda_glu_backward_workspace_bytes.argtypes = [PG]
+    lib.orda_glu_backward.restype = _i32
+    lib.orda_glu_backward.argtypes = [PG, _vp, ctypes.c_size_t, _vp]
+    lib.orda_rotary_forward.restype = _i32
+    lib.orda_rotary_forward.argtypes = [PR, _vp]
+    lib.orda_qk_norm_rotary_backward_workspace_bytes.restype = ctypes.c_size_t
+    lib.orda_qk_norm_rotary_backward_workspace_bytes.argtypes = [PR]
+    lib.orda_qk_norm_rotary_backward.restype = _i32
+    lib.orda_qk_norm_rotary_backward.argtypes = [PR, _vp, ctypes.c_size_t, _vp]
+    lib.orda_clip_workspace_bytes.restype = ctypes.c_size_t
+    lib.orda_clip_workspace_bytes.argtypes = [PT]
+    lib.orda_clip_gradients.restype = _i32
+    lib.orda_clip_gradients.argtypes = [PT, ctypes.c_double, ctypes.c_double, _vp, _vp, ctypes.c_size_t, _vp]
     lib.orda_debug_gemm.restype = _i32
     lib.orda_debug_gemm.argtypes = [_i32, _i32, _i32, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp]
     lib.orda_debug_gemm_pair.restype = _i32
