@@ -25,6 +25,9 @@ extern "C" {
 #define ORDA_ACT_GELU_TANH 2  /* g / 2 (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3)))            */
 #define ORDA_ACT_RELU 3       /* max(g, 0), derivative 0 at 0                               */
 
+/* Up to this many rows the 16-bit forward call streams the weights without pipeline waits. */
+#define ORDA_GLU_FEW_ROWS 32
+
 typedef struct orda_glu_args {
   int32_t abi_version;   /* = ORDA_ABI_VERSION */
   int32_t dtype;         /* ORDA_F32 / ORDA_F16 / ORDA_BF16 of every tensor below            */
@@ -47,7 +50,8 @@ typedef struct orda_glu_args {
   void* dweights;                       /* [ceil8(F) + F, H] row stride hidden, or NULL: rows 0 .. F-1 the
                                            gradient of gate, rows ceil8(F) .. that of up; the rows
                                            between (at most 7) hold no value                 */
-  int32_t* device_status;               /* int32 device word, zero on entry                  */
+  int32_t* device_status;               /* int32 device word, zero on entry; may be NULL for ORDA_F32 and for
+                                           a forward call of at most ORDA_GLU_FEW_ROWS rows  */
 } orda_glu_args_t;
 
 /* h (and, where asked for, the products before the activation, which the backward pass reads). */

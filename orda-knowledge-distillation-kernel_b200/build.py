@@ -2,7 +2,10 @@
 
     python orda-knowledge-distillation-kernel_b200/build.py [--force]
 
-Rebuilds only when a source under csrc/ or include/ is newer than the library.
+and ``orda_ce_kernel/_student.so``, the Python binding of the student-step operators, with g++ against the
+installed torch.
+
+Rebuilds only when a source under csrc/ or include/ is newer than a library.
 """
 from __future__ import annotations
 
@@ -11,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -19,6 +23,7 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB_NAME = "liborda_b200.so"
 LIB = os.path.join(HERE, "orda_ce_kernel", LIB_NAME)
+BINDING = os.path.join(HERE, "orda_ce_kernel", "_student.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -37,14 +42,31 @@ def _nvcc() -> str:
 
 def sources() -> list[str]:
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))
-                  + glob.glob(os.path.join(INCLUDE, "*.h")))
+                  + glob.glob(os.path.join(CSRC, "*.cpp")) + glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(BINDING):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(BINDING))
     return any(os.path.getmtime(s) > t for s in sources())
+
+
+def _binding_flags() -> tuple[list[str], list[str]]:
+    """(compiler, linker) flags of the torch extension."""
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    paths = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    compile_flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_API_INCLUDE_EXTENSION_H",
+                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
+                     *[f for p in dict.fromkeys(paths) for f in ("-isystem", p)]]
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    link_flags = ["-L", torch_lib, "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-ltorch_python",
+                  "-L", os.path.join(cuda, "lib64"), "-lcudart", f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN",
+                  f"-Wl,-rpath,{torch_lib}"]
+    return compile_flags, link_flags
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -60,12 +82,21 @@ def build(force: bool = False, verbose: bool = False) -> str:
             if verbose:
                 print(" ".join(cmd))
             running.append((cmd, subprocess.Popen(cmd)))
+        compile_flags, link_flags = _binding_flags()
+        binding_object = os.path.join(tmp, "student_binding.o")
+        cmd = ["g++", *compile_flags, "-c", os.path.join(CSRC, "student_binding.cpp"), "-o", binding_object]
+        if verbose:
+            print(" ".join(cmd))
+        running.append((cmd, subprocess.Popen(cmd)))
         failed = [cmd for cmd, p in running if p.wait() != 0]
         if failed:
             raise subprocess.CalledProcessError(1, failed[0])
         lib = os.path.join(tmp, LIB_NAME)
         subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", lib, *objects], check=True)
+        binding = os.path.join(tmp, "_student.so")
+        subprocess.run(["g++", "-shared", "-o", binding, binding_object, "-L", tmp, *link_flags], check=True)
         os.replace(lib, LIB)
+        os.replace(binding, BINDING)
     return LIB
 
 

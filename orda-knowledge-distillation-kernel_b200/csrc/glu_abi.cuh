@@ -7,9 +7,6 @@
 
 namespace {
 
-// Rows up to which the weight-streaming kernel runs instead of the pair GEMM.
-constexpr int64_t kGluRowsMax = 32;
-
 int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
 
 int check_glu(const orda_glu_args_t* a, bool backward) {
@@ -20,7 +17,9 @@ int check_glu(const orda_glu_args_t* a, bool backward) {
   if (a->rows > (int64_t(1) << 31) - 1024 || a->hidden > (int64_t(1) << 30) || a->ffn > (int64_t(1) << 30))
     return ORDA_ERR_UNSUPPORTED;  // tile coordinates are 32-bit
   if (a->rows == 0) return ORDA_OK;
-  if (!a->x || !a->gate || !a->up || !a->device_status) return ORDA_ERR_INVALID_ARGUMENT;
+  if (!a->x || !a->gate || !a->up) return ORDA_ERR_INVALID_ARGUMENT;
+  if (!a->device_status && a->dtype != ORDA_F32 && (backward || a->rows > ORDA_GLU_FEW_ROWS))
+    return ORDA_ERR_INVALID_ARGUMENT;
   if (a->ld_x < a->hidden || a->ld_gate < a->hidden || a->ld_up < a->hidden || a->ld_h < a->ffn)
     return ORDA_ERR_INVALID_ARGUMENT;
   if (backward) {
@@ -57,7 +56,7 @@ int glu_rows_launch(const orda_glu_args_t* a, cudaStream_t s) {
 
 template <typename T16>
 int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
-  if (a->rows <= kGluRowsMax) return glu_rows_launch<T16>(a, s);
+  if (a->rows <= ORDA_GLU_FEW_ROWS) return glu_rows_launch<T16>(a, s);
   TcGemmParams prm{};
   prm.status = a->device_status;
   int rc;

@@ -164,7 +164,7 @@ def _glu(**kw):
     (dict(abi_version=9), _native.ERR_INVALID_ARGUMENT), (dict(dtype=5), _native.ERR_INVALID_ARGUMENT),
     (dict(activation=4), _native.ERR_INVALID_ARGUMENT), (dict(rows=-1), _native.ERR_INVALID_ARGUMENT),
     (dict(hidden=0), _native.ERR_INVALID_ARGUMENT), (dict(x=None), _native.ERR_INVALID_ARGUMENT),
-    (dict(h=None), _native.ERR_INVALID_ARGUMENT), (dict(pre_gate=16), _native.ERR_INVALID_ARGUMENT),
+    (dict(h=None), _native.ERR_INVALID_ARGUMENT), (dict(rows=33, device_status=None), _native.ERR_INVALID_ARGUMENT), (dict(pre_gate=16), _native.ERR_INVALID_ARGUMENT),
     (dict(ld_gate=8), _native.ERR_INVALID_ARGUMENT), (dict(x=24), _native.ERR_ALIGNMENT),
     (dict(hidden=12), _native.ERR_ALIGNMENT), (dict(ld_up=20), _native.ERR_ALIGNMENT),
     (dict(rows=1 << 31), _native.ERR_UNSUPPORTED), (dict(rows=0), _native.OK),
@@ -246,9 +246,9 @@ def test_c_clip_checks():
 def test_fake_shapes():
     with FakeTensorMode():
         x, w = torch.empty(6, 16, dtype=torch.bfloat16), torch.empty(13, 16, dtype=torch.bfloat16)
-        h, g, u = torch.ops.orda_b200.glu_forward(x, w, w, 0)
-        assert h.shape == (6, 13) and g.shape == u.shape == (6, 16) and h.dtype == torch.bfloat16
-        dx, dg, du = torch.ops.orda_b200.glu_backward(h, x, w, w, g, u, 0)
+        h, pre = torch.ops.orda_b200.glu_forward(x, w, w, 0)
+        assert h.shape == (6, 13) and pre.shape == (2, 6, 16) and h.dtype == torch.bfloat16
+        dx, dg, du = torch.ops.orda_b200.glu_backward(h, x, w, w, pre, 0)
         assert dx.shape == x.shape and dg.shape == du.shape == w.shape
         q, k, pos = torch.empty(2, 5, 4, 32), torch.empty(2, 5, 2, 32), torch.empty(2, 5, dtype=torch.long)
         cfg = student._config_values(student.RotaryConfig(32))
