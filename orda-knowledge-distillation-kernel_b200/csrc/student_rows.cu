@@ -99,15 +99,15 @@ RotaryPlan plan_rotary(const orda_rotary_args_t* a, bool backward) {
   while (p.lanes < slots && p.lanes < 32) p.lanes *= 2;
   const int at_once = 32 / p.lanes;
   const int64_t want = 16 * num_sms();  // warps
-  const int most = std::max(a->heads[0], a->heads[1]);
-  int hpu = static_cast<int>(cdiv(std::max(most, 1), at_once)) * at_once;
-  while (hpu > at_once && static_cast<int64_t>(p.tokens) * (cdiv(a->heads[0], hpu) + cdiv(a->heads[1], hpu)) < want)
+  const int first = backward ? a->heads[0] : a->heads[0] + a->heads[1], second = backward ? a->heads[1] : 0;
+  int hpu = static_cast<int>(cdiv(std::max({first, second, 1}), at_once)) * at_once;
+  while (hpu > at_once && static_cast<int64_t>(p.tokens) * (cdiv(first, hpu) + cdiv(second, hpu)) < want)
     hpu = static_cast<int>(cdiv(hpu / at_once, 2)) * at_once;
   p.heads_per_unit = hpu;
-  p.units[0] = static_cast<int32_t>(cdiv(a->heads[0], hpu));
-  p.units[1] = static_cast<int32_t>(cdiv(a->heads[1], hpu));
-  const int64_t units = static_cast<int64_t>(p.tokens) * (p.units[0] + p.units[1]);
-  r.grid = static_cast<int>(std::min<int64_t>(cdiv(units, kRotWarps), (backward ? 4 : 16) * num_sms()));
+  p.units[0] = static_cast<int32_t>(cdiv(first, hpu));
+  p.units[1] = static_cast<int32_t>(cdiv(second, hpu));
+  const int64_t units = static_cast<int64_t>(p.tokens) * std::max(p.units[0], p.units[1]);
+  r.grid = static_cast<int>(std::min<int64_t>(cdiv(units, kRotWarps), (backward ? 4 : 5) * num_sms()));
   return r;
 }
 
