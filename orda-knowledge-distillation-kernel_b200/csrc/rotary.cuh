@@ -7,14 +7,17 @@
 // n = x r, r = rsqrt(mean x^2 + eps), y = R(w n):
 //   dz = R^T dy,  dw = sum over heads and tokens of dz n,  e = w dz,  dx = r (e - n mean(e n)).
 //
-// Angles: theta_i / 2 pi is held in 64 bits, p times it is reduced to [-1/2, 1/2] turns in 64 bits
-// and only then rounded to 32, so the angle is off by less than 2e-7 rad at any position below 2^31
-// (a 32-bit product is already off by 0.06 rad at position 1e6). No table: a warp computes a token's
-// angles once for the heads that it turns.
+// Angles: theta_i / 2 pi is held as a 64-bit fraction of a turn, and the low 64 bits of its product with
+// the position are the angle modulo one turn, off by |p| 2^-65 turns plus the rounding of theta_i. The
+// top 32 of them go to fp32, so the angle is off by less than 2e-7 rad at any position below 2^31 (a
+// 32-bit float product is already off by 0.06 rad at position 1e6). No table and no fp64 arithmetic: a
+// warp computes a token's angles once for the heads that it turns.
 //
 // What bounds it: memory. Each head's values are read and written once, 16-byte vectors, and a lane's
 // cosines, sines and norm weights stay in registers over the heads of the token.
 #pragma once
+
+#include <type_traits>
 
 #include "distill_common.cuh"
 #include "orda_b200_student.h"
@@ -24,25 +27,44 @@ namespace orda {
 constexpr int kRotWarps = 4;                              // warps per block
 constexpr int kRotMaxPairs = ORDA_ROTARY_MAX_DIM / 2;
 
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery's round-up method).
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+
+inline FastDiv make_fast_div(uint32_t d) {
+  FastDiv f{d, 0, 0};
+  while ((uint64_t(1) << f.shift) < d) ++f.shift;
+  f.mul = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << f.shift) - d)) / d + 1);
+  return f;
+}
+
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv& f) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(__umulhi(n, f.mul)) + n) >> f.shift);
+}
+
 struct RotaryParams {
   const void* x[2];
   const void* dy[2];
   void* out[2];
   const void* w[2];
-  int64_t xs[2][3], os[2][3], ds[2][3];
+  int64_t xs[2][2], os[2][2], ds[2][2];  // element strides of batch and seq
+  int32_t xh[2], oh[2], dh[2];           // and of heads
   const void* pos;
   int64_t ps[2];
   float* dw_partial;              // [grid][2][D]
-  int32_t seq, tokens;
+  int32_t tokens;
+  FastDiv seq;
   int32_t heads[2];
-  int32_t units[2];               // work units of a token: groups of heads_per_unit heads. Forward: [0] over query
-                                  // and key heads together; backward: over the query heads, over the key heads
+  // Work units of a token: groups of heads_per_unit heads. Forward: [0] over query and key heads
+  // together; backward: over the query heads, over the key heads.
+  FastDiv units[2];
   int32_t heads_per_unit;
   int32_t head_dim, rotary_dim;
   int32_t lanes;                  // lanes per head: a power of two <= 32
-  int32_t pos64, interleaved, w_dtype;
-  float magnitude, sin_sign, eps;
-  double turns[kRotMaxPairs];     // theta_i / (2 pi)
+  int32_t pos64, w_dtype;
+  float magnitude, sin_sign, eps, inv_head_dim;
+  uint64_t turns[kRotMaxPairs];   // theta_i / (2 pi) modulo 1, times 2^64
 };
 
 __device__ __forceinline__ float load_weight(const void* w, int dtype, int i) {
@@ -51,34 +73,14 @@ __device__ __forceinline__ float load_weight(const void* w, int dtype, int i) {
   return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
 }
 
-// V consecutive elements as they lie in memory; the address is a multiple of V * sizeof(T) bytes (at
-// most 16). Kept packed so that a lane can have several heads in flight.
+// V consecutive elements as they lie in memory; their address is a multiple of V * sizeof(T) bytes (at
+// most 16).
 template <typename T, int V>
 struct Raw {
   static constexpr int kBytes = V * static_cast<int>(sizeof(T));
   static constexpr int kWords = kBytes >= 4 ? kBytes / 4 : 1;
   uint32_t w[kWords];
 
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = 0u;
-  }
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (kBytes >= 16) {
-#pragma unroll
-      for (int q = 0; q < kBytes / 16; ++q) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + q);
-        w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
-      }
-    } else if constexpr (kBytes == 8) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-      w[0] = u.x; w[1] = u.y;
-    } else if constexpr (kBytes == 4) {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-    } else {
-      w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
-    }
-  }
   __device__ __forceinline__ void unpack(float (&v)[V]) const {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -118,43 +120,190 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
   }
 }
 
-// Where a lane's slot (2 V elements of a head) lies: a rotated slot holds V whole pairs (half layout:
-// the first vector's elements with the second's; interleaved: neighbours), the slots behind rotary_dim
-// hold 2 V values that pass through.
+// Two floats of a register pair, for Blackwell's packed fp32 instructions: the kernels below would
+// otherwise be bound by instruction issue (300 a pass of four 128-element heads, at 70% of the issue
+// slots and half the memory rate).
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 pk(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpk(F2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 fma_v(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 mul_v(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float fma_v(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float mul_v(float a, float b) { return a * b; }
+
+// V floats as the packed (V = 1: single) registers that these work on
+template <int V>
+struct Vec {
+  static constexpr int N = V > 1 ? V / 2 : 1;
+  using E = std::conditional_t<(V > 1), F2, float>;
+  E e[N];
+
+  static __device__ __forceinline__ E all(float x) {
+    if constexpr (V > 1) return pk(x, x);
+    else return x;
+  }
+  __device__ __forceinline__ void fill(float x) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = all(x);
+  }
+  __device__ __forceinline__ float sum() const {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (V > 1) {
+        float a, b;
+        unpk(e[i], a, b);
+        t += a + b;
+      } else {
+        t += e[i];
+      }
+    }
+    return t;
+  }
+  __device__ __forceinline__ void get(float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (V > 1) unpk(e[i], v[2 * i], v[2 * i + 1]);
+      else v[0] = e[0];
+    }
+  }
+  __device__ __forceinline__ void set(const float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (V > 1) e[i] = pk(v[2 * i], v[2 * i + 1]);
+      else e[0] = v[0];
+    }
+  }
+};
+
+// Where a lane's slot (2 V elements of a head) lies: two vectors of V elements at a and b. A rotated
+// slot holds V whole pairs (u_i, v_i): in the half layout u is the first vector and v the second, in the
+// interleaved one u are the even and v the odd elements of both. The slots behind rotary_dim hold 2 V
+// values that pass through. In every case the lanes' first vectors lie side by side, and so do their
+// second ones: with a lane's two vectors side by side instead, each access used half of its 32-byte
+// sectors.
 template <int V>
 struct Slot {
-  int a, b;       // first element of the two V-vectors
+  int a, b;
   bool on, on_b;  // inside the head (V = 1 and an odd head size: the last slot has no b)
   bool turned;
 };
 
-template <int V>
+template <int V, bool IL>
 __device__ __forceinline__ Slot<V> slot_of(const RotaryParams& p, int s) {
   Slot<V> r;
   const int rotated = p.rotary_dim / (2 * V);
   r.turned = s < rotated;
   if (r.turned) {
-    r.a = p.interleaved ? s * 2 * V : s * V;
-    r.b = p.interleaved ? s * 2 * V + V : p.rotary_dim / 2 + s * V;
+    r.a = IL && V == 1 ? 2 * s : s * V;
+    r.b = IL && V == 1 ? 2 * s + 1 : p.rotary_dim / 2 + s * V;
   } else {
-    r.a = p.rotary_dim + (s - rotated) * 2 * V;
-    r.b = r.a + V;
+    r.a = p.rotary_dim + (s - rotated) * V;
+    r.b = r.a + (p.head_dim - p.rotary_dim + 1) / 2;
+    if (r.a >= p.rotary_dim + (p.head_dim - p.rotary_dim + 1) / 2) r.a = r.b = p.head_dim;
   }
   r.on = r.a < p.head_dim;
   r.on_b = r.b < p.head_dim;
   return r;
 }
 
-// Where a warp keeps the (cos, sin) of a token's pairs, and a block its norm weights, in shared memory:
-// the V of a slot as 16-byte pieces, piece k of every slot side by side, so that the lanes' 16-byte reads
-// of one piece are consecutive (64 bytes apart they would meet in the same banks four by four).
-template <int V>
-__device__ __forceinline__ int pair_at(int slots, int pair) {
-  if constexpr (V < 4) {
-    return pair;
+// Element of the head that u_i (side 0) or v_i (side 1) of a slot is.
+template <int V, bool IL>
+__device__ __forceinline__ int slot_element(const Slot<V>& s, int side, int i) {
+  if constexpr (IL && V > 1) {
+    const int k = 2 * i + side;
+    return k < V ? s.a + k : s.b + k - V;
+  }
+  return (side ? s.b : s.a) + i;
+}
+
+template <typename T, int V, bool IL>
+__device__ __forceinline__ void to_pairs(const Raw<T, V>& ra, const Raw<T, V>& rb, Vec<V>& u, Vec<V>& v) {
+  float a[V], b[V];
+  ra.unpack(a);
+  rb.unpack(b);
+  if constexpr (IL && V > 1) {
+    float x[V], y[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      x[i] = i < V / 2 ? a[2 * i] : b[2 * i - V];
+      y[i] = i < V / 2 ? a[2 * i + 1] : b[2 * i + 1 - V];
+    }
+    u.set(x);
+    v.set(y);
   } else {
-    const int s = pair / V, i = pair % V;
-    return ((i / 2) * slots + s) * 2 + i % 2;
+    u.set(a);
+    v.set(b);
+  }
+}
+
+template <typename T, int V, bool IL>
+__device__ __forceinline__ void store_pairs(T* out, const Slot<V>& s, bool live, const Vec<V>& u, const Vec<V>& v) {
+  float x[V], y[V];
+  u.get(x);
+  v.get(y);
+  if constexpr (IL && V > 1) {
+    float a[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      a[2 * i] = x[i];
+      a[2 * i + 1] = y[i];
+      b[2 * i] = x[V / 2 + i];
+      b[2 * i + 1] = y[V / 2 + i];
+    }
+    if (live && s.on) store_vec<T, V>(out + s.a, a);
+    if (live && s.on_b) store_vec<T, V>(out + s.b, b);
+  } else {
+    if (live && s.on) store_vec<T, V>(out + s.a, x);
+    if (live && s.on_b) store_vec<T, V>(out + s.b, y);
+  }
+}
+
+// Per-pair values (cosines, sines, norm weights) in shared memory: with 8-element slots, piece k (four
+// values) of every slot side by side, so that the lanes' 16-byte reads of one piece are consecutive
+// (32 bytes apart they would meet in the same banks two by two).
+template <int V>
+__device__ __forceinline__ int place_of(int slots, int s, int i) {
+  if constexpr (V < 8) return s * V + i;
+  else return (i / 4 * slots + s) * 4 + i % 4;
+}
+
+// The place of a rotated pair's values.
+template <int V, bool IL>
+__device__ __forceinline__ int pair_at(const RotaryParams& p, int pair) {
+  const int rotated = p.rotary_dim / (2 * V);
+  if constexpr (IL && V > 1) {
+    const int second = pair >= rotated * (V / 2);  // in the slot's second vector
+    const int k = pair - second * rotated * (V / 2);
+    return place_of<V>(rotated, k / (V / 2), k % (V / 2) + second * (V / 2));
+  }
+  return place_of<V>(rotated, pair / V, pair % V);
+}
+
+template <int V>
+__device__ __forceinline__ void load_pairs(const float* table, int slots, int s, Vec<V>& out) {
+  if constexpr (V == 8) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const ulonglong2 u = reinterpret_cast<const ulonglong2*>(table)[k * slots + s];
+      out.e[2 * k] = u.x;
+      out.e[2 * k + 1] = u.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < Vec<V>::N; ++i) out.e[i] = reinterpret_cast<const typename Vec<V>::E*>(table)[s * Vec<V>::N + i];
   }
 }
 
@@ -163,76 +312,68 @@ __device__ __forceinline__ int64_t token_position(const RotaryParams& p, int b, 
   return p.pos64 ? __ldg(static_cast<const long long*>(p.pos) + at) : __ldg(static_cast<const int32_t*>(p.pos) + at);
 }
 
-// The angles of one token, by its warp: magnitude * (cos, +-sin) of each pair.
-template <int V>
-__device__ __forceinline__ void token_angles(const RotaryParams& p, int64_t position, int lane, float2* cs) {
-  const double pos = static_cast<double>(position);
-  const int rotated = p.rotary_dim / (2 * V);
+// A token's angles, formed by its warp: magnitude times cosine, sine and negative sine of each pair.
+struct TokenAngles {
+  float cos[kRotMaxPairs], sin[kRotMaxPairs], neg_sin[kRotMaxPairs];
+};
+
+// `turns`: the block's copy of p.turns (lanes that read different constants wait for one another).
+template <int V, bool IL>
+__device__ __forceinline__ void token_angles(const RotaryParams& p, const uint64_t* turns, int64_t position, int lane,
+                                             TokenAngles& out) {
   for (int i = lane; i < p.rotary_dim / 2; i += 32) {
-    double turn = pos * p.turns[i];
-    turn -= rint(turn);
+    const uint64_t turn = static_cast<uint64_t>(position) * turns[i];
     float s, c;
-    sincospif(2.f * static_cast<float>(turn), &s, &c);
-    cs[pair_at<V>(rotated, i)] = make_float2(p.magnitude * c, p.magnitude * p.sin_sign * s);
+    // the top 32 bits as a signed number: units of 2^-31 half turns
+    sincospif(static_cast<float>(static_cast<int32_t>(turn >> 32)) * 4.656612873077393e-10f, &s, &c);
+    s *= p.magnitude * p.sin_sign;
+    const int at = pair_at<V, IL>(p, i);
+    out.cos[at] = p.magnitude * c;
+    out.sin[at] = s;
+    out.neg_sin[at] = -s;
   }
   __syncwarp();
 }
 
-// The (cos, sin) of slot s, (1, 0) where the slot passes through.
+// The angles of slot s; (1, 0) where the slot passes through.
 template <int V>
-__device__ __forceinline__ void slot_angles(const RotaryParams& p, const float2* cs, int s, bool turned,
-                                            float2 (&out)[V]) {
-  const int rotated = p.rotary_dim / (2 * V);
-  if constexpr (V < 4) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = turned ? cs[s * V + i] : make_float2(1.f, 0.f);
-  } else {
-#pragma unroll
-    for (int k = 0; k < V / 2; ++k) {
-      const float4 u = turned ? reinterpret_cast<const float4*>(cs)[k * rotated + s] : make_float4(1.f, 0.f, 1.f, 0.f);
-      out[2 * k] = make_float2(u.x, u.y);
-      out[2 * k + 1] = make_float2(u.z, u.w);
+struct SlotAngles {
+  Vec<V> cos, sin, neg_sin;
+
+  __device__ __forceinline__ void load(const RotaryParams& p, const TokenAngles& t, int s, bool turned) {
+    if (turned) {
+      const int rotated = p.rotary_dim / (2 * V);
+      load_pairs<V>(t.cos, rotated, s, cos);
+      load_pairs<V>(t.sin, rotated, s, sin);
+      load_pairs<V>(t.neg_sin, rotated, s, neg_sin);
+    } else {
+      cos.fill(1.f);
+      sin.fill(0.f);
+      neg_sin.fill(0.f);
     }
   }
-}
-
-// (weight of a, weight of b) of slot s
-template <int V>
-__device__ __forceinline__ void slot_weights(const float2* w_s, int slots, int s, float2 (&out)[V]) {
-  if constexpr (V < 4) {
+  __device__ __forceinline__ void turn(Vec<V>& u, Vec<V>& v) const {
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = w_s[s * V + i];
-  } else {
-#pragma unroll
-    for (int k = 0; k < V / 2; ++k) {
-      const float4 u = reinterpret_cast<const float4*>(w_s)[k * slots + s];
-      out[2 * k] = make_float2(u.x, u.y);
-      out[2 * k + 1] = make_float2(u.z, u.w);
+    for (int i = 0; i < Vec<V>::N; ++i) {
+      const auto x = fma_v(u.e[i], cos.e[i], mul_v(v.e[i], neg_sin.e[i]));
+      v.e[i] = fma_v(v.e[i], cos.e[i], mul_v(u.e[i], sin.e[i]));
+      u.e[i] = x;
     }
   }
-}
+};
 
-// One slot turned in place by the (cos, sin) of its V pairs.
-template <int V>
-__device__ __forceinline__ void turn_slot(float (&a)[V], float (&b)[V], const float2 (&cs)[V], bool interleaved) {
-  if (V == 1 || !interleaved) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float ya = a[i] * cs[i].x - b[i] * cs[i].y;
-      b[i] = b[i] * cs[i].x + a[i] * cs[i].y;
-      a[i] = ya;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      const float2 c1 = cs[i], c2 = cs[V / 2 + i];
-      const float ya = a[2 * i] * c1.x - a[2 * i + 1] * c1.y;
-      a[2 * i + 1] = a[2 * i + 1] * c1.x + a[2 * i] * c1.y;
-      a[2 * i] = ya;
-      const float yb = b[2 * i] * c2.x - b[2 * i + 1] * c2.y;
-      b[2 * i + 1] = b[2 * i + 1] * c2.x + b[2 * i] * c2.y;
-      b[2 * i] = yb;
-    }
+// The norm weights of a head in pair order, zero outside the head.
+struct PairWeights {
+  float u[kRotMaxPairs], v[kRotMaxPairs];
+};
+
+template <int V, bool IL>
+__device__ __forceinline__ void load_pair_weights(const RotaryParams& p, int which, int slots, PairWeights& out) {
+  for (int i = threadIdx.x; i < slots * V; i += blockDim.x) {
+    const Slot<V> s = slot_of<V, IL>(p, i / V);
+    const int eu = slot_element<V, IL>(s, 0, i % V), ev = slot_element<V, IL>(s, 1, i % V);
+    out.u[place_of<V>(slots, i / V, i % V)] = eu < p.head_dim ? load_weight(p.w[which], p.w_dtype, eu) : 0.f;
+    out.v[place_of<V>(slots, i / V, i % V)] = ev < p.head_dim ? load_weight(p.w[which], p.w_dtype, ev) : 0.f;
   }
 }
 
@@ -247,294 +388,389 @@ constexpr int rotary_slots_per_lane() {
   return kRotMaxPairs / (32 * V);
 }
 
-// Where a warp stands: a unit (a token's group of heads) and the pass over its heads, at_once heads a pass.
-// Both kernels load the values of the next pass, of the next unit if need be, before they work on the
-// current one: a warp always has a pass in flight, and a token's angles are formed while its first
-// values arrive.
-struct RotaryStep {
-  int64_t unit;
-  int head;         // first head of the pass
-  int end;          // behind the unit's last head
-  int64_t xq, xk;   // element offset of the token in the two inputs
-  int64_t position;
-  int b, t;
+// Both kernels walk units (a token's group of heads) in passes of at_once heads, and fetch the values of
+// the next passes, of the next units if need be, while they work on the current one. Four KB a warp are
+// on their way at any time: with one pass of register loads ahead (1 KB) the reads stopped at 2.3 TB/s,
+// waiting for a memory latency of about 1 us under load. The fetched bytes go to shared memory by
+// cp.async, each lane reads back only what it fetched itself, so no lane waits for another.
+template <typename T, int V, int VECTORS>  // VECTORS: V-element vectors of a lane in a pass
+struct PassRing {
+  static constexpr int kBytes = V * static_cast<int>(sizeof(T));
+  static constexpr int kPass = VECTORS * 32 * (kBytes < 4 ? 4 : kBytes);
+  static constexpr int kStages = kPass >= 2048 ? 2 : kPass >= 1536 ? 3 : 4;
+  static constexpr bool kAsync = kBytes >= 4;  // cp.async moves at least 4 bytes
+  static constexpr int kWords = kBytes >= 16 ? 4 : kBytes >= 4 ? kBytes / 4 : 1;  // of one access
+  static constexpr int kParts = kBytes > 16 ? kBytes / 16 : 1;                    // accesses of a vector
+  uint32_t w[kStages][VECTORS][kParts][32][kWords];
+
+  __device__ __forceinline__ void clear(int v, int lane) {
+    for (int s = 0; s < kStages; ++s)
+      for (int q = 0; q < kParts; ++q)
+        for (int k = 0; k < kWords; ++k) w[s][v][q][lane][k] = 0u;
+  }
+  __device__ __forceinline__ void fetch(int stage, int v, int lane, const T* p) {
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+      uint32_t* dst = w[stage][v][q][lane];
+      if constexpr (kBytes >= 16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                     "l"(reinterpret_cast<const uint4*>(p) + q)
+                     : "memory");
+      } else if constexpr (kAsync) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+                         static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                     "l"(p), "n"(kBytes)
+                     : "memory");
+      } else {
+        dst[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+      }
+    }
+  }
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  // all but the newest kStages - 1 fetches have arrived
+  static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
+  __device__ __forceinline__ Raw<T, V> get(int stage, int v, int lane) const {
+    Raw<T, V> r;
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+      if constexpr (kWords == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(w[stage][v][q][lane]);
+        r.w[4 * q] = u.x; r.w[4 * q + 1] = u.y; r.w[4 * q + 2] = u.z; r.w[4 * q + 3] = u.w;
+      } else if constexpr (kWords == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(w[stage][v][q][lane]);
+        r.w[0] = u.x; r.w[1] = u.y;
+      } else {
+        r.w[0] = w[stage][v][q][lane][0];
+      }
+    }
+    return r;
+  }
 };
 
-template <typename T, int V, bool NORM>
-__global__ void __launch_bounds__(32 * kRotWarps) rotary_forward_kernel(const __grid_constant__ RotaryParams p) {
+// A place in the walk: the token and the heads [head, end) left of the unit.
+struct RotaryCursor {
+  uint32_t unit;
+  int b, t, head, end;
+
+  __device__ __forceinline__ void begin(const RotaryParams& p, const FastDiv& units, int heads, uint32_t u) {
+    unit = u;
+    const uint32_t token = fast_div(u, units);
+    b = static_cast<int>(fast_div(token, p.seq));
+    t = static_cast<int>(token) - b * static_cast<int>(p.seq.d);
+    head = static_cast<int>(u - token * units.d) * p.heads_per_unit;
+    end = min(heads, head + p.heads_per_unit);
+  }
+};
+
+__device__ __forceinline__ int64_t unit_position(const RotaryParams& p, const FastDiv& units, uint32_t u) {
+  const uint32_t token = fast_div(u, units);
+  const int b = static_cast<int>(fast_div(token, p.seq));
+  return token_position(p, b, static_cast<int>(token) - b * static_cast<int>(p.seq.d));
+}
+
+template <typename T, int V, bool NORM, bool IL>
+__global__ void __launch_bounds__(32 * kRotWarps, 5) rotary_forward_kernel(const __grid_constant__ RotaryParams p) {
   constexpr int NS = rotary_slots_per_lane<V>();
-  __shared__ __align__(16) float2 cs_all[kRotWarps][kRotMaxPairs];
-  __shared__ __align__(16) float2 w_s[NORM ? 2 : 1][NORM ? kRotMaxPairs : 1];  // (of a, of b) of each slot
+  using Ring = PassRing<T, V, 2 * NS>;
+  __shared__ __align__(16) Ring ring_all[kRotWarps];
+  __shared__ __align__(16) TokenAngles angles_all[kRotWarps];
+  __shared__ uint64_t turns[kRotMaxPairs];
+  __shared__ __align__(16) PairWeights weights[NORM ? 2 : 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  float2* cs_token = cs_all[warp];
+  Ring& ring = ring_all[warp];
+  TokenAngles& angles = angles_all[warp];
+  for (int i = threadIdx.x; i < p.rotary_dim / 2; i += blockDim.x) turns[i] = p.turns[i];
   const int heads = p.heads[0] + p.heads[1];
-  const int64_t total = static_cast<int64_t>(p.tokens) * p.units[0];
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kRotWarps;
+  const uint32_t total = static_cast<uint32_t>(p.tokens) * p.units[0].d;  // below 2^31: checked by the host
+  const uint32_t stride = gridDim.x * kRotWarps;
   const int sub = lane / p.lanes, sl = lane % p.lanes, at_once = 32 / p.lanes;
   const int slots = NS * p.lanes;
   Slot<V> slot[NS];
 #pragma unroll
-  for (int n = 0; n < NS; ++n) slot[n] = slot_of<V>(p, sl + n * p.lanes);
-  if constexpr (NORM) {
-    for (int i = threadIdx.x; i < slots * V; i += blockDim.x) {
-      const Slot<V> q = slot_of<V>(p, i / V);
-      const int e = i % V;
-#pragma unroll
-      for (int w = 0; w < 2; ++w)
-        w_s[w][pair_at<V>(slots, i)] = make_float2(q.on ? load_weight(p.w[w], p.w_dtype, q.a + e) : 0.f,
-                                                   q.on_b ? load_weight(p.w[w], p.w_dtype, q.b + e) : 0.f);
-    }
-    __syncthreads();
+  for (int n = 0; n < NS; ++n) {
+    slot[n] = slot_of<V, IL>(p, sl + n * p.lanes);
+    // a vector that lies outside the head counts as zeros
+    if (!slot[n].on) ring.clear(2 * n, lane);
+    if (!slot[n].on_b) ring.clear(2 * n + 1, lane);
   }
-  auto begin = [&](int64_t unit) {
-    RotaryStep st;
-    st.unit = unit;
-    const int token = static_cast<int>(unit / p.units[0]);
-    const int g = static_cast<int>(unit - static_cast<int64_t>(token) * p.units[0]);
-    st.b = token / p.seq;
-    st.t = token - st.b * p.seq;
-    st.head = g * p.heads_per_unit;
-    st.end = min(heads, st.head + p.heads_per_unit);
-    st.xq = st.b * p.xs[0][0] + st.t * p.xs[0][1];
-    st.xk = st.b * p.xs[1][0] + st.t * p.xs[1][1];
-    st.position = token_position(p, st.b, st.t);
-    return st;
+  if constexpr (NORM) {
+    load_pair_weights<V, IL>(p, 0, slots, weights[0]);
+    load_pair_weights<V, IL>(p, 1, slots, weights[1]);
+  }
+  __syncthreads();
+  const uint32_t first = blockIdx.x * kRotWarps + warp;
+  if (first >= total) return;
+
+  RotaryCursor in, at;  // of the fetches, of the work
+  const T *xq = nullptr, *xk = nullptr;
+  bool more_in = true;
+  auto begin_in = [&](uint32_t u) {
+    in.begin(p, p.units[0], heads, u);
+    xq = static_cast<const T*>(p.x[0]) + in.b * p.xs[0][0] + in.t * p.xs[0][1];
+    xk = static_cast<const T*>(p.x[1]) + in.b * p.xs[1][0] + in.t * p.xs[1][1];
   };
-  Raw<T, V> ra[NS], rb[NS];
-  auto fetch = [&](const RotaryStep& st) {
-    const int h = st.head + sub;
-    const bool key = h >= p.heads[0];
-    const T* x = key ? static_cast<const T*>(p.x[1]) + st.xk + (h - p.heads[0]) * p.xs[1][2]
-                     : static_cast<const T*>(p.x[0]) + st.xq + h * p.xs[0][2];
+  auto fetch = [&](int stage) {
+    if (more_in) {
+      const int h = in.head + sub;
+      const bool key = h >= p.heads[0];
+      const T* x = (key ? xk : xq) + static_cast<int64_t>(key ? h - p.heads[0] : h) * (key ? p.xh[1] : p.xh[0]);
+      if (h < in.end) {  // a lane whose head is behind the unit's keeps older values, which go nowhere
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      ra[n].clear();
-      rb[n].clear();
-      if (h < st.end && slot[n].on) ra[n].load(x + slot[n].a);
-      if (h < st.end && slot[n].on_b) rb[n].load(x + slot[n].b);
-    }
-  };
-  int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + warp;
-  if (unit >= total) return;
-  RotaryStep next = begin(unit);
-  fetch(next);
-  float2 cs[NS][V];
-  bool fresh = true;  // the pass is its unit's first
-  while (true) {
-    const RotaryStep st = next;
-    Raw<T, V> ca[NS], cb[NS];
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      ca[n] = ra[n];
-      cb[n] = rb[n];
-    }
-    const bool same = st.head + at_once < st.end;
-    const bool more = same || st.unit + stride < total;
-    if (same) next.head += at_once;
-    else if (more) next = begin(st.unit + stride);
-    if (more) fetch(next);
-    if (fresh) {
-      __syncwarp();  // the previous unit's angles have been read
-      token_angles<V>(p, st.position, lane, cs_token);
-#pragma unroll
-      for (int n = 0; n < NS; ++n) slot_angles<V>(p, cs_token, sl + n * p.lanes, slot[n].turned, cs[n]);
-    }
-    const int h = st.head + sub;
-    const bool live = h < st.end, key = h >= p.heads[0];
-    T* out = key ? static_cast<T*>(p.out[1]) + st.b * p.os[1][0] + st.t * p.os[1][1] + (h - p.heads[0]) * p.os[1][2]
-                 : static_cast<T*>(p.out[0]) + st.b * p.os[0][0] + st.t * p.os[0][1] + h * p.os[0][2];
-    float va[NS][V], vb[NS][V];
-    float ss = 0.f;
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      ca[n].unpack(va[n]);
-      cb[n].unpack(vb[n]);
-      if constexpr (NORM) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) ss += va[n][i] * va[n][i] + vb[n][i] * vb[n][i];
-      }
-    }
-    float r = 1.f;
-    if constexpr (NORM) r = rsqrtf(group_sum(ss, p.lanes) / p.head_dim + p.eps);
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      if constexpr (NORM) {
-        float2 w[V];
-        slot_weights<V>(w_s[key], slots, sl + n * p.lanes, w);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          va[n][i] *= r * w[i].x;
-          vb[n][i] *= r * w[i].y;
+        for (int n = 0; n < NS; ++n) {
+          if (slot[n].on) ring.fetch(stage, 2 * n, lane, x + slot[n].a);
+          if (slot[n].on_b) ring.fetch(stage, 2 * n + 1, lane, x + slot[n].b);
         }
       }
-      turn_slot<V>(va[n], vb[n], cs[n], p.interleaved != 0);
-      if (live && slot[n].on) store_vec<T, V>(out + slot[n].a, va[n]);
-      if (live && slot[n].on_b) store_vec<T, V>(out + slot[n].b, vb[n]);
+      in.head += at_once;
+      if (in.head >= in.end) {
+        more_in = in.unit + stride < total;
+        if (more_in) begin_in(in.unit + stride);
+      }
     }
-    if (!more) break;
-    fresh = !same;
+    Ring::commit();
+  };
+  begin_in(first);
+#pragma unroll
+  for (int s = 0; s < Ring::kStages - 1; ++s) fetch(s);
+  at.begin(p, p.units[0], heads, first);
+  int64_t position = unit_position(p, p.units[0], first);
+  SlotAngles<V> sa[NS];
+  T *oq = nullptr, *ok = nullptr;
+  bool fresh = true;  // the pass is its unit's first
+  for (int stage = 0;; stage = stage + 1 == Ring::kStages ? 0 : stage + 1) {
+    fetch(stage == 0 ? Ring::kStages - 1 : stage - 1);
+    if (fresh) {
+      oq = static_cast<T*>(p.out[0]) + at.b * p.os[0][0] + at.t * p.os[0][1];
+      ok = static_cast<T*>(p.out[1]) + at.b * p.os[1][0] + at.t * p.os[1][1];
+      __syncwarp();  // the previous unit's angles have been read
+      token_angles<V, IL>(p, turns, position, lane, angles);
+#pragma unroll
+      for (int n = 0; n < NS; ++n) sa[n].load(p, angles, sl + n * p.lanes, slot[n].turned);
+      // the next unit's position, wanted when this one is done
+      if (at.unit + stride < total) position = unit_position(p, p.units[0], at.unit + stride);
+    }
+    Ring::wait();
+    Vec<V> u[NS], v[NS];
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+      to_pairs<T, V, IL>(ring.get(stage, 2 * n, lane), ring.get(stage, 2 * n + 1, lane), u[n], v[n]);
+    const int h = at.head + sub;
+    const bool live = h < at.end, key = h >= p.heads[0];
+    T* out = (key ? ok : oq) + static_cast<int64_t>(key ? h - p.heads[0] : h) * (key ? p.oh[1] : p.oh[0]);
+    typename Vec<V>::E r = Vec<V>::all(1.f);
+    if constexpr (NORM) {
+      Vec<V> ss;
+      ss.fill(0.f);
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int i = 0; i < Vec<V>::N; ++i) ss.e[i] = fma_v(v[n].e[i], v[n].e[i], fma_v(u[n].e[i], u[n].e[i], ss.e[i]));
+      r = Vec<V>::all(rsqrtf(group_sum(ss.sum(), p.lanes) * p.inv_head_dim + p.eps));
+    }
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      if constexpr (NORM) {
+        Vec<V> wu, wv;
+        load_pairs<V>(weights[key].u, slots, sl + n * p.lanes, wu);
+        load_pairs<V>(weights[key].v, slots, sl + n * p.lanes, wv);
+#pragma unroll
+        for (int i = 0; i < Vec<V>::N; ++i) {
+          u[n].e[i] = mul_v(mul_v(u[n].e[i], r), wu.e[i]);
+          v[n].e[i] = mul_v(mul_v(v[n].e[i], r), wv.e[i]);
+        }
+      }
+      sa[n].turn(u[n], v[n]);
+      store_pairs<T, V, IL>(out, slot[n], live, u[n], v[n]);
+    }
+    at.head += at_once;
+    fresh = at.head >= at.end;
+    if (fresh) {
+      if (at.unit + stride >= total) break;
+      at.begin(p, p.units[0], heads, at.unit + stride);
+    }
   }
 }
 
 // Backward of the normed form. Each lane adds up the weight gradients of its elements over every head
 // it meets, the block adds its warps' and head groups' sums in a fixed order and writes one partial row;
 // norm_weight_grad_kernel adds the blocks' rows, again in a fixed order: the same inputs give the same
-// bits. Cosines, sines and weights stay in shared memory: in registers they would leave room for half
-// as many warps.
-template <typename T, int V>
+// bits. Angles and weights stay in shared memory: in registers they would leave room for half as many
+// warps.
+template <typename T, int V, bool IL>
 __global__ void __launch_bounds__(32 * kRotWarps, 4)
     qk_norm_rotary_backward_kernel(const __grid_constant__ RotaryParams p) {
   constexpr int NS = rotary_slots_per_lane<V>();
-  __shared__ __align__(16) float2 cs_all[kRotWarps][kRotMaxPairs];
-  __shared__ __align__(16) float2 w_s[kRotMaxPairs];  // (weight of a, weight of b) of each slot
-  __shared__ float dw_s[kRotWarps][ORDA_ROTARY_MAX_DIM];
+  using Ring = PassRing<T, V, 4 * NS>;  // vector 4 n: x's a, + 1: x's b, + 2, + 3: dy's
+  union Shared {
+    Ring ring[kRotWarps];
+    float dw[kRotWarps][ORDA_ROTARY_MAX_DIM];
+  };
+  __shared__ __align__(16) Shared sh;
+  __shared__ __align__(16) TokenAngles angles_all[kRotWarps];
+  __shared__ __align__(16) PairWeights weights;
+  __shared__ uint64_t turns[kRotMaxPairs];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  float2* cs_token = cs_all[warp];
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kRotWarps;
+  Ring& ring = sh.ring[warp];
+  TokenAngles& angles = angles_all[warp];
+  for (int i = threadIdx.x; i < p.rotary_dim / 2; i += blockDim.x) turns[i] = p.turns[i];
+  const uint32_t stride = gridDim.x * kRotWarps, first = blockIdx.x * kRotWarps + warp;
   const int sub = lane / p.lanes, sl = lane % p.lanes, at_once = 32 / p.lanes;
   const int slots = NS * p.lanes;
   Slot<V> slot[NS];
 #pragma unroll
-  for (int n = 0; n < NS; ++n) slot[n] = slot_of<V>(p, sl + n * p.lanes);
+  for (int n = 0; n < NS; ++n) slot[n] = slot_of<V, IL>(p, sl + n * p.lanes);
+#pragma unroll 1
   for (int which = 0; which < 2; ++which) {
     __syncthreads();  // the previous weights and sums have been read
-    for (int i = threadIdx.x; i < slots * V; i += blockDim.x) {
-      const Slot<V> q = slot_of<V>(p, i / V);
-      const int e = i % V;
-      w_s[pair_at<V>(slots, i)] = make_float2(q.on ? load_weight(p.w[which], p.w_dtype, q.a + e) : 0.f,
-                                              q.on_b ? load_weight(p.w[which], p.w_dtype, q.b + e) : 0.f);
-    }
-    __syncthreads();
-    const int64_t total = static_cast<int64_t>(p.tokens) * p.units[which];
-    float dwa[NS][V], dwb[NS][V];
 #pragma unroll
     for (int n = 0; n < NS; ++n)
 #pragma unroll
-      for (int i = 0; i < V; ++i) dwa[n][i] = dwb[n][i] = 0.f;
-    auto begin = [&](int64_t unit) {
-      RotaryStep st;
-      st.unit = unit;
-      const int token = static_cast<int>(unit / p.units[which]);
-      const int g = static_cast<int>(unit - static_cast<int64_t>(token) * p.units[which]);
-      st.b = token / p.seq;
-      st.t = token - st.b * p.seq;
-      st.head = g * p.heads_per_unit;
-      st.end = min(p.heads[which], st.head + p.heads_per_unit);
-      st.xq = st.b * p.xs[which][0] + st.t * p.xs[which][1];
-      st.xk = st.b * p.ds[which][0] + st.t * p.ds[which][1];  // (of dy)
-      st.position = token_position(p, st.b, st.t);
-      return st;
-    };
-    Raw<T, V> rx[NS][2], rz[NS][2];
-    auto fetch = [&](const RotaryStep& st) {
-      const int h = st.head + sub;
-      const T* x = static_cast<const T*>(p.x[which]) + st.xq + h * p.xs[which][2];
-      const T* z = static_cast<const T*>(p.dy[which]) + st.xk + h * p.ds[which][2];
-#pragma unroll
-      for (int n = 0; n < NS; ++n) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          rx[n][j].clear();
-          rz[n][j].clear();
-        }
-        if (h < st.end && slot[n].on) {
-          rx[n][0].load(x + slot[n].a);
-          rz[n][0].load(z + slot[n].a);
-        }
-        if (h < st.end && slot[n].on_b) {
-          rx[n][1].load(x + slot[n].b);
-          rz[n][1].load(z + slot[n].b);
-        }
+      for (int j = 0; j < 2; ++j) {
+        if (!slot[n].on) ring.clear(4 * n + 2 * j, lane);
+        if (!slot[n].on_b) ring.clear(4 * n + 2 * j + 1, lane);
       }
-    };
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + warp;
-    RotaryStep next{};
-    bool more = unit < total, fresh = true;
-    if (more) {
-      next = begin(unit);
-      fetch(next);
+    load_pair_weights<V, IL>(p, which, slots, weights);
+    __syncthreads();
+    const uint32_t total = static_cast<uint32_t>(p.tokens) * p.units[which].d;
+    Vec<V> dwu[NS], dwv[NS];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      dwu[n].fill(0.f);
+      dwv[n].fill(0.f);
     }
-    while (more) {
-      const RotaryStep st = next;
-      Raw<T, V> cx[NS][2], cz[NS][2];
+    if (first < total && p.heads[which] > 0) {
+      RotaryCursor in, at;
+      const T *x = nullptr, *dy = nullptr;
+      bool more_in = true;
+      auto begin_in = [&](uint32_t u) {
+        in.begin(p, p.units[which], p.heads[which], u);
+        x = static_cast<const T*>(p.x[which]) + in.b * p.xs[which][0] + in.t * p.xs[which][1];
+        dy = static_cast<const T*>(p.dy[which]) + in.b * p.ds[which][0] + in.t * p.ds[which][1];
+      };
+      auto fetch = [&](int stage) {
+        if (more_in) {
+          const int h = in.head + sub;
+          if (h < in.end) {
+            const T* xh = x + static_cast<int64_t>(h) * p.xh[which];
+            const T* zh = dy + static_cast<int64_t>(h) * p.dh[which];
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          cx[n][j] = rx[n][j];
-          cz[n][j] = rz[n][j];
+            for (int n = 0; n < NS; ++n) {
+              if (slot[n].on) {
+                ring.fetch(stage, 4 * n, lane, xh + slot[n].a);
+                ring.fetch(stage, 4 * n + 2, lane, zh + slot[n].a);
+              }
+              if (slot[n].on_b) {
+                ring.fetch(stage, 4 * n + 1, lane, xh + slot[n].b);
+                ring.fetch(stage, 4 * n + 3, lane, zh + slot[n].b);
+              }
+            }
+          }
+          in.head += at_once;
+          if (in.head >= in.end) {
+            more_in = in.unit + stride < total;
+            if (more_in) begin_in(in.unit + stride);
+          }
         }
-      const bool same = st.head + at_once < st.end;
-      more = same || st.unit + stride < total;
-      if (same) next.head += at_once;
-      else if (more) next = begin(st.unit + stride);
-      if (more) fetch(next);
-      if (fresh) {
-        __syncwarp();  // the previous unit's angles have been read
-        token_angles<V>(p, st.position, lane, cs_token);
-      }
-      fresh = !same;
-      const int h = st.head + sub;
-      const bool live = h < st.end;
-      T* out = static_cast<T*>(p.out[which]) + st.b * p.os[which][0] + st.t * p.os[which][1] + h * p.os[which][2];
-      float xa[NS][V], xb[NS][V], za[NS][V], zb[NS][V];
-      float ss = 0.f, ex = 0.f;  // sum x^2, sum (w dz) x
+        Ring::commit();
+      };
+      begin_in(first);
 #pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        const int s = sl + n * p.lanes;
-        cx[n][0].unpack(xa[n]);
-        cx[n][1].unpack(xb[n]);
-        cz[n][0].unpack(za[n]);
-        cz[n][1].unpack(zb[n]);
-        float2 cs[V], w[V];
-        slot_angles<V>(p, cs_token, s, slot[n].turned, cs);
-        slot_weights<V>(w_s, slots, s, w);
-        turn_slot<V>(za[n], zb[n], cs, p.interleaved != 0);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          ss += xa[n][i] * xa[n][i] + xb[n][i] * xb[n][i];
-          ex += za[n][i] * w[i].x * xa[n][i] + zb[n][i] * w[i].y * xb[n][i];
+      for (int s = 0; s < Ring::kStages - 1; ++s) fetch(s);
+      at.begin(p, p.units[which], p.heads[which], first);
+      int64_t position = unit_position(p, p.units[which], first);
+      T* out_token = nullptr;
+      bool fresh = true;
+#pragma unroll 1
+      for (int stage = 0;; stage = stage + 1 == Ring::kStages ? 0 : stage + 1) {
+        fetch(stage == 0 ? Ring::kStages - 1 : stage - 1);
+        if (fresh) {
+          out_token = static_cast<T*>(p.out[which]) + at.b * p.os[which][0] + at.t * p.os[which][1];
+          __syncwarp();  // the previous unit's angles have been read
+          token_angles<V, IL>(p, turns, position, lane, angles);
+          if (at.unit + stride < total) position = unit_position(p, p.units[which], at.unit + stride);
         }
-      }
-      ss = group_sum(ss, p.lanes);
-      ex = group_sum(ex, p.lanes);
-      const float r = rsqrtf(ss / p.head_dim + p.eps);
-      const float m = r * r * ex / p.head_dim;  // r mean(e n)
+        Ring::wait();
+        Vec<V> u[NS], v[NS], zu[NS], zv[NS];
 #pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        float2 w[V];
-        slot_weights<V>(w_s, slots, sl + n * p.lanes, w);
-        float ga[V], gb[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          dwa[n][i] += za[n][i] * (xa[n][i] * r);
-          dwb[n][i] += zb[n][i] * (xb[n][i] * r);
-          ga[i] = r * (za[n][i] * w[i].x - xa[n][i] * m);
-          gb[i] = r * (zb[n][i] * w[i].y - xb[n][i] * m);
+        for (int n = 0; n < NS; ++n) {
+          to_pairs<T, V, IL>(ring.get(stage, 4 * n, lane), ring.get(stage, 4 * n + 1, lane), u[n], v[n]);
+          to_pairs<T, V, IL>(ring.get(stage, 4 * n + 2, lane), ring.get(stage, 4 * n + 3, lane), zu[n], zv[n]);
         }
-        if (live && slot[n].on) store_vec<T, V>(out + slot[n].a, ga);
-        if (live && slot[n].on_b) store_vec<T, V>(out + slot[n].b, gb);
+        const int h = at.head + sub;
+        const bool live = h < at.end;
+        T* out = out_token + static_cast<int64_t>(h) * p.oh[which];
+        Vec<V> ss, ex;  // sum x^2, sum (w dz) x
+        ss.fill(0.f);
+        ex.fill(0.f);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          SlotAngles<V> sa;
+          sa.load(p, angles, sl + n * p.lanes, slot[n].turned);
+          sa.turn(zu[n], zv[n]);
+          Vec<V> wu, wv;
+          load_pairs<V>(weights.u, slots, sl + n * p.lanes, wu);
+          load_pairs<V>(weights.v, slots, sl + n * p.lanes, wv);
+#pragma unroll
+          for (int i = 0; i < Vec<V>::N; ++i) {
+            ss.e[i] = fma_v(v[n].e[i], v[n].e[i], fma_v(u[n].e[i], u[n].e[i], ss.e[i]));
+            ex.e[i] = fma_v(mul_v(zu[n].e[i], wu.e[i]), u[n].e[i], ex.e[i]);
+            ex.e[i] = fma_v(mul_v(zv[n].e[i], wv.e[i]), v[n].e[i], ex.e[i]);
+          }
+        }
+        const float r = rsqrtf(group_sum(ss.sum(), p.lanes) * p.inv_head_dim + p.eps);
+        const float m = -r * r * r * (group_sum(ex.sum(), p.lanes) * p.inv_head_dim);  // -r^2 mean(e n)
+        const auto r2 = Vec<V>::all(r), m2 = Vec<V>::all(m);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          Vec<V> wu, wv;
+          load_pairs<V>(weights.u, slots, sl + n * p.lanes, wu);
+          load_pairs<V>(weights.v, slots, sl + n * p.lanes, wv);
+#pragma unroll
+          for (int i = 0; i < Vec<V>::N; ++i) {
+            const auto tu = mul_v(zu[n].e[i], r2), tv = mul_v(zv[n].e[i], r2);  // r dz
+            if (live) {
+              dwu[n].e[i] = fma_v(tu, u[n].e[i], dwu[n].e[i]);
+              dwv[n].e[i] = fma_v(tv, v[n].e[i], dwv[n].e[i]);
+            }
+            u[n].e[i] = fma_v(u[n].e[i], m2, mul_v(tu, wu.e[i]));
+            v[n].e[i] = fma_v(v[n].e[i], m2, mul_v(tv, wv.e[i]));
+          }
+          store_pairs<T, V, IL>(out, slot[n], live, u[n], v[n]);
+        }
+        at.head += at_once;
+        fresh = at.head >= at.end;
+        if (fresh) {
+          if (at.unit + stride >= total) break;
+          at.begin(p, p.units[which], p.heads[which], at.unit + stride);
+        }
       }
     }
     // head groups of the warp, then the warps of the block
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the sums take the rings' place
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+    for (int n = 0; n < NS; ++n) {
+      float du[V], dv[V];
+      dwu[n].get(du);
+      dwv[n].get(dv);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float a = dwa[n][i], b = dwb[n][i];
         for (int o = p.lanes; o < 32; o *= 2) {
-          a += __shfl_xor_sync(0xffffffffu, a, o);
-          b += __shfl_xor_sync(0xffffffffu, b, o);
+          du[i] += __shfl_xor_sync(0xffffffffu, du[i], o);
+          dv[i] += __shfl_xor_sync(0xffffffffu, dv[i], o);
         }
-        if (sub == 0 && slot[n].on) dw_s[warp][slot[n].a + i] = a;
-        if (sub == 0 && slot[n].on_b) dw_s[warp][slot[n].b + i] = b;
+        const int eu = slot_element<V, IL>(slot[n], 0, i), ev = slot_element<V, IL>(slot[n], 1, i);
+        if (sub == 0 && eu < p.head_dim) sh.dw[warp][eu] = du[i];
+        if (sub == 0 && ev < p.head_dim) sh.dw[warp][ev] = dv[i];
       }
+    }
     __syncthreads();
     float* row = p.dw_partial + (static_cast<int64_t>(blockIdx.x) * 2 + which) * p.head_dim;
     for (int i = threadIdx.x; i < p.head_dim; i += blockDim.x) {
       float v = 0.f;
 #pragma unroll
-      for (int k = 0; k < kRotWarps; ++k) v += dw_s[k][i];
+      for (int k = 0; k < kRotWarps; ++k) v += sh.dw[k][i];
       row[i] = v;
     }
   }

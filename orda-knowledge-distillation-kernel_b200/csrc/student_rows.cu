@@ -21,7 +21,13 @@ int check_rotary(const orda_rotary_args_t* a, bool backward) {
   if (a->batch < 0 || a->seq < 0 || a->heads[0] < 0 || a->heads[1] < 0) return ORDA_ERR_INVALID_ARGUMENT;
   if (a->head_dim < 1 || a->rotary_dim < 0 || a->rotary_dim % 2 || a->rotary_dim > a->head_dim)
     return ORDA_ERR_INVALID_ARGUMENT;
-  if (a->head_dim > ORDA_ROTARY_MAX_DIM || a->batch * a->seq > INT32_MAX) return ORDA_ERR_UNSUPPORTED;
+  // the kernels count units (a token's groups of heads) and step from head to head in 32 bits
+  if (a->head_dim > ORDA_ROTARY_MAX_DIM || a->batch > INT32_MAX || a->seq > INT32_MAX ||
+      a->batch * a->seq > INT32_MAX)
+    return ORDA_ERR_UNSUPPORTED;
+  for (int i = 0; i < 2; ++i)
+    for (int64_t stride : {a->x_stride[i][2], a->out_stride[i][2], a->dy_stride[i][2]})
+      if (stride > INT32_MAX || stride < INT32_MIN) return ORDA_ERR_UNSUPPORTED;
   if (a->layout != ORDA_ROTARY_HALF && a->layout != ORDA_ROTARY_INTERLEAVED) return ORDA_ERR_INVALID_ARGUMENT;
   const bool norm = a->weight[0] || a->weight[1];
   if ((norm || backward) && (!a->weight[0] || !a->weight[1] || !float_dtype(a->weight_dtype)))
@@ -29,6 +35,8 @@ int check_rotary(const orda_rotary_args_t* a, bool backward) {
   if (backward && (!a->dweight[0] || !a->dweight[1])) return ORDA_ERR_INVALID_ARGUMENT;
   if (a->batch * a->seq > 0) {
     if (!a->positions || (a->rotary_dim > 0 && !a->frequencies)) return ORDA_ERR_INVALID_ARGUMENT;
+    for (int i = 0; i < a->rotary_dim / 2; ++i)
+      if (!std::isfinite(a->frequencies[i])) return ORDA_ERR_INVALID_ARGUMENT;
     for (int i = 0; i < 2; ++i)
       if (a->heads[i] > 0 && (!a->x[i] || !a->out[i] || (backward && !a->dy[i]))) return ORDA_ERR_INVALID_ARGUMENT;
   }
@@ -63,6 +71,7 @@ int rotary_width(const orda_rotary_args_t* a, bool backward) {
 struct RotaryPlan {
   RotaryParams p;
   int width, grid;
+  bool interleaved;
 };
 
 // A unit of work (one warp) is a group of heads of one token. Large calls give a warp all heads of a
@@ -74,26 +83,34 @@ RotaryPlan plan_rotary(const orda_rotary_args_t* a, bool backward) {
   r.width = rotary_width(a, backward);
   for (int i = 0; i < 2; ++i) {
     p.x[i] = a->x[i]; p.dy[i] = a->dy[i]; p.out[i] = a->out[i]; p.w[i] = a->weight[i];
-    for (int j = 0; j < 3; ++j) {
+    for (int j = 0; j < 2; ++j) {
       p.xs[i][j] = a->x_stride[i][j];
       p.os[i][j] = a->out_stride[i][j];
       p.ds[i][j] = a->dy_stride[i][j];
     }
+    p.xh[i] = static_cast<int32_t>(a->x_stride[i][2]);
+    p.oh[i] = static_cast<int32_t>(a->out_stride[i][2]);
+    p.dh[i] = static_cast<int32_t>(a->dy_stride[i][2]);
     p.heads[i] = a->heads[i];
   }
   p.pos = a->positions;
   p.ps[0] = a->position_stride[0]; p.ps[1] = a->position_stride[1];
   p.pos64 = a->positions_int64;
-  p.seq = static_cast<int32_t>(a->seq);
+  p.seq = make_fast_div(static_cast<uint32_t>(a->seq));
   p.tokens = static_cast<int32_t>(a->batch * a->seq);
   p.head_dim = a->head_dim; p.rotary_dim = a->rotary_dim;
-  p.interleaved = a->layout == ORDA_ROTARY_INTERLEAVED;
+  r.interleaved = a->layout == ORDA_ROTARY_INTERLEAVED;
+  p.inv_head_dim = 1.f / static_cast<float>(a->head_dim);
   p.w_dtype = a->weight_dtype;
   p.magnitude = a->magnitude;
   p.sin_sign = (a->inverse != 0) != backward ? -1.f : 1.f;
   p.eps = a->eps;
-  const double two_pi = 6.283185307179586476925286766559;
-  for (int i = 0; i < a->rotary_dim / 2; ++i) p.turns[i] = a->frequencies[i] / two_pi;
+  const long double two_pi = 6.283185307179586476925286766559L;
+  for (int i = 0; i < a->rotary_dim / 2; ++i) {
+    long double turn = a->frequencies[i] / two_pi;
+    turn -= floorl(turn);
+    p.turns[i] = static_cast<uint64_t>(turn * 18446744073709551616.0L);
+  }
   const int slots = static_cast<int>(cdiv(a->head_dim, 2 * r.width));
   p.lanes = 1;
   while (p.lanes < slots && p.lanes < 32) p.lanes *= 2;
@@ -101,40 +118,55 @@ RotaryPlan plan_rotary(const orda_rotary_args_t* a, bool backward) {
   const int64_t want = 16 * num_sms();  // warps
   const int first = backward ? a->heads[0] : a->heads[0] + a->heads[1], second = backward ? a->heads[1] : 0;
   int hpu = static_cast<int>(cdiv(std::max({first, second, 1}), at_once)) * at_once;
+  // (a unit index stays below 2^31)
   while (hpu > at_once && static_cast<int64_t>(p.tokens) * (cdiv(first, hpu) + cdiv(second, hpu)) < want)
     hpu = static_cast<int>(cdiv(hpu / at_once, 2)) * at_once;
   p.heads_per_unit = hpu;
-  p.units[0] = static_cast<int32_t>(cdiv(first, hpu));
-  p.units[1] = static_cast<int32_t>(cdiv(second, hpu));
-  const int64_t units = static_cast<int64_t>(p.tokens) * std::max(p.units[0], p.units[1]);
+  const int64_t u0 = cdiv(first, hpu), u1 = cdiv(second, hpu);
+  p.units[0] = make_fast_div(static_cast<uint32_t>(std::max<int64_t>(u0, 1)));
+  p.units[1] = make_fast_div(static_cast<uint32_t>(std::max<int64_t>(u1, 1)));
+  const int64_t units = static_cast<int64_t>(p.tokens) * std::max<int64_t>(u0, u1);
+  // no more blocks than run at once (the kernels' launch bounds): a warp walks the units that are left
   r.grid = static_cast<int>(std::min<int64_t>(cdiv(units, kRotWarps), (backward ? 4 : 5) * num_sms()));
   return r;
 }
 
-template <typename T, int V>
+template <typename T, int V, bool IL>
 int run_rotary(const RotaryPlan& r, bool norm, cudaStream_t s) {
   count_launch();
-  if (norm) rotary_forward_kernel<T, V, true><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
-  else rotary_forward_kernel<T, V, false><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
+  if (norm) rotary_forward_kernel<T, V, true, IL><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
+  else rotary_forward_kernel<T, V, false, IL><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
   return launch_status();
 }
 
+// Single-element slots hold (u, v) in either layout: slot_of alone tells the layouts apart.
 template <typename T>
 int dispatch_rotary(const RotaryPlan& r, bool norm, cudaStream_t s) {
-  switch (r.width) {
-    case 8: return run_rotary<T, 8>(r, norm, s);
-    case 2: return run_rotary<T, 2>(r, norm, s);
-    default: return run_rotary<T, 1>(r, norm, s);
+  switch (r.width * 2 + r.interleaved) {
+    case 16: return run_rotary<T, 8, false>(r, norm, s);
+    case 17: return run_rotary<T, 8, true>(r, norm, s);
+    case 4: return run_rotary<T, 2, false>(r, norm, s);
+    case 5: return run_rotary<T, 2, true>(r, norm, s);
+    case 2: return run_rotary<T, 1, false>(r, norm, s);
+    default: return run_rotary<T, 1, true>(r, norm, s);
   }
+}
+
+template <typename T, int V, bool IL>
+void run_norm_backward(const RotaryPlan& r, cudaStream_t s) {
+  qk_norm_rotary_backward_kernel<T, V, IL><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
 }
 
 template <typename T>
 int dispatch_norm_backward(const RotaryPlan& r, cudaStream_t s) {
   count_launch();
-  switch (r.width) {
-    case 8: qk_norm_rotary_backward_kernel<T, 8><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p); break;
-    case 2: qk_norm_rotary_backward_kernel<T, 2><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p); break;
-    default: qk_norm_rotary_backward_kernel<T, 1><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p); break;
+  switch (r.width * 2 + r.interleaved) {
+    case 16: run_norm_backward<T, 8, false>(r, s); break;
+    case 17: run_norm_backward<T, 8, true>(r, s); break;
+    case 4: run_norm_backward<T, 2, false>(r, s); break;
+    case 5: run_norm_backward<T, 2, true>(r, s); break;
+    case 2: run_norm_backward<T, 1, false>(r, s); break;
+    default: run_norm_backward<T, 1, true>(r, s); break;
   }
   return launch_status();
 }
