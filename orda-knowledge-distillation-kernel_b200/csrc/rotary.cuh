@@ -377,9 +377,16 @@ __device__ __forceinline__ void load_pair_weights(const RotaryParams& p, int whi
   }
 }
 
-__device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int o = lanes / 2; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// Sums over the `lanes` lanes of a head (a power of two, uniform over the grid).
+template <int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], int lanes) {
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) {
+    if (lanes > o) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+  }
 }
 
 // slots a lane may have to hold (1 with 8-element vectors: 32 lanes cover 512 elements)
@@ -566,7 +573,9 @@ __global__ void __launch_bounds__(32 * kRotWarps, 5) rotary_forward_kernel(const
       for (int n = 0; n < NS; ++n)
 #pragma unroll
         for (int i = 0; i < Vec<V>::N; ++i) ss.e[i] = fma_v(v[n].e[i], v[n].e[i], fma_v(u[n].e[i], u[n].e[i], ss.e[i]));
-      r = Vec<V>::all(rsqrtf(group_sum(ss.sum(), p.lanes) * p.inv_head_dim + p.eps));
+      float sum[1] = {ss.sum()};
+      group_sum(sum, p.lanes);
+      r = Vec<V>::all(rsqrtf(sum[0] * p.inv_head_dim + p.eps));
     }
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
@@ -718,8 +727,10 @@ __global__ void __launch_bounds__(32 * kRotWarps, 4)
             ex.e[i] = fma_v(mul_v(zv[n].e[i], wv.e[i]), v[n].e[i], ex.e[i]);
           }
         }
-        const float r = rsqrtf(group_sum(ss.sum(), p.lanes) * p.inv_head_dim + p.eps);
-        const float m = -r * r * r * (group_sum(ex.sum(), p.lanes) * p.inv_head_dim);  // -r^2 mean(e n)
+        float sum[2] = {ss.sum(), ex.sum()};
+        group_sum(sum, p.lanes);
+        const float r = rsqrtf(sum[0] * p.inv_head_dim + p.eps);
+        const float m = -r * r * r * (sum[1] * p.inv_head_dim);  // -r^2 mean(e n)
         const auto r2 = Vec<V>::all(r), m2 = Vec<V>::all(m);
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
@@ -776,22 +787,28 @@ __global__ void __launch_bounds__(32 * kRotWarps, 4)
   }
 }
 
-// dweight[which][i] = sum over the blocks' partial rows; one block per 32 columns of one weight.
-static __global__ void __launch_bounds__(256) norm_weight_grad_kernel(const float* partial, int rows, int head_dim,
-                                                                      int dtype, void* dwq, void* dwk) {
-  __shared__ float acc[8][32];
-  const int which = blockIdx.y, col = blockIdx.x * 32 + threadIdx.x % 32, part = threadIdx.x / 32;
+// dweight[which][i] = sum over the blocks' partial rows; one block per 32 columns of one weight, the rows
+// shared out over its 32 warps.
+static __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* __restrict__ partial, int rows,
+                                                                       int head_dim, int dtype, void* dwq, void* dwk) {
+  __shared__ float acc[32][33];
+  const int which = blockIdx.y, lane = threadIdx.x % 32, part = threadIdx.x / 32;
+  const int col = blockIdx.x * 32 + lane;
   float v = 0.f;
-  if (col < head_dim)
-    for (int r = part; r < rows; r += 8) v += partial[(static_cast<int64_t>(r) * 2 + which) * head_dim + col];
-  acc[part][threadIdx.x % 32] = v;
+  if (col < head_dim) {
+#pragma unroll 8
+    for (int r = part; r < rows; r += 32) v += partial[(static_cast<int64_t>(r) * 2 + which) * head_dim + col];
+  }
+  acc[part][lane] = v;
   __syncthreads();
-  if (part != 0 || col >= head_dim) return;
-  for (int k = 1; k < 8; ++k) v += acc[k][threadIdx.x];
+  v = acc[lane][part];  // warp `part` now adds up column `part`
+  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int out_col = blockIdx.x * 32 + part;
+  if (lane != 0 || out_col >= head_dim) return;
   void* out = which ? dwk : dwq;
-  if (dtype == ORDA_F32) static_cast<float*>(out)[col] = v;
-  else if (dtype == ORDA_F16) static_cast<__half*>(out)[col] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(out)[col] = __float2bfloat16_rn(v);
+  if (dtype == ORDA_F32) static_cast<float*>(out)[out_col] = v;
+  else if (dtype == ORDA_F16) static_cast<__half*>(out)[out_col] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(out)[out_col] = __float2bfloat16_rn(v);
 }
 
 }  // namespace orda
