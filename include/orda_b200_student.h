@@ -25,8 +25,9 @@ extern "C" {
 #define ORDA_ACT_GELU_TANH 2  /* g / 2 (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3)))            */
 #define ORDA_ACT_RELU 3       /* max(g, 0), derivative 0 at 0                               */
 
-/* Up to this many rows the 16-bit forward call streams the weights without pipeline waits. */
-#define ORDA_GLU_FEW_ROWS 32
+/* Up to this many rows the 16-bit forward call needs no status word from its caller: a pipeline wait that
+   timed out leaves NaN in h. */
+#define ORDA_GLU_FEW_ROWS 128
 
 typedef struct orda_glu_args {
   int32_t abi_version;   /* = ORDA_ABI_VERSION */

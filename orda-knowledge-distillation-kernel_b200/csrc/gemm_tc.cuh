@@ -30,6 +30,7 @@ constexpr int kBK = 64;                       // k elements per stage (128 B of 
 constexpr uint32_t kATileBytes = kTileRows * kBK * 2;
 constexpr int kGemmThreads = 192;
 constexpr uint32_t kSmemBudget = 200 * 1024;
+constexpr uint32_t kStagePieceBytes = 4096;       // a warp's staging buffer of a TMA-store epilogue: 32 rows x 64 columns
 
 struct StoreEpiParams {
   void* out;         // D destination

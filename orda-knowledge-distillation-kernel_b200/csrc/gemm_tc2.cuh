@@ -6,7 +6,9 @@
 // their own TMEM. Two accumulator buffers (512 TMEM columns) let the epilogue of one tile overlap
 // the mainloop of the next. Every CTA loads only the tiles it consumes (no multicast).
 // Used for dHidden (few output tiles: 256 x 256 tiles fill more SMs than the 512 x 256 tiles of the
-// wide kernel in gemm_tc2w.cuh) and for the testing GEMM.
+// wide kernel in gemm_tc2w.cuh), for the gated feed-forward block where K is short (EPI_GLU: 256 rows x
+// 128 features a tile; CTA 0 loads its half of B from the gate weight, CTA 1 the same features of the
+// up weight; 8 epilogue warps) and for the testing GEMM.
 //
 //   warp 0 (each CTA) : TMA producer; transaction bytes of both CTAs land on the leader's barrier
 //   warp 1 (leader)   : MMA issuer; one multicast commit releases the smem stage in both CTAs
@@ -22,6 +24,7 @@
 #include "distill_common.cuh"
 #include "fwd_epilogue.cuh"
 #include "gemm_tc.cuh"
+#include "glu_epilogue.cuh"
 #include "sm100_ptx.cuh"
 
 namespace orda {
@@ -40,19 +43,22 @@ __device__ unsigned long long g_tc2_prof[kProfSlots][8];
 
 __device__ __forceinline__ long long clk() { return clock64(); }
 
-template <int AMODE>
+template <int EPI>
 struct PairShape {
   static constexpr int kStages = 6;
+  static constexpr int kEpiWarps = EPI == EPI_GLU ? 8 : 4;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr uint32_t kStaging = EPI == EPI_GLU ? kEpiWarps * kStagePieceBytes : 0;
   static constexpr uint32_t kBarBytes = (2 * kStages + 4) * 8 + 16;
-  static constexpr uint32_t kSmemBytes = kStages * kPairStageBytes + kBarBytes + 1024;
+  static constexpr uint32_t kSmemBytes = kStages * kPairStageBytes + kStaging + kBarBytes + 1024;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
 template <bool A_MN, bool B_MN, int AMODE, bool TWO_SEG, int EPI, typename T16>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<EPI>::kThreads, 1)
     tc2_gemm_kernel(const __grid_constant__ TcGemmParams p) {
-  static_assert(EPI == EPI_STORE, "the 256 x 256 pair kernel stores D; the logits epilogue runs in the wide kernel");
-  using S = PairShape<AMODE>;
+  static_assert(EPI == EPI_STORE || EPI == EPI_GLU, "the logits epilogue runs in the wide kernel");
+  using S = PairShape<EPI>;
   constexpr uint32_t kIdesc = make_idesc_f16(std::is_same<T16, __nv_bfloat16>::value ? 1u : 0u, 256, kPairBN,
                                              A_MN ? 1u : 0u, B_MN ? 1u : 0u);
   constexpr uint32_t kTmemCols = 512;  // two 256-column accumulator buffers
@@ -60,7 +66,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t tiles_addr = (raw_addr + 1023u) & ~1023u;
-  const uint32_t bar_addr = tiles_addr + S::kStages * kPairStageBytes;
+  const uint32_t staging_addr = tiles_addr + S::kStages * kPairStageBytes;
+  const uint32_t bar_addr = staging_addr + S::kStaging;
   auto full_bar = [&](int s) { return bar_addr + 8u * s; };
   auto empty_bar = [&](int s) { return bar_addr + 8u * (S::kStages + s); };
   auto tfull_bar = [&](int b) { return bar_addr + 8u * (2 * S::kStages + b); };
@@ -82,7 +89,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), 8);  // one elected lane per epilogue warp of both CTAs
+      mbar_init(tempty_bar(b), 2 * S::kEpiWarps);  // one elected lane per epilogue warp of both CTAs
     }
     fence_barrier_init();
   }
@@ -90,7 +97,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     tma_prefetch_desc(&p.a0);
     tma_prefetch_desc(&p.b0);
     if (AMODE == A_INTERLEAVE || TWO_SEG) tma_prefetch_desc(&p.a1);
-    if (TWO_SEG) tma_prefetch_desc(&p.b1);
+    if (TWO_SEG || EPI == EPI_GLU) tma_prefetch_desc(&p.b1);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, kTmemCols);
@@ -112,7 +119,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
       for (int32_t t = pair; t < num_tiles && ok; t += npairs) {
         int32_t mt, nt;
         tile_coords(t, p.m_tiles, p.n_tiles, p.group_m, mt, nt);
-        const int32_t n_cta = nt * kPairBN + static_cast<int32_t>(rank) * 128;
+        const int32_t n_cta = EPI == EPI_GLU ? nt * 128 : nt * kPairBN + static_cast<int32_t>(rank) * 128;
         for (int32_t kb = 0; kb < kb_total; ++kb) {
           const long long c0 = prof ? clk() : 0;
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, p.status)) { ok = false; break; }
@@ -124,7 +131,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
           const bool seg1 = TWO_SEG && kb >= p.kb0;
           const int32_t k0 = (seg1 ? kb - p.kb0 : kb) * kBK;
           const CUtensorMap* amap = seg1 ? &p.a1 : &p.a0;
-          const CUtensorMap* bmap = seg1 ? &p.b1 : &p.b0;
+          const CUtensorMap* bmap = (EPI == EPI_GLU ? rank != 0 : seg1) ? &p.b1 : &p.b0;
           if constexpr (AMODE == A_INTERLEAVE) {
             const int32_t r = mt * 128 + static_cast<int32_t>(rank) * 64;
             tma_load_2d_pair(sa, &p.a0, lead_full, k0, r);
@@ -196,7 +203,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
       }
     }
   } else {
-    // ------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
+    // ------------------------------------------------------------ epilogue (warps 2.., both CTAs)
+    // TMEM lanes 32 * (warp % 4) .. + 31; with 8 warps, warps 2..5 take the first 64 features of a tile
+    // and warps 6..9 the others
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     int it = 0;
@@ -215,7 +224,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kPairBN;
       const int64_t n0 = static_cast<int64_t>(nt) * kPairBN;
       const int64_t row = static_cast<int64_t>(mt) * 256 + rank * 128 + r;
-      store_epilogue<T16>(p.st, tbase, row, n0, kPairBN);
+      if constexpr (EPI == EPI_GLU) {
+        const int part = (warp - 2) >> 2;
+        glu_store<T16>(p, tbase, staging_addr + (warp - 2) * kStagePieceBytes, row - lane,
+                       static_cast<int64_t>(nt) * 128, part, part + 1, lane);
+      } else {
+        store_epilogue<T16>(p.st, tbase, row, n0, kPairBN);
+      }
       tc_fence_before();
       __syncwarp();
       if (prof) busy += clk() - c1;
@@ -224,6 +239,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         else mbar_arrive_cluster(map_to_cta(tempty_bar(buf), 0));
       }
     }
+    if (EPI == EPI_GLU && lane == 0) bulk_wait_all();  // staged stores complete before the shared memory goes away
     if (prof) {
       atomicAdd(&g_tc2_prof[p.prof_slot][3], static_cast<unsigned long long>(w_tfull));
       atomicAdd(&g_tc2_prof[p.prof_slot][4], static_cast<unsigned long long>(busy));

@@ -3,8 +3,8 @@
 //   h = act(g) u,  g = x Wg^T,  u = x Wu^T
 //   dg = dh u act'(g),  du = dh act(g)
 //
-// Many rows run on the wide pair GEMM (gemm_tc2w.cuh, EPI_GLU). With a few rows the two weights are all
-// that has to be read, so glu_rows_kernel streams them once, straight from memory into the fragments
+// Many rows run on the pair GEMMs (gemm_tc2w.cuh, gemm_tc2.cuh, EPI_GLU), up to 128 on glu_swap.cuh. With at
+// most 8 rows the two weights are all that has to be read, so glu_rows_kernel streams them once, straight from memory into the fragments
 // of mma.sync (m16n8k16): 16 features of each weight a block, the block's 8 warps share out K, the
 // partial sums meet in shared memory in a fixed order. A lane's 16-byte load holds 8 consecutive k of one
 // weight row; which of them an instruction takes as its k = 0 .. 15 is free as long as x is permuted
@@ -57,10 +57,10 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {
   return u;
 }
 
-// NB: blocks of 8 rows of x (1, 2, 4): rows <= 8 NB
-template <typename T, int NB>
+// At most 8 rows: one n = 8 fragment of x.
+template <typename T>
 __global__ void __launch_bounds__(32 * kGluWarps) glu_rows_kernel(const __grid_constant__ GluRowsParams p) {
-  __shared__ float part[kGluWarps][2][kGluFeatures][8 * NB + 1];
+  __shared__ float part[kGluWarps][2][kGluFeatures][8 + 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int r = lane / 4, q = lane % 4;
   const int64_t f0 = static_cast<int64_t>(blockIdx.x) * kGluFeatures;
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(32 * kGluWarps) glu_rows_kernel(const __grid_c
   const T* g1 = static_cast<const T*>(p.gate) + fb * p.ld_gate;
   const T* u0 = static_cast<const T*>(p.up) + fa * p.ld_up;
   const T* u1 = static_cast<const T*>(p.up) + fb * p.ld_up;
-  float cg[NB][4] = {}, cu[NB][4] = {};
+  float cg[4] = {}, cu[4] = {};
   const uint4 zero = make_uint4(0, 0, 0, 0);
   for (int k0 = warp * kGluK * kGluUnroll; k0 < p.hidden; k0 += kGluWarps * kGluK * kGluUnroll) {
     uint4 w[kGluUnroll][4];
@@ -87,27 +87,21 @@ __global__ void __launch_bounds__(32 * kGluWarps) glu_rows_kernel(const __grid_c
 #pragma unroll
     for (int j = 0; j < kGluUnroll; ++j) {
       const int k = k0 + j * kGluK + q * 8;
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int row = n * 8 + r;
-        uint4 x = zero;
-        if (row < p.rows && k < p.hidden)
-          x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + row * p.ld_x + k));
-        mma_16x8x16<T>(cg[n], w[j][0].x, w[j][1].x, w[j][0].y, w[j][1].y, x.x, x.y);
-        mma_16x8x16<T>(cg[n], w[j][0].z, w[j][1].z, w[j][0].w, w[j][1].w, x.z, x.w);
-        mma_16x8x16<T>(cu[n], w[j][2].x, w[j][3].x, w[j][2].y, w[j][3].y, x.x, x.y);
-        mma_16x8x16<T>(cu[n], w[j][2].z, w[j][3].z, w[j][2].w, w[j][3].w, x.z, x.w);
-      }
+      uint4 x = zero;
+      if (r < p.rows && k < p.hidden)
+        x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + r * p.ld_x + k));
+      mma_16x8x16<T>(cg, w[j][0].x, w[j][1].x, w[j][0].y, w[j][1].y, x.x, x.y);
+      mma_16x8x16<T>(cg, w[j][0].z, w[j][1].z, w[j][0].w, w[j][1].w, x.z, x.w);
+      mma_16x8x16<T>(cu, w[j][2].x, w[j][3].x, w[j][2].y, w[j][3].y, x.x, x.y);
+      mma_16x8x16<T>(cu, w[j][2].z, w[j][3].z, w[j][2].w, w[j][3].w, x.z, x.w);
     }
   }
   // accumulator element e of a lane: feature r (+ 8 for e >= 2), row 2 q + (e & 1)
 #pragma unroll
-  for (int n = 0; n < NB; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      part[warp][0][r + (e >> 1) * 8][n * 8 + 2 * q + (e & 1)] = cg[n][e];
-      part[warp][1][r + (e >> 1) * 8][n * 8 + 2 * q + (e & 1)] = cu[n][e];
-    }
+  for (int e = 0; e < 4; ++e) {
+    part[warp][0][r + (e >> 1) * 8][2 * q + (e & 1)] = cg[e];
+    part[warp][1][r + (e >> 1) * 8][2 * q + (e & 1)] = cu[e];
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < kGluFeatures * p.rows; i += 32 * kGluWarps) {
     const int f = i % kGluFeatures, row = i / kGluFeatures;

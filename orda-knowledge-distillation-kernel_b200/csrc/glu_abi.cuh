@@ -3,6 +3,7 @@
 #pragma once
 
 #include "glu.cuh"
+#include "glu_swap.cuh"
 #include "orda_b200_student.h"
 
 namespace {
@@ -48,15 +49,57 @@ int glu_rows_launch(const orda_glu_args_t* a, cudaStream_t s) {
   p.rows = static_cast<int32_t>(a->rows); p.hidden = static_cast<int32_t>(a->hidden); p.act = a->activation;
   const int grid = static_cast<int>(cdiv(a->ffn, kGluFeatures));
   count_launch();
-  if (a->rows <= 8) glu_rows_kernel<T16, 1><<<grid, 32 * kGluWarps, 0, s>>>(p);
-  else if (a->rows <= 16) glu_rows_kernel<T16, 2><<<grid, 32 * kGluWarps, 0, s>>>(p);
-  else glu_rows_kernel<T16, 4><<<grid, 32 * kGluWarps, 0, s>>>(p);
+  glu_rows_kernel<T16><<<grid, 32 * kGluWarps, 0, s>>>(p);
   return launch_status();
 }
 
 template <typename T16>
+int glu_swap_launch(const orda_glu_args_t* a, cudaStream_t s) {
+  GluSwapParams p{};
+  int tokens = 16;
+  while (tokens < a->rows && tokens < 128) tokens *= 2;
+  int rc;
+  if ((rc = make_map(&p.gate, a->dtype, a->gate, a->hidden, a->ffn, a->ld_gate, 64, kSwapFeatures))) return rc;
+  if ((rc = make_map(&p.up, a->dtype, a->up, a->hidden, a->ffn, a->ld_up, 64, kSwapFeatures))) return rc;
+  if ((rc = make_map(&p.x, a->dtype, a->x, a->hidden, a->rows, a->ld_x, 64, static_cast<uint32_t>(tokens)))) return rc;
+  p.h = a->h; p.pre_gate = a->pre_gate; p.pre_up = a->pre_up;
+  p.ld_h = a->ld_h; p.ffn = a->ffn; p.rows = a->rows;
+  p.tokens = tokens;
+  p.kb = static_cast<int32_t>(cdiv(a->hidden, kBK));
+  p.act = a->activation;
+  p.idesc = make_idesc_f16(a->dtype == ORDA_BF16 ? 1u : 0u, 128, static_cast<uint32_t>(tokens), 0u, 0u);
+  p.status = a->device_status;
+  // as many stages as half an SM holds (6 at 16 tokens, 3 at 128); the exchange of the two products needs
+  // 512 bytes a token of the same memory
+  p.stages = static_cast<int32_t>(std::min<uint32_t>(8, (kSwapSmem - 1024) / swap_stage_bytes(tokens)));
+  const uint32_t smem = 1024 + p.stages * swap_stage_bytes(tokens);
+  set_smem(glu_swap_kernel<T16>, smem);
+  // Blocks that share a tile's K: as many as fit beside the other tiles, two blocks an SM, each with at least
+  // four k blocks (one round of stages).
+  const int64_t f_tiles = cdiv(a->ffn, kSwapFeatures), t_tiles = cdiv(a->rows, tokens);
+  int64_t split = std::min<int64_t>({8, 2 * num_sms() / (f_tiles * t_tiles), p.kb / 4});
+  split = std::max<int64_t>(split, 1);
+  p.kb_part = static_cast<int32_t>(cdiv(p.kb, split));
+  p.split = static_cast<int32_t>(cdiv(p.kb, p.kb_part));  // no block without a k block
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(f_tiles * p.split), 1, static_cast<unsigned>(t_tiles));
+  cfg.blockDim = dim3(kSwapThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = static_cast<unsigned>(p.split);
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  count_launch();
+  return cudaLaunchKernelEx(&cfg, glu_swap_kernel<T16>, p) == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+}
+
+template <typename T16>
 int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
-  if (a->rows <= ORDA_GLU_FEW_ROWS) return glu_rows_launch<T16>(a, s);
+  if (a->rows <= 8) return glu_rows_launch<T16>(a, s);
+  if (a->rows <= ORDA_GLU_FEW_ROWS) return glu_swap_launch<T16>(a, s);
   TcGemmParams prm{};
   prm.status = a->device_status;
   int rc;
@@ -73,7 +116,17 @@ int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
   prm.kb0 = static_cast<int32_t>(cdiv(a->hidden, kBK));
   prm.st.M = a->rows;
   prm.st.N = a->ffn;
-  return launch_tc2w<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 512), 2 * round8(a->ffn), s, 4);
+  // 512 x 128 or 256 x 128 tiles: the wide kernel moves a quarter less per product, the 256-row one has two
+  // accumulator buffers, so that a short K does not wait for the epilogue, and wastes less of a ragged
+  // batch. In clocks of a CTA pair, measured over K = 1024 and 4096: 1050 a k block + 9500 a tile against
+  // 570 + 2500. (8192 x 1024 -> 2816: 94 us wide, 82 us here; 8192 x 4096 -> 11264: 1036 against 1075.)
+  const int64_t pairs = std::max(1, num_sms() / 2), f_tiles = cdiv(a->ffn, 128);
+  const int64_t wide = cdiv(cdiv(a->rows, 512) * f_tiles, pairs) * (1050 * prm.kb0 + 9500);
+  const int64_t half = cdiv(cdiv(a->rows, 256) * f_tiles, pairs) * (570 * prm.kb0 + 2500);
+  const int64_t cols = 2 * round8(a->ffn);
+  if (half < wide)
+    return launch_tc2<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 256), cols, s, 8);
+  return launch_tc2w<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 512), cols, s, 4);
 }
 
 // K split of a gradient GEMM with M x N outputs and `kb` k blocks on the wide kernel: the split whose

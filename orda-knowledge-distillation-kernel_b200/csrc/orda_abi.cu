@@ -283,7 +283,7 @@ enum GemmRole { ROLE_LOGITS = 0, ROLE_DH = 1, ROLE_DW = 2 };
 template <bool A_MN, bool B_MN, int AMODE, bool TWO_SEG, int EPI, typename T16>
 int launch_tc2(TcGemmParams& prm, int64_t M_tiles, int64_t N, cudaStream_t stream, int group_m,
                int reserve_sms = 0) {
-  using S = PairShape<AMODE>;
+  using S = PairShape<EPI>;
   prm.m_tiles = static_cast<int32_t>(M_tiles);
   prm.n_tiles = static_cast<int32_t>(cdiv(N, kPairBN));
   prm.group_m = group_m;
@@ -296,7 +296,7 @@ int launch_tc2(TcGemmParams& prm, int64_t M_tiles, int64_t N, cudaStream_t strea
   const int usable = std::max(2, num_sms() - std::max(0, reserve_sms));
   const int pairs = static_cast<int>(std::min<int64_t>(tiles, usable / 2));
   count_launch();
-  k<<<2 * pairs, kGemmThreads, S::kSmemBytes, stream>>>(prm);
+  k<<<2 * pairs, S::kThreads, S::kSmemBytes, stream>>>(prm);
   return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
 }
 

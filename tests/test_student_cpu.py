@@ -164,7 +164,7 @@ def _glu(**kw):
     (dict(abi_version=9), _native.ERR_INVALID_ARGUMENT), (dict(dtype=5), _native.ERR_INVALID_ARGUMENT),
     (dict(activation=4), _native.ERR_INVALID_ARGUMENT), (dict(rows=-1), _native.ERR_INVALID_ARGUMENT),
     (dict(hidden=0), _native.ERR_INVALID_ARGUMENT), (dict(x=None), _native.ERR_INVALID_ARGUMENT),
-    (dict(h=None), _native.ERR_INVALID_ARGUMENT), (dict(rows=33, device_status=None), _native.ERR_INVALID_ARGUMENT), (dict(pre_gate=16), _native.ERR_INVALID_ARGUMENT),
+    (dict(h=None), _native.ERR_INVALID_ARGUMENT), (dict(rows=129, device_status=None), _native.ERR_INVALID_ARGUMENT), (dict(pre_gate=16), _native.ERR_INVALID_ARGUMENT),
     (dict(ld_gate=8), _native.ERR_INVALID_ARGUMENT), (dict(x=24), _native.ERR_ALIGNMENT),
     (dict(hidden=12), _native.ERR_ALIGNMENT), (dict(ld_up=20), _native.ERR_ALIGNMENT),
     (dict(rows=1 << 31), _native.ERR_UNSUPPORTED), (dict(rows=0), _native.OK),
