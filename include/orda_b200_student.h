@@ -40,10 +40,10 @@ typedef struct orda_glu_args {
   const void* x; int64_t ld_x;          /* [N, H]                                            */
   const void* gate; int64_t ld_gate;    /* [F, H]                                            */
   const void* up; int64_t ld_up;        /* [F, H]                                            */
-  /* forward: h; backward reads pre_gate, pre_up and dh. ld_h is the row stride of h, dh, pre_gate
-     and pre_up. 16-bit types: hidden, ld_* multiples of 8, bases 16-byte aligned.           */
-  void* h; int64_t ld_h;                /* [N, F]                                            */
-  void* pre_gate;                       /* [N, F] x Wgate^T, written where not NULL          */
+  /* 16-bit types: hidden and the strides of x, gate, up multiples of 8; ld_pre always. Bases 16-byte aligned,
+     but for h and dh, which may lie anywhere.                                              */
+  void* h; int64_t ld_h;                /* [N, F]; ld_h is the row stride of dh too          */
+  void* pre_gate; int64_t ld_pre;       /* [N, F] x Wgate^T, written where not NULL          */
   void* pre_up;                         /* [N, F] x Wup^T (both or neither)                  */
   /* backward */
   const void* dh;                       /* [N, F]                                            */

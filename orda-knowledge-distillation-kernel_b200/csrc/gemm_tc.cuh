@@ -56,7 +56,7 @@ struct TcGemmParams {
   // wide kernel, store epilogue with st_tma = 1: the 16-bit output [M, N] (64 x 32 boxes, 128-byte
   // swizzle); the epilogue stages each 32-row x 64-column piece in shared memory and stores it by TMA
   CUtensorMap out_map;
-  int32_t st_tma;
+  int32_t st_tma;     // 1: 16-bit output; 2: fp32 partials of a k split, out_map is [split, M, N] in 32 x 32 boxes
   // with st_tma and rows routed to peers (st.peers > 0, slab_rows a multiple of 512): map k covers
   // this GPU's slot [slab_rows, N] in peer k's slot buffer
   CUtensorMap peer_maps[ORDA_MAX_PEERS];
@@ -73,6 +73,7 @@ struct TcGemmParams {
   // EPI_GLU: b0 / b1 are the gate / up weights, out_map stores h, ws_s_map / ws_t_map the products before
   // the activation (glu_save = 1)
   int32_t glu_act, glu_save;
+  void* glu_h;       // not NULL: h has rows that TMA cannot store (st.ldo elements apart) and goes out by plain stores
   FwdEpiParams fwd;
   StoreEpiParams st;
 };

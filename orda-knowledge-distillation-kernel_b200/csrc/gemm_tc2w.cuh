@@ -248,6 +248,36 @@ __device__ __forceinline__ void wide_store_tma(const TcGemmParams& p, uint32_t t
   }
 }
 
+// fp32 partials of k split `ks` through shared memory and TMA: the warp's 32 rows x 256 columns leave as eight
+// 32 x 32 pieces of full 128-byte lines (16-byte stores one row per lane touch 32 lines an instruction).
+__device__ __forceinline__ void wide_store_partial_tma(const TcGemmParams& p, uint32_t tbase, uint32_t staging,
+                                                       int64_t y0, int64_t n0, int32_t ks, int lane) {
+#pragma unroll 1
+  for (int g = 0; g < kPairBN / 32; ++g) {
+    const int64_t c0 = n0 + g * 32;
+    uint32_t r[32];
+    tmem_ld32_async(tbase + g * 32, r);
+    tmem_wait_ld();
+    if (c0 >= p.st.N || y0 >= p.st.M) continue;  // warp-uniform
+    if (lane == 0) bulk_wait_read_all();  // the previous piece has left the staging buffer
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const uint32_t addr = staging + static_cast<uint32_t>(lane) * 128u +
+                            ((static_cast<uint32_t>(q) ^ static_cast<uint32_t>(lane & 7)) << 4);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[4 * q]), "r"(r[4 * q + 1]),
+                   "r"(r[4 * q + 2]), "r"(r[4 * q + 3])
+                   : "memory");
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(&p.out_map, staging, static_cast<int32_t>(c0), static_cast<int32_t>(y0), ks);
+      bulk_commit_group();
+    }
+  }
+}
+
 template <bool A_MN, bool B_MN, int AMODE, bool TWO_SEG, int EPI, typename T16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThreads, 1)
     tc2w_gemm_kernel(const __grid_constant__ TcGemmParams p) {
@@ -520,7 +550,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThr
           glu_store<T16>(p, tbase, staging, y0, static_cast<int64_t>(nt) * 128, 0, 2, lane);
         } else {
           const int64_t y0 = static_cast<int64_t>(mt) * 512 + j * 256 + rank * 128 + quarter * 32;
-          if (p.st_tma) {
+          if (p.st_tma == 2) {
+            wide_store_partial_tma(p, tbase, staging, y0, n0, ks, lane);
+          } else if (p.st_tma) {
             wide_store_tma<T16>(p, tbase, staging, y0, n0, lane);
           } else {
             StoreEpiParams st = p.st;

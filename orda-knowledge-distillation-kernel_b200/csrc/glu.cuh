@@ -28,7 +28,7 @@ constexpr int kGluUnroll = 4;     // loads of each row in flight: 128 k a step
 struct GluRowsParams {
   const void *x, *gate, *up;
   void *h, *pre_gate, *pre_up;
-  int64_t ld_x, ld_gate, ld_up, ld_h;
+  int64_t ld_x, ld_gate, ld_up, ld_h, ld_pre;
   int64_t ffn;
   int32_t rows, hidden, act;
 };
@@ -114,33 +114,35 @@ __global__ void __launch_bounds__(32 * kGluWarps) glu_rows_kernel(const __grid_c
     }
     float a = 0.f, d;
     with_act(p.act, [&](auto tag) { glu_act<decltype(tag)::kAct, false>(g, a, d); });
-    const int64_t at = row * p.ld_h + f0 + f;
-    static_cast<T*>(p.h)[at] = Conv<T>::from_f(a * u);
+    static_cast<T*>(p.h)[row * p.ld_h + f0 + f] = Conv<T>::from_f(a * u);
     if (p.pre_gate) {
-      static_cast<T*>(p.pre_gate)[at] = Conv<T>::from_f(g);
-      static_cast<T*>(p.pre_up)[at] = Conv<T>::from_f(u);
+      static_cast<T*>(p.pre_gate)[row * p.ld_pre + f0 + f] = Conv<T>::from_f(g);
+      static_cast<T*>(p.pre_up)[row * p.ld_pre + f0 + f] = Conv<T>::from_f(u);
     }
   }
 }
 
-// h = act(g) u of the fp32 path. Rows of `cols` values with row stride ld (g, u, h alike).
+// h = act(g) u of the fp32 path. Rows of `cols` values, row stride ld of g and u, ld_h of h.
 static __global__ void __launch_bounds__(256) glu_act_kernel(const float* g, const float* u, float* h, int64_t rows,
-                                                             int64_t cols, int64_t ld, int act) {
+                                                             int64_t cols, int64_t ld, int64_t ld_h, int act) {
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows * cols;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t at = i / cols * ld + i % cols;
     float a = 0.f, d;
     with_act(act, [&](auto tag) { glu_act<decltype(tag)::kAct, true>(g[at], a, d); });
-    h[at] = a * u[at];
+    h[i / cols * ld_h + i % cols] = a * u[at];
   }
 }
 
 // dg and du into the two halves of `out`, rows of 2 * cols_pad: columns [0, cols_pad) dg, the rest du.
-// Every pointer 16-byte aligned, cols_pad and ld multiples of 8; the columns behind `cols` (the padding)
-// are set to zero. One 8-element vector per thread and step; memory-bound (three reads, two writes).
+// g, u and out 16-byte aligned, cols_pad and ld (the row stride of g and u) multiples of 8; dh (row stride
+// ld_dh) any, read element by element unless dh_vec. The columns behind `cols` (the padding) are set to
+// zero. One 8-element vector per thread and step; memory-bound (three reads, two writes).
 template <typename T>
-__global__ void __launch_bounds__(256) glu_grad_kernel(const T* dh, const T* g, const T* u, T* out, int64_t rows,
-                                                       int64_t cols, int64_t cols_pad, int64_t ld, int act) {
+__global__ void __launch_bounds__(256) glu_grad_kernel(const T* __restrict__ dh, int64_t ld_dh, int dh_vec,
+                                                       const T* __restrict__ g, const T* __restrict__ u,
+                                                       T* __restrict__ out, int64_t rows, int64_t cols,
+                                                       int64_t cols_pad, int64_t ld, int act) {
   const int64_t vecs = cols_pad / 8, total = rows * vecs;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -150,7 +152,8 @@ __global__ void __launch_bounds__(256) glu_grad_kernel(const T* dh, const T* g, 
     constexpr int Q = sizeof(T) / 2;
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
-      const uint4 a = __ldcs(reinterpret_cast<const uint4*>(dh + at) + k);
+      uint4 a = make_uint4(0, 0, 0, 0);
+      if (dh_vec) a = __ldcs(reinterpret_cast<const uint4*>(dh + row * ld_dh + c) + k);
       const uint4 b = __ldcs(reinterpret_cast<const uint4*>(g + at) + k);
       const uint4 e = __ldcs(reinterpret_cast<const uint4*>(u + at) + k);
       const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w}, we[4] = {e.x, e.y, e.z, e.w};
@@ -166,6 +169,10 @@ __global__ void __launch_bounds__(256) glu_grad_kernel(const T* dh, const T* g, 
           unpack2<T>(we[j], vu[2 * j], vu[2 * j + 1]);
         }
       }
+    }
+    if (!dh_vec) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vd[j] = c + j < cols ? Conv<T>::to_f(dh[row * ld_dh + c + j]) : 0.f;
     }
     float og[8], ou[8];
     with_act(act, [&](auto tag) {

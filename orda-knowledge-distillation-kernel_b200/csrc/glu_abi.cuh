@@ -21,7 +21,8 @@ int check_glu(const orda_glu_args_t* a, bool backward) {
   if (!a->x || !a->gate || !a->up) return ORDA_ERR_INVALID_ARGUMENT;
   if (!a->device_status && a->dtype != ORDA_F32 && (backward || a->rows > ORDA_GLU_FEW_ROWS))
     return ORDA_ERR_INVALID_ARGUMENT;
-  if (a->ld_x < a->hidden || a->ld_gate < a->hidden || a->ld_up < a->hidden || a->ld_h < a->ffn)
+  if (a->ld_x < a->hidden || a->ld_gate < a->hidden || a->ld_up < a->hidden || a->ld_h < a->ffn ||
+      ((a->pre_gate || backward) && a->ld_pre < a->ffn))
     return ORDA_ERR_INVALID_ARGUMENT;
   if (backward) {
     if (!a->pre_gate || !a->pre_up || !a->dh) return ORDA_ERR_INVALID_ARGUMENT;
@@ -30,10 +31,10 @@ int check_glu(const orda_glu_args_t* a, bool backward) {
   }
   auto off = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };
   const int64_t unit = a->dtype == ORDA_F32 ? 1 : 8;
-  if (a->hidden % unit || a->ld_x % unit || a->ld_gate % unit || a->ld_up % unit || a->ld_h % 8)
+  if (a->hidden % unit || a->ld_x % unit || a->ld_gate % unit || a->ld_up % unit ||
+      ((a->pre_gate || backward) && a->ld_pre % 8))
     return ORDA_ERR_ALIGNMENT;
-  if (off(a->x) || off(a->gate) || off(a->up) || off(a->h) || off(a->pre_gate) || off(a->pre_up) || off(a->dh) ||
-      off(a->dx) || off(a->dweights))
+  if (off(a->x) || off(a->gate) || off(a->up) || off(a->pre_gate) || off(a->pre_up) || off(a->dx) || off(a->dweights))
     return ORDA_ERR_ALIGNMENT;
   if (a->dtype == ORDA_F32 && !backward && !a->pre_gate) return ORDA_ERR_INVALID_ARGUMENT;  // its products need a place
   return ORDA_OK;
@@ -44,7 +45,7 @@ int glu_rows_launch(const orda_glu_args_t* a, cudaStream_t s) {
   GluRowsParams p{};
   p.x = a->x; p.gate = a->gate; p.up = a->up;
   p.h = a->h; p.pre_gate = a->pre_gate; p.pre_up = a->pre_up;
-  p.ld_x = a->ld_x; p.ld_gate = a->ld_gate; p.ld_up = a->ld_up; p.ld_h = a->ld_h;
+  p.ld_x = a->ld_x; p.ld_gate = a->ld_gate; p.ld_up = a->ld_up; p.ld_h = a->ld_h; p.ld_pre = a->ld_pre;
   p.ffn = a->ffn;
   p.rows = static_cast<int32_t>(a->rows); p.hidden = static_cast<int32_t>(a->hidden); p.act = a->activation;
   const int grid = static_cast<int>(cdiv(a->ffn, kGluFeatures));
@@ -63,7 +64,7 @@ int glu_swap_launch(const orda_glu_args_t* a, cudaStream_t s) {
   if ((rc = make_map(&p.up, a->dtype, a->up, a->hidden, a->ffn, a->ld_up, 64, kSwapFeatures))) return rc;
   if ((rc = make_map(&p.x, a->dtype, a->x, a->hidden, a->rows, a->ld_x, 64, static_cast<uint32_t>(tokens)))) return rc;
   p.h = a->h; p.pre_gate = a->pre_gate; p.pre_up = a->pre_up;
-  p.ld_h = a->ld_h; p.ffn = a->ffn; p.rows = a->rows;
+  p.ld_h = a->ld_h; p.ld_pre = a->ld_pre; p.ffn = a->ffn; p.rows = a->rows;
   p.tokens = tokens;
   p.kb = static_cast<int32_t>(cdiv(a->hidden, kBK));
   p.act = a->activation;
@@ -106,12 +107,17 @@ int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
   if ((rc = make_operand_map(&prm.a0, a->dtype, a->x, false, a->rows, a->hidden, a->ld_x, kTileRows))) return rc;
   if ((rc = make_operand_map(&prm.b0, a->dtype, a->gate, false, a->ffn, a->hidden, a->ld_gate, 128))) return rc;
   if ((rc = make_operand_map(&prm.b1, a->dtype, a->up, false, a->ffn, a->hidden, a->ld_up, 128))) return rc;
-  if ((rc = make_map(&prm.out_map, a->dtype, a->h, a->ffn, a->rows, a->ld_h, 64, 32))) return rc;
+  if (a->ld_h % 8 == 0 && (reinterpret_cast<uintptr_t>(a->h) & 15u) == 0) {
+    if ((rc = make_map(&prm.out_map, a->dtype, a->h, a->ffn, a->rows, a->ld_h, 64, 32))) return rc;
+  } else {
+    prm.glu_h = a->h;
+    prm.st.ldo = a->ld_h;
+  }
   prm.glu_act = a->activation;
   prm.glu_save = a->pre_gate != nullptr;
   if (prm.glu_save) {
-    if ((rc = make_map(&prm.ws_s_map, a->dtype, a->pre_gate, a->ffn, a->rows, a->ld_h, 64, 32))) return rc;
-    if ((rc = make_map(&prm.ws_t_map, a->dtype, a->pre_up, a->ffn, a->rows, a->ld_h, 64, 32))) return rc;
+    if ((rc = make_map(&prm.ws_s_map, a->dtype, a->pre_gate, a->ffn, a->rows, a->ld_pre, 64, 32))) return rc;
+    if ((rc = make_map(&prm.ws_t_map, a->dtype, a->pre_up, a->ffn, a->rows, a->ld_pre, 64, 32))) return rc;
   }
   prm.kb0 = static_cast<int32_t>(cdiv(a->hidden, kBK));
   prm.st.M = a->rows;
@@ -119,10 +125,10 @@ int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
   // 512 x 128 or 256 x 128 tiles: the wide kernel moves a quarter less per product, the 256-row one has two
   // accumulator buffers, so that a short K does not wait for the epilogue, and wastes less of a ragged
   // batch. In clocks of a CTA pair, measured over K = 1024 and 4096: 1050 a k block + 9500 a tile against
-  // 570 + 2500. (8192 x 1024 -> 2816: 94 us wide, 82 us here; 8192 x 4096 -> 11264: 1036 against 1075.)
+  // 590 + 2300. (8192 x 1024 -> 2816: 94 us wide, 82 us here; 8192 x 4096 -> 11264: 1036 against 1075.)
   const int64_t pairs = std::max(1, num_sms() / 2), f_tiles = cdiv(a->ffn, 128);
   const int64_t wide = cdiv(cdiv(a->rows, 512) * f_tiles, pairs) * (1050 * prm.kb0 + 9500);
-  const int64_t half = cdiv(cdiv(a->rows, 256) * f_tiles, pairs) * (570 * prm.kb0 + 2500);
+  const int64_t half = cdiv(cdiv(a->rows, 256) * f_tiles, pairs) * (590 * prm.kb0 + 2300);
   const int64_t cols = 2 * round8(a->ffn);
   if (half < wide)
     return launch_tc2<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 256), cols, s, 8);
@@ -130,8 +136,8 @@ int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
 }
 
 // K split of a gradient GEMM with M x N outputs and `kb` k blocks on the wide kernel: the split whose
-// estimated time is smallest, from the time of a wave (every CTA pair one tile), a wave's fixed cost and
-// the traffic of the fp32 partials (written once, read once).
+// estimated time is smallest. A wave (every CTA pair one tile) takes 0.65 us a k block and 4 us more; a
+// split adds a launch and the traffic of the fp32 partials, written once and read once at 6.5 TB/s.
 int glu_split(int64_t M, int64_t N, int64_t kb) {
   const int64_t tiles = cdiv(M, 512) * cdiv(N, kPairBN);
   const int64_t pairs = std::max(1, num_sms() / 2);
@@ -139,8 +145,8 @@ int glu_split(int64_t M, int64_t N, int64_t kb) {
   double best_us = 0;
   for (int sp = 1; sp <= 8 && sp <= kb; ++sp) {
     if (sp > 1 && cdiv(kb, sp) * (sp - 1) >= kb) continue;  // a range would be empty
-    double us = static_cast<double>(cdiv(tiles * sp, pairs)) * (0.75 * cdiv(kb, sp) + 2.0);
-    if (sp > 1) us += 3.0 + 8.0 * sp * M * N / 5.0e6;
+    double us = static_cast<double>(cdiv(tiles * sp, pairs)) * (0.65 * cdiv(kb, sp) + 4.0);
+    if (sp > 1) us += 2.5 + (4.0 * sp + 2.0) * M * N / 6.5e6;
     if (sp == 1 || us < best_us) {
       best = sp;
       best_us = us;
@@ -177,6 +183,19 @@ GluPlan plan_glu_backward(const orda_glu_args_t* a) {
   return p;
 }
 
+// [split, M, N] fp32 array in boxes of one split's 32 x 32 values, 128-byte swizzle.
+int make_partial_map(CUtensorMap* m, void* base, int64_t N, int64_t M, int split) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return ORDA_ERR_CUDA;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(M), static_cast<cuuint64_t>(split)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(N) * 4, static_cast<cuuint64_t>(N) * M * 4};
+  const cuuint32_t box[3] = {32, 32, 1}, ones[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims, strides, box, ones,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? ORDA_OK : ORDA_ERR_INVALID_ARGUMENT;
+}
+
 // Destination of a gradient GEMM: `out` itself (TMA store where its rows are whole 64-column pieces), or
 // fp32 partials added in a fixed order by sum_split_kernel.
 template <bool A_MN, bool TWO_SEG, typename T16>
@@ -195,6 +214,8 @@ int glu_grad_gemm(TcGemmParams& prm, int dtype, int64_t M, int64_t N, int split,
   prm.kb_split = static_cast<int32_t>(cdiv(prm.kb0 + prm.kb1, split));
   prm.split_bytes = static_cast<int64_t>(sizeof(float)) * M * N;
   prm.st = StoreEpiParams{part, N, M, N, 1, 0};
+  if ((rc = make_partial_map(&prm.out_map, part, N, M, split))) return rc;  // (rows of N floats: 32-byte multiples)
+  prm.st_tma = 2;
   if ((rc = launch_tc2w<A_MN, true, A_PLAIN, TWO_SEG, EPI_STORE, T16>(prm, cdiv(M, 512), N, s, 4))) return rc;
   const int64_t count8 = M * N / 8;
   count_launch();
@@ -208,9 +229,10 @@ int glu_grad_launch(const orda_glu_args_t* a, const GluPlan& P, T* out, cudaStre
   const int64_t vecs = a->rows * (P.fp / 8);
   const int grid = static_cast<int>(std::min<int64_t>(cdiv(vecs, 256), 16 * num_sms()));
   count_launch();
-  glu_grad_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(a->dh), static_cast<const T*>(a->pre_gate),
-                                          static_cast<const T*>(a->pre_up), out, a->rows, a->ffn, P.fp, a->ld_h,
-                                          a->activation);
+  const bool dh_vec = a->ffn % 8 == 0 && (a->ld_h * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(a->dh) & 15u) == 0;
+  glu_grad_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(a->dh), a->ld_h, dh_vec,
+                                          static_cast<const T*>(a->pre_gate), static_cast<const T*>(a->pre_up), out,
+                                          a->rows, a->ffn, P.fp, a->ld_pre, a->activation);
   return launch_status();
 }
 
@@ -249,11 +271,11 @@ int glu_forward_f32(const orda_glu_args_t* a, cudaStream_t s) {
   float* g = static_cast<float*>(a->pre_gate);
   float* u = static_cast<float*>(a->pre_up);
   const float* x = static_cast<const float*>(a->x);
-  simt_gemm(x, a->ld_x, 1, static_cast<const float*>(a->gate), a->ld_gate, 1, g, a->ld_h, a->rows, a->ffn, a->hidden, 0, s);
-  simt_gemm(x, a->ld_x, 1, static_cast<const float*>(a->up), a->ld_up, 1, u, a->ld_h, a->rows, a->ffn, a->hidden, 0, s);
+  simt_gemm(x, a->ld_x, 1, static_cast<const float*>(a->gate), a->ld_gate, 1, g, a->ld_pre, a->rows, a->ffn, a->hidden, 0, s);
+  simt_gemm(x, a->ld_x, 1, static_cast<const float*>(a->up), a->ld_up, 1, u, a->ld_pre, a->rows, a->ffn, a->hidden, 0, s);
   count_launch();
   glu_act_kernel<<<static_cast<int>(std::min<int64_t>(cdiv(a->rows * a->ffn, 256), 16 * num_sms())), 256, 0, s>>>(
-      g, u, static_cast<float*>(a->h), a->rows, a->ffn, a->ld_h, a->activation);
+      g, u, static_cast<float*>(a->h), a->rows, a->ffn, a->ld_pre, a->ld_h, a->activation);
   return launch_status();
 }
 

@@ -8,6 +8,22 @@
 
 namespace orda {
 
+// erfc(y / sqrt 2) / 2 for y >= 0: with x = y / sqrt 2 and t = 1 / (1 + x / 2), ln(erfc(x) e^{x^2} / t) is smooth
+// in t, and a polynomial of degree 7 fitted to it (Chebyshev points over 0 <= x <= 14) leaves a relative
+// error of 1.1e-6 everywhere: a third of erfcf's instructions, and enough for 16-bit results.
+__device__ __forceinline__ float half_erfc_of(float y) {
+  const float t = __fdividef(1.f, fmaf(0.35355339059327376f, y, 1.f));
+  float p = -0.19184046983718872f;
+  p = fmaf(p, t, 0.7685127854347229f);
+  p = fmaf(p, t, -1.0301551818847656f);
+  p = fmaf(p, t, 0.37635737657546997f);
+  p = fmaf(p, t, -0.05336221680045128f);
+  p = fmaf(p, t, 0.39794403314590454f);
+  p = fmaf(p, t, 0.997983455657959f);
+  p = fmaf(p, t, -1.265440583229065f);
+  return 0.5f * t * fast_exp(fmaf(-0.5f * y, y, p));
+}
+
 // act(g) in `a`, act'(g) in `d`. The exponentials use the hardware's approximations (relative error about
 // 2^-22), far below the rounding of a 16-bit result; EXACT takes the library functions instead, for
 // 32-bit tensors.
@@ -21,8 +37,15 @@ __device__ __forceinline__ void glu_act(float g, float& a, float& d) {
     a = fmaxf(g, 0.f);
     d = g > 0.f ? 1.f : 0.f;
   } else if constexpr (ACT == ORDA_ACT_GELU) {
-    const float cdf = 0.5f * erfcf(g * -0.70710678118654752f);
-    const float e = EXACT ? expf(-0.5f * g * g) : fast_exp(-0.5f * g * g);
+    float cdf, e;
+    if constexpr (EXACT) {
+      cdf = 0.5f * erfcf(g * -0.70710678118654752f);
+      e = expf(-0.5f * g * g);
+    } else {
+      const float half_erfc = half_erfc_of(fabsf(g));
+      cdf = g > 0.f ? 1.f - half_erfc : half_erfc;
+      e = fast_exp(-0.5f * g * g);
+    }
     a = g * cdf;
     d = cdf + g * e * 0.39894228040143268f;
   } else {

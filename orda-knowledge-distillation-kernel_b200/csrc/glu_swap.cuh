@@ -32,7 +32,7 @@ constexpr uint32_t kSwapSmem = 113 * 1024;  // of a block: two fit an SM
 struct GluSwapParams {
   CUtensorMap gate, up, x;  // boxes: 64 x 64 of the weights, 64 x tokens of x
   void *h, *pre_gate, *pre_up;
-  int64_t ld_h, ffn, rows;
+  int64_t ld_h, ld_pre, ffn, rows;
   int32_t tokens;           // tokens of a tile: 16, 32, 64 or 128
   int32_t stages, kb, kb_part, act;  // k blocks: all, of one block of the cluster
   int32_t split;            // blocks of the cluster
@@ -148,16 +148,21 @@ __global__ void __launch_bounds__(kSwapThreads, 2) glu_swap_kernel(const __grid_
   if (p.split > 1) cluster_sync_all();  // every block's part is in its shared memory
   else __syncthreads();
   if (warp >= 2) {
-    for (int r = 0; r < p.split; ++r) ok = ok && cluster_load_int(map_to_cta(smem_u32(&failed), r)) == 0;
+    ok = ok && failed == 0;
+    if (p.split > 1)
+      for (int r = 0; r < p.split; ++r) ok = ok && cluster_load_int(map_to_cta(smem_u32(&failed), r)) == 0;
     const uint32_t sg = smem_u32(exchange), su = sg + p.tokens * kSwapFeatures * 4;
     const int64_t f = f0 + 2 * lane;
-    const bool pair = f + 1 < p.ffn && p.ld_h % 2 == 0;
+    const bool pair = f + 1 < p.ffn;
     for (int t = part * 4 + warp - 2; t < p.tokens && t0 + t < p.rows; t += 4 * p.split) {
       if (f >= p.ffn) break;
       const float nan = __int_as_float(0x7fffffff);
       const uint32_t at_pair = (t * kSwapFeatures + 2 * lane) * 4;
       float2 g = make_float2(0.f, 0.f), u = g;
-      for (int r = 0; r < p.split; ++r) {
+      if (p.split == 1) {
+        g = *reinterpret_cast<const float2*>(exchange + t * kSwapFeatures + 2 * lane);
+        u = *reinterpret_cast<const float2*>(exchange + (p.tokens + t) * kSwapFeatures + 2 * lane);
+      } else for (int r = 0; r < p.split; ++r) {
         const float2 x = cluster_load_float2(map_to_cta(sg + at_pair, r)), y = cluster_load_float2(map_to_cta(su + at_pair, r));
         g.x += x.x; g.y += x.y;
         u.x += y.x; u.y += y.y;
@@ -169,20 +174,19 @@ __global__ void __launch_bounds__(kSwapThreads, 2) glu_swap_kernel(const __grid_
         glu_act<decltype(tag)::kAct, false>(g.y, a1, d);
       });
       if (!ok) a0 = a1 = nan;
-      const int64_t at = (t0 + t) * p.ld_h + f;
-      auto put = [&](void* out, float x, float y) {
-        T16* o = static_cast<T16*>(out) + at;
-        if (pair) {
+      auto put = [&](void* out, int64_t ld, float x, float y) {
+        T16* o = static_cast<T16*>(out) + (t0 + t) * ld + f;
+        if (pair && ld % 2 == 0) {
           *reinterpret_cast<uint32_t*>(o) = pack2<T16>(x, y);
         } else {
           o[0] = Conv<T16>::from_f(x);
           if (f + 1 < p.ffn) o[1] = Conv<T16>::from_f(y);
         }
       };
-      put(p.h, a0 * u.x, a1 * u.y);
+      put(p.h, p.ld_h, a0 * u.x, a1 * u.y);
       if (p.pre_gate) {
-        put(p.pre_gate, g.x, g.y);
-        put(p.pre_up, u.x, u.y);
+        put(p.pre_gate, p.ld_pre, g.x, g.y);
+        put(p.pre_up, p.ld_pre, u.x, u.y);
       }
     }
     if (!ok && p.status) atomicCAS(p.status, 0, ORDA_ERR_TIMEOUT);

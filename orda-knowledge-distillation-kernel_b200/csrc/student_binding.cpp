@@ -128,7 +128,8 @@ orda_glu_args_t glu_args(const Tensor& x, const Tensor& gate, const Tensor& up, 
   a.ld_gate = row_stride(gate);
   a.up = up.data_ptr();
   a.ld_up = row_stride(up);
-  a.ld_h = round8(a.ffn);
+  a.ld_h = a.ffn;
+  a.ld_pre = round8(a.ffn);
   return a;
 }
 
@@ -140,15 +141,14 @@ std::pair<Tensor, Tensor> glu_forward(const Tensor& x, const Tensor& gate, const
   const auto dt = x.scalar_type();
   Tensor h = new_empty({a.rows, a.ld_h}, dt, x), pre, status;
   if (save || dt == at::kFloat) {
-    pre = new_empty({2, a.rows, a.ld_h}, dt, x);
+    pre = new_empty({2, a.rows, a.ld_pre}, dt, x);
     a.pre_gate = pre.data_ptr();
-    a.pre_up = static_cast<char*>(pre.data_ptr()) + a.rows * a.ld_h * pre.element_size();
+    a.pre_up = static_cast<char*>(pre.data_ptr()) + a.rows * a.ld_pre * pre.element_size();
   }
   if (a.rows > ORDA_GLU_FEW_ROWS && dt != at::kFloat) status = new_status(x, s);
   a.h = h.data_ptr();
   a.device_status = static_cast<int32_t*>(ptr(status));
   check_status(orda_glu_forward(&a, s), "orda_glu_forward");
-  if (a.ld_h != a.ffn) h = h.slice(1, 0, a.ffn).contiguous();
   return {h, pre};
 }
 
@@ -162,16 +162,14 @@ std::pair<Tensor, Tensor> glu_backward(Tensor dh, const Tensor& x, const Tensor&
   const auto dt = x.scalar_type();
   Tensor dx, dw, ws, status;
   if (need_x) dx = new_empty({a.rows, a.hidden}, dt, x);
-  if (need_w) dw = new_empty({a.ld_h + a.ffn, a.hidden}, dt, x);
+  if (need_w) dw = new_empty({a.ld_pre + a.ffn, a.hidden}, dt, x);
   if (a.rows == 0) {
     if (dw.defined()) dw.zero_();
     return {dx, dw};
   }
-  if (a.ld_h != a.ffn) dh = at::constant_pad_nd(dh, {0, a.ld_h - a.ffn});
   dh = dh.contiguous();
-  if (reinterpret_cast<uintptr_t>(dh.data_ptr()) % 16) dh = dh.clone();
   a.pre_gate = pre.data_ptr();
-  a.pre_up = static_cast<char*>(pre.data_ptr()) + a.rows * a.ld_h * pre.element_size();
+  a.pre_up = static_cast<char*>(pre.data_ptr()) + a.rows * a.ld_pre * pre.element_size();
   a.dh = dh.data_ptr();
   a.dx = ptr(dx);
   a.dweights = ptr(dw);

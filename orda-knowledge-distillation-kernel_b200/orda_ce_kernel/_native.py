@@ -109,7 +109,7 @@ class GluArgs(ctypes.Structure):
         ("abi_version", _i32), ("dtype", _i32), ("activation", _i32), ("reserved", _i32),
         ("rows", _i64), ("hidden", _i64), ("ffn", _i64),
         ("x", _vp), ("ld_x", _i64), ("gate", _vp), ("ld_gate", _i64), ("up", _vp), ("ld_up", _i64),
-        ("h", _vp), ("ld_h", _i64), ("pre_gate", _vp), ("pre_up", _vp),
+        ("h", _vp), ("ld_h", _i64), ("pre_gate", _vp), ("ld_pre", _i64), ("pre_up", _vp),
         ("dh", _vp), ("dx", _vp), ("dweights", _vp),
         ("device_status", _vp),
     ]

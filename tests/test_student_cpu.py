@@ -156,7 +156,7 @@ def test_struct_mirrors_match_the_header(tmp_path):
 
 def _glu(**kw):
     a = dict(abi_version=_native.ABI_VERSION, dtype=_native.BF16, activation=0, rows=4, hidden=16, ffn=8, x=16, ld_x=16,
-             gate=16, ld_gate=16, up=16, ld_up=16, h=16, ld_h=8, device_status=16) | kw
+             gate=16, ld_gate=16, up=16, ld_up=16, h=16, ld_h=8, ld_pre=8, device_status=16) | kw
     return _native.GluArgs(**a)
 
 
