@@ -196,18 +196,16 @@ int make_partial_map(CUtensorMap* m, void* base, int64_t N, int64_t M, int split
   return r == CUDA_SUCCESS ? ORDA_OK : ORDA_ERR_INVALID_ARGUMENT;
 }
 
-// Destination of a gradient GEMM: `out` itself (TMA store where its rows are whole 64-column pieces), or
-// fp32 partials added in a fixed order by sum_split_kernel.
+// Destination of a gradient GEMM: `out` itself, or fp32 partials added in a fixed order by sum_split_kernel;
+// both leave by TMA stores.
 template <bool A_MN, bool TWO_SEG, typename T16>
 int glu_grad_gemm(TcGemmParams& prm, int dtype, int64_t M, int64_t N, int split, void* out, uint8_t* part,
                   cudaStream_t s) {
   int rc;
   if (split <= 1) {
     prm.st = StoreEpiParams{out, N, M, N, 0, 0};
-    if (N % 64 == 0) {
-      if ((rc = make_map(&prm.out_map, dtype, out, N, M, N, 64, 32))) return rc;
-      prm.st_tma = 1;
-    }
+    if ((rc = make_map(&prm.out_map, dtype, out, N, M, N, 64, 32))) return rc;  // (clips a last piece at N)
+    prm.st_tma = 1;
     return launch_tc2w<A_MN, true, A_PLAIN, TWO_SEG, EPI_STORE, T16>(prm, cdiv(M, 512), N, s, 4);
   }
   prm.ksplit = split;

@@ -7,10 +7,12 @@
 // The tensors are cut into equal chunks that the blocks take in a fixed order; each block writes one
 // 64-bit partial sum, and every block of the second launch adds all of them up for itself in the same
 // order, so the result does not depend on which block ran first and no counter has to be reset.
-// Squares are formed and added in 64 bits: a norm neither overflows nor vanishes before its own value does.
+// Squares are added in 64 bits: a norm neither overflows nor vanishes before its own value does.
 //
 // What bounds it: memory; the gradients are read twice and written once. The second launch walks the
-// chunks backwards, so the ones read last by the first come from L2.
+// chunks backwards, from the ones that the first read last (1% on a list of 247 MB; evict-last and streaming
+// cache hints gave no more: B200 writes at 3.8 TB/s at most, and that, not the second read, is what the
+// second launch waits for).
 #pragma once
 
 #include "distill_common.cuh"
@@ -77,10 +79,34 @@ __device__ __forceinline__ uint4 pack16(const float (&v)[16 / sizeof(T)]) {
     return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }
 
+// Sum of squares of one 16-byte vector. 16-bit types: the eight squares are formed and added in fp32 (exact
+// products) and converted once, since converting every value to fp64 bounds the kernel by the conversion
+// pipe (393 us against 364 for 1.2e9 bf16 values); a sum near either end of fp32's range is taken again in fp64.
+template <typename T>
+__device__ __forceinline__ double vector_squares(const uint4& u) {
+  constexpr int V = 16 / sizeof(T);
+  float v[V];
+  unpack16<T>(u, v);
+  if constexpr (sizeof(T) == 2) {
+    float a = v[0] * v[0], b = v[1] * v[1];
+#pragma unroll
+    for (int e = 2; e < V; e += 2) {
+      a = fmaf(v[e], v[e], a);
+      b = fmaf(v[e + 1], v[e + 1], b);
+    }
+    a += b;
+    if (a > 1e-27f && a < 1e36f) return static_cast<double>(a);
+  }
+  double s = 0.0;
+#pragma unroll
+  for (int e = 0; e < V; ++e) s += square(v[e]);
+  return s;
+}
+
 template <typename T>
 __device__ __forceinline__ double chunk_squares(const T* p, int64_t n) {
   constexpr int V = 16 / sizeof(T);
-  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  double acc[2] = {0.0, 0.0};
   int64_t done = 0;
   if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
     const int64_t vecs = n / V;
@@ -91,23 +117,13 @@ __device__ __forceinline__ double chunk_squares(const T* p, int64_t n) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) u[k] = __ldg(q + i + k * kGradThreads);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float v[V];
-        unpack16<T>(u[k], v);
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[e & 3] += square(v[e]);
-      }
+      for (int k = 0; k < 4; ++k) acc[k & 1] += vector_squares<T>(u[k]);
     }
-    for (; i < vecs; i += kGradThreads) {
-      float v[V];
-      unpack16<T>(__ldg(q + i), v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) acc[e & 3] += square(v[e]);
-    }
+    for (; i < vecs; i += kGradThreads) acc[0] += vector_squares<T>(__ldg(q + i));
     done = vecs * V;
   }
   for (int64_t i = done + threadIdx.x; i < n; i += kGradThreads) acc[0] += square(Conv<T>::to_f(p[i]));
-  return (acc[0] + acc[1]) + (acc[2] + acc[3]);
+  return acc[0] + acc[1];
 }
 
 template <typename T>
