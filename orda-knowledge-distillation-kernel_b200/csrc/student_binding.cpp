@@ -533,10 +533,26 @@ std::tuple<std::vector<Tensor>, Tensor> clip_gradients(const std::vector<Tensor>
   src.reserve(grads.size());
   out.reserve(grads.size());
   c10::cuda::CUDAGuard guard(grads[0].device());
+  int64_t bytes = 0;
   for (const Tensor& g : grads) {
     src.push_back(dense(g));
-    const Tensor& d = src.back();
-    out.push_back(Tensor(at::detail::empty_strided_cuda(d.sizes(), d.strides(), d.scalar_type(), d.device())));
+    bytes += (src.back().nbytes() + 255) / 256 * 256;
+  }
+  // Short lists: the host's allocations would take longer than the kernels, so the results share one.
+  // (16 fp32 tensors of a 0.5M-parameter model: 25 us a call with an allocation each.)
+  if (bytes <= (int64_t(16) << 20)) {
+    const Tensor all = new_empty({bytes}, at::kByte, grads[0]);
+    int64_t at = 0;
+    for (const Tensor& d : src) {
+      Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()),
+                                                          c10::DispatchKeySet(c10::DispatchKey::CUDA), d.dtype());
+      t.unsafeGetTensorImpl()->set_sizes_and_strides(d.sizes(), d.strides(), at / d.element_size());
+      out.push_back(std::move(t));
+      at += (d.nbytes() + 255) / 256 * 256;
+    }
+  } else {
+    for (const Tensor& d : src)
+      out.push_back(Tensor(at::detail::empty_strided_cuda(d.sizes(), d.strides(), d.scalar_type(), d.device())));
   }
   Tensor norm = clip_call(src, &out, max_norm, eps);
   return {std::move(out), std::move(norm)};

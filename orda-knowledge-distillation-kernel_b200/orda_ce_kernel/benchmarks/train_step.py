@@ -3,6 +3,7 @@ peak memory with the loss as a ``torch.compile``d PyTorch formula vs the fused k
 
     python -m orda_ce_kernel.benchmarks.train_step [--teacher separate-student] [--vocabs 32768]
                                                    [--seqs 512 1024 2048] [--steps 50] [--json out.json]
+                                                   [--qk-norm] [--clip-norm 1.0]
 
 Protocol of the reference's training benchmark (``test/benchmark/src/_train.py:102-452``,
 ``Train_*.py``, model of ``src/core.py:106-138``): a pre-norm decoder (RMSNorm, rotary position
@@ -14,7 +15,11 @@ step on random token ids. Backends:
   torch-compile  - teacher, student and the PyTorch loss formula in one compiled function;
   orda_b200      - compiled teacher and student, the fused loss called eagerly;
   orda_b200-graph- the student forward and the fused loss compiled together (the loss is a custom op,
-                   so the compiled region has no graph break).
+                   so the compiled region has no graph break);
+  orda_b200-ops  - as orda_b200, with the models' rotary positions (and query/key norms), their gated
+                   feed-forward blocks and gradient clipping through ``orda_ce_kernel.student``.
+``--qk-norm`` puts an RMS norm with a weight on every query and key head, ``--clip-norm`` clips the gradients
+to that global norm before the optimizer step; both are off in the reference's protocol.
 """
 from __future__ import annotations
 
@@ -26,12 +31,14 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .. import student as student_ops
+from ..student import RotaryConfig
 from ._common import write_json
 
 TEACHER_CFG = dict(dim=1024, q_heads=8, kv_heads=2, n_layers=16, ffn_dim=2816)
 STUDENT_CFG = dict(dim=1024, q_heads=8, kv_heads=2, n_layers=8, ffn_dim=2816)
 BATCH, TEMP, WARMUP = 16, 3.0, 5
-BACKENDS = ["torch-compile", "orda_b200", "orda_b200-graph"]
+BACKENDS = ["torch-compile", "orda_b200", "orda_b200-graph", "orda_b200-ops"]
 TEACHERS = ["tied", "separate-student", "separate-full", "precomputed-logits", "precomputed-hidden"]
 
 
@@ -60,11 +67,17 @@ def rotate(x, cos, sin):
 
 
 class Attention(nn.Module):
-    def __init__(self, d, q_heads, kv_heads, seq):
+    """``ops``: positions (and norms) of queries and keys through the student operators."""
+
+    def __init__(self, d, q_heads, kv_heads, seq, qk_norm=False, ops=False):
         super().__init__()
+        self.ops = ops
         self.hq, self.hkv, self.dh = q_heads, kv_heads, d // q_heads
         self.qkv = nn.Linear(d, (q_heads + 2 * kv_heads) * self.dh, bias=False)
         self.proj = nn.Linear(d, d, bias=False)
+        self.q_norm, self.k_norm = (RMSNorm(self.dh), RMSNorm(self.dh)) if qk_norm else (None, None)
+        self.rotary = RotaryConfig(self.dh)
+        self.register_buffer("positions", torch.arange(seq), persistent=False)
         cos, sin = rotary_tables(self.dh, seq)
         self.register_buffer("cos", cos, persistent=False)
         self.register_buffer("sin", sin, persistent=False)
@@ -72,11 +85,21 @@ class Attention(nn.Module):
     def forward(self, x):
         b, t, d = x.shape
         q, k, v = self.qkv(x).split([self.hq * self.dh, self.hkv * self.dh, self.hkv * self.dh], dim=-1)
-        q = q.view(b, t, self.hq, self.dh).transpose(1, 2)
-        k = k.view(b, t, self.hkv, self.dh).transpose(1, 2)
+        q, k = q.view(b, t, self.hq, self.dh), k.view(b, t, self.hkv, self.dh)
         v = v.view(b, t, self.hkv, self.dh).transpose(1, 2)
-        cos, sin = self.cos[:t].to(x.dtype), self.sin[:t].to(x.dtype)
-        q, k = rotate(q, cos, sin), rotate(k, cos, sin)
+        if self.ops:
+            positions = self.positions[:t]
+            if self.q_norm is not None:
+                q, k = student_ops.qk_norm_rotary(q, k, self.q_norm.scale, self.k_norm.scale, positions, self.rotary,
+                                                  self.q_norm.eps)
+            else:
+                q, k = student_ops.rotary_embedding(q, k, positions, self.rotary)
+            q, k = q.transpose(1, 2), k.transpose(1, 2)
+        else:
+            if self.q_norm is not None:
+                q, k = self.q_norm(q), self.k_norm(k)
+            cos, sin = self.cos[:t].to(x.dtype), self.sin[:t].to(x.dtype)
+            q, k = rotate(q.transpose(1, 2), cos, sin), rotate(k.transpose(1, 2), cos, sin)
         rep = self.hq // self.hkv
         k = k.repeat_interleave(rep, dim=1)
         v = v.repeat_interleave(rep, dim=1)
@@ -85,23 +108,26 @@ class Attention(nn.Module):
 
 
 class MLP(nn.Module):
-    def __init__(self, d, ff):
+    def __init__(self, d, ff, ops=False):
         super().__init__()
+        self.ops = ops
         self.gate = nn.Linear(d, ff, bias=False)
         self.up = nn.Linear(d, ff, bias=False)
         self.down = nn.Linear(ff, d, bias=False)
 
     def forward(self, x):
+        if self.ops:
+            return self.down(student_ops.gated_linear_unit(x, self.gate.weight, self.up.weight, activation="silu"))
         return self.down(F.silu(self.gate(x)) * self.up(x))
 
 
 class Block(nn.Module):
-    def __init__(self, cfg, seq):
+    def __init__(self, cfg, seq, qk_norm=False, ops=False):
         super().__init__()
         d = cfg["dim"]
         self.n1, self.n2 = RMSNorm(d), RMSNorm(d)
-        self.attn = Attention(d, cfg["q_heads"], cfg["kv_heads"], seq)
-        self.mlp = MLP(d, cfg["ffn_dim"])
+        self.attn = Attention(d, cfg["q_heads"], cfg["kv_heads"], seq, qk_norm, ops)
+        self.mlp = MLP(d, cfg["ffn_dim"], ops)
 
     def forward(self, x):
         x = x + self.attn(self.n1(x))
@@ -111,11 +137,11 @@ class Block(nn.Module):
 class TinyLM(nn.Module):
     """Decoder with the lm_head tied to the token embedding; ``hidden`` returns the final normed states."""
 
-    def __init__(self, vocab, cfg, seq):
+    def __init__(self, vocab, cfg, seq, qk_norm=False, ops=False):
         super().__init__()
         self.embed = nn.Embedding(vocab, cfg["dim"])
         nn.init.normal_(self.embed.weight, std=0.02)
-        self.blocks = nn.ModuleList(Block(cfg, seq) for _ in range(cfg["n_layers"]))
+        self.blocks = nn.ModuleList(Block(cfg, seq, qk_norm, ops) for _ in range(cfg["n_layers"]))
         self.norm = RMSNorm(cfg["dim"])
 
     @property
@@ -159,11 +185,13 @@ def fused_loss(h_s, w_s, labels, teacher, z_t=None, h_t=None, w_t=None):
 
 
 # ------------------------------------------------------------------------------------------ step
-def make_step(backend, teacher, vocab, seq, device, dtype=torch.bfloat16):
+def make_step(backend, teacher, vocab, seq, device, dtype=torch.bfloat16, qk_norm=False, clip_norm=None):
     torch.manual_seed(0)
-    student = TinyLM(vocab, STUDENT_CFG, seq).to(device=device, dtype=dtype)
-    teacher_lm = TinyLM(vocab, TEACHER_CFG, seq).to(device=device, dtype=dtype).requires_grad_(False)
+    ops = backend == "orda_b200-ops"
+    student = TinyLM(vocab, STUDENT_CFG, seq, qk_norm, ops).to(device=device, dtype=dtype)
+    teacher_lm = TinyLM(vocab, TEACHER_CFG, seq, qk_norm, ops).to(device=device, dtype=dtype).requires_grad_(False)
     opt = torch.optim.SGD(student.parameters(), lr=1e-3)
+    clip = student_ops.clip_grad_norm_ if ops else torch.nn.utils.clip_grad_norm_
     ids = torch.randint(0, vocab, (BATCH, seq), device=device)
     labels = torch.randint(0, vocab, (BATCH * seq,), device=device)
     d = STUDENT_CFG["dim"]
@@ -208,19 +236,21 @@ def make_step(backend, teacher, vocab, seq, device, dtype=torch.bfloat16):
         opt.zero_grad(set_to_none=True)
         loss = run(ids, labels)
         loss.backward()
+        if clip_norm is not None:
+            clip(student.parameters(), clip_norm)
         opt.step()
         return loss
 
     return step
 
 
-def time_backend(backend, teacher, vocab, seq, steps, device="cuda"):
+def time_backend(backend, teacher, vocab, seq, steps, device="cuda", qk_norm=False, clip_norm=None):
     """(ms per step, peak MB during the timed steps); inf on out-of-memory."""
     torch._dynamo.reset()
     gc.collect()
     torch.cuda.empty_cache()
     try:
-        step = make_step(backend, teacher, vocab, seq, device)
+        step = make_step(backend, teacher, vocab, seq, device, qk_norm=qk_norm, clip_norm=clip_norm)
         for _ in range(WARMUP):
             step()
         torch.cuda.synchronize()
@@ -251,6 +281,8 @@ def main(argv=None) -> int:
     p.add_argument("--steps", type=int, default=50)
     p.add_argument("--passes", type=int, default=2)
     p.add_argument("--backends", nargs="+", default=BACKENDS, choices=BACKENDS)
+    p.add_argument("--qk-norm", action="store_true", help="RMS norms on query and key heads")
+    p.add_argument("--clip-norm", type=float, default=None, help="clip gradients to this global norm")
     p.add_argument("--json", default=None)
     a = p.parse_args(argv)
     if not torch.cuda.is_available():
@@ -262,9 +294,11 @@ def main(argv=None) -> int:
             for ps in range(a.passes):
                 order = a.backends if ps % 2 == 0 else list(reversed(a.backends))
                 for b in order:
-                    acc[b].append(time_backend(b, a.teacher, vocab, seq, a.steps))
+                    acc[b].append(time_backend(b, a.teacher, vocab, seq, a.steps, qk_norm=a.qk_norm,
+                                               clip_norm=a.clip_norm))
             print(f"\n-- {a.teacher}  vocab={vocab // 1024}k  seq={seq}  batch={BATCH}")
-            rec = {"teacher": a.teacher, "vocab": vocab, "seq": seq, "batch": BATCH}
+            rec = {"teacher": a.teacher, "vocab": vocab, "seq": seq, "batch": BATCH, "qk_norm": a.qk_norm,
+                   "clip_norm": a.clip_norm}
             for b in a.backends:
                 ms = sum(x[0] for x in acc[b]) / len(acc[b])
                 mb = max(x[1] for x in acc[b])

@@ -294,7 +294,8 @@ def grad_norm(gradients: Iterable[torch.Tensor]) -> torch.Tensor:
 def clip_gradients(gradients: Iterable[torch.Tensor], max_norm: float, *,
                    eps: float = 1e-6) -> tuple[list[torch.Tensor], torch.Tensor]:
     """``(clipped, norm)``: new tensors ``g * min(1, max_norm / (norm + eps))`` and the norm over all of them
-    before clipping (0-dim fp32). The gradients themselves stay as they are. A norm that is infinite or
+    before clipping (0-dim fp32). The gradients themselves stay as they are. Results of up to 16 MiB in all
+    share one allocation. A norm that is infinite or
     NaN passes into the values, as in ``torch.nn.utils.clip_grad_norm_``. No synchronisation."""
     return (_binding or _bound()).clip_gradients(list(gradients), max_norm, eps)
 

@@ -628,6 +628,35 @@ def test_operators_and_loss_in_one_step():
         within(t.grad, w, w.abs() * (half(t.dtype) + 2.0 ** -22))
 
 
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_training_benchmark_model_through_the_operators(qk_norm):
+    """The training benchmark's decoder with its rotations, norms and feed-forward blocks through the
+    operators, against the same weights through plain PyTorch in 64 bits."""
+    from orda_ce_kernel.benchmarks.train_step import TinyLM
+
+    cfg = dict(dim=256, q_heads=4, kv_heads=2, n_layers=2, ffn_dim=704)
+    torch.manual_seed(3)
+    plain = TinyLM(500, cfg, 64, qk_norm).cuda().double()
+    fused = TinyLM(500, cfg, 64, qk_norm, ops=True).cuda()
+    fused.load_state_dict(plain.state_dict())  # fp32 copies of the same weights
+    ids = torch.randint(0, 500, (2, 48), device="cuda")
+    dy = randn(2, 48, 256, seed=9)
+    for lm in (plain, fused):
+        (lm.hidden(ids) * dy.to(lm.embed.weight.dtype)).sum().backward()
+    for (name, a), (_, b) in zip(fused.named_parameters(), plain.named_parameters()):
+        # fp32 against fp64 through two layers: sums of up to 704 terms at 2^-24 each step
+        rel = float((a.grad.double() - b.grad).norm() / b.grad.norm())
+        assert rel < 1e-4, (name, rel)
+
+
+def test_training_benchmark_step_clips_through_the_operators():
+    from orda_ce_kernel.benchmarks import train_step
+
+    step = train_step.make_step("orda_b200-ops", "separate-student", 32_768, 128, "cuda", qk_norm=True, clip_norm=0.5)
+    first, second = float(step()), float(step())
+    assert math.isfinite(first) and math.isfinite(second) and first != second
+
+
 @pytest.mark.parametrize("act", ["silu"])
 def test_compiled_calls_match_eager(act):
     x, gate, up, dh = glu_inputs(40, 66, 75, BF16, 500)

@@ -138,6 +138,29 @@ def test_config_survives_its_plain_values():
         assert (back.layout, back.dim, back.head_dim) == (c.layout, c.dim, c.head_dim)
 
 
+def test_config_copies_and_pickles():
+    import copy
+    import pickle
+
+    c = student.RotaryConfig(64, scaling="yarn", factor=2.0)
+    student._plan(c)
+    for d in (copy.deepcopy(c), pickle.loads(pickle.dumps(c)), copy.copy(c)):
+        assert d == c and hash(d) == hash(c) and d.frequencies() == c.frequencies()
+        student._plan(d)
+
+
+def test_training_benchmark_model_without_operators_runs_on_cpu():
+    from orda_ce_kernel.benchmarks import train_step
+
+    cfg = dict(dim=32, q_heads=4, kv_heads=2, n_layers=1, ffn_dim=64)
+    ids = torch.randint(0, 97, (2, 8))
+    lm = train_step.TinyLM(97, cfg, 8, qk_norm=True)
+    lm.hidden(ids).sum().backward()
+    assert lm.blocks[0].attn.q_norm.scale.grad is not None
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        train_step.TinyLM(97, cfg, 8, ops=True).hidden(ids)
+
+
 # ------------------------------------------------------------------------------------------ C boundary
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="needs gcc")
 def test_struct_mirrors_match_the_header(tmp_path):
