@@ -51,8 +51,9 @@ typedef struct orda_glu_args {
   void* dweights;                       /* [ceil8(F) + F, H] row stride hidden, or NULL: rows 0 .. F-1 the
                                            gradient of gate, rows ceil8(F) .. that of up; the rows
                                            between (at most 7) hold no value                 */
-  int32_t* device_status;               /* int32 device word, zero on entry; may be NULL for ORDA_F32 and for
-                                           a forward call of at most ORDA_GLU_FEW_ROWS rows  */
+  int32_t* device_status;               /* int32 device word, zero on entry of a forward call; a backward call
+                                           clears it. May be NULL for ORDA_F32 and for a forward call of
+                                           at most ORDA_GLU_FEW_ROWS rows                    */
 } orda_glu_args_t;
 
 /* h (and, where asked for, the products before the activation, which the backward pass reads). */
@@ -82,12 +83,16 @@ typedef struct orda_rotary_args {
   const void* positions; int64_t position_stride[2]; /* [batch, seq] integers                */
   int32_t positions_int64;       /* 1: int64, 0: int32                                       */
   int32_t weight_dtype;
-  const double* frequencies;     /* HOST: rotary_dim / 2 angles (radians) per position       */
+  const uint64_t* turns;         /* HOST: rotary_dim / 2 angles per position, from orda_rotary_turns */
   float magnitude;               /* factor of the rotated values                             */
   float eps;
   const void* weight[2];         /* [D] norm weights, both NULL: no norm                     */
   void* dweight[2];              /* [D] their gradients (weight_dtype)                       */
 } orda_rotary_args_t;
+
+/* Angles per position in the kernels' form: out[i] = radians[i] / (2 pi) modulo 1, times 2^64. HOST arrays.
+ * ORDA_ERR_INVALID_ARGUMENT where an angle is not finite. */
+int32_t orda_rotary_turns(const double* radians, int32_t n, uint64_t* out);
 
 /* out = rotate(x) or rotate(weight * x / sqrt(mean x^2 + eps)). */
 int32_t orda_rotary_forward(const orda_rotary_args_t* args, void* stream);

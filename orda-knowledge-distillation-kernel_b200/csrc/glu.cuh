@@ -142,7 +142,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) glu_grad_kernel(const T* __restrict__ dh, int64_t ld_dh, int dh_vec,
                                                        const T* __restrict__ g, const T* __restrict__ u,
                                                        T* __restrict__ out, int64_t rows, int64_t cols,
-                                                       int64_t cols_pad, int64_t ld, int act) {
+                                                       int64_t cols_pad, int64_t ld, int act, int32_t* status) {
+  if (status && blockIdx.x == 0 && threadIdx.x == 0) *status = 0;  // for the gradient GEMMs that follow
   const int64_t vecs = cols_pad / 8, total = rows * vecs;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {

@@ -15,11 +15,17 @@ namespace orda {
 inline std::atomic<uint64_t> g_launches{0};
 inline void count_launch(uint64_t n = 1) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
+// SMs of the current device (asked once per device: a launch of a few microseconds calls this twice).
 inline int num_sms() {
+  static std::atomic<int> known[64];
   int dev = 0, n = 0;
   cudaGetDevice(&dev);
+  const bool slot = dev >= 0 && dev < 64;
+  if (slot && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
+  if (n <= 0) return 148;
+  if (slot) known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }

@@ -173,7 +173,7 @@ std::pair<Tensor, Tensor> glu_backward(Tensor dh, const Tensor& x, const Tensor&
   a.dh = dh.data_ptr();
   a.dx = ptr(dx);
   a.dweights = ptr(dw);
-  if (dt != at::kFloat) status = new_status(x, s);
+  if (dt != at::kFloat) status = new_empty({1}, at::kInt, x);  // the call clears it
   a.device_status = static_cast<int32_t*>(ptr(status));
   const size_t bytes = orda_glu_backward_workspace_bytes(&a);
   ws = new_empty({static_cast<int64_t>(bytes)}, at::kByte, x);
@@ -257,15 +257,17 @@ std::tuple<Tensor, Tensor, Tensor> glu_backward_op(const Tensor& dh, const Tenso
 // ------------------------------------------------------------------ rotary positions
 // What a RotaryConfig says, in the form the kernels take.
 struct RotaryPlan : torch::CustomClassHolder {
-  std::vector<double> frequencies;
+  std::vector<uint64_t> turns;
   int32_t head_dim, rotary_dim, layout;
   float magnitude;
-  RotaryPlan(std::vector<double> f, int64_t head_dim_, bool interleaved, double magnitude_)
-      : frequencies(std::move(f)), head_dim(static_cast<int32_t>(head_dim_)),
+  RotaryPlan(const std::vector<double>& frequencies, int64_t head_dim_, bool interleaved, double magnitude_)
+      : turns(frequencies.size()), head_dim(static_cast<int32_t>(head_dim_)),
         rotary_dim(static_cast<int32_t>(2 * frequencies.size())),
         layout(interleaved ? ORDA_ROTARY_INTERLEAVED : ORDA_ROTARY_HALF), magnitude(static_cast<float>(magnitude_)) {
     TORCH_CHECK_VALUE(head_dim >= rotary_dim && head_dim <= ORDA_ROTARY_MAX_DIM, "rotary plan of ", rotary_dim, " of ",
                       head_dim, " elements");
+    check_status(orda_rotary_turns(frequencies.data(), static_cast<int32_t>(turns.size()), turns.data()),
+                 "orda_rotary_turns");
   }
 };
 using PlanPtr = c10::intrusive_ptr<RotaryPlan>;
@@ -333,7 +335,7 @@ orda_rotary_args_t rotary_args(const Tensor& q, const Tensor& k, const Tensor& p
   a.position_stride[0] = positions.dim() == 2 ? positions.stride(0) : 0;
   a.position_stride[1] = positions.stride(-1);
   a.positions_int64 = positions.scalar_type() == at::kLong;
-  a.frequencies = plan.frequencies.data();
+  a.turns = plan.turns.data();
   a.magnitude = plan.magnitude;
   return a;
 }
@@ -420,16 +422,18 @@ struct QkNormRotaryFunction : torch::autograd::Function<QkNormRotaryFunction> {
   }
 };
 
-variable_list rotary_embedding(const Tensor& q_, const Tensor& k_, const Tensor& positions, PlanPtr plan) {
+std::tuple<Tensor, Tensor> two(const variable_list& v) { return {v[0], v[1]}; }
+
+std::tuple<Tensor, Tensor> rotary_embedding(const Tensor& q_, const Tensor& k_, const Tensor& positions, PlanPtr plan) {
   check_qk("rotary_embedding", q_, k_, positions, *plan);
   require_cuda("rotary_embedding", q_, {&k_, &positions});
   const Tensor q = dense_last(q_), k = dense_last(k_);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad()))
-    return RotaryFunction::apply(q, k, positions, plan);
-  return rotate(q, k, positions, *plan, false, {}, {}, 0.0);
+    return two(RotaryFunction::apply(q, k, positions, plan));
+  return two(rotate(q, k, positions, *plan, false, {}, {}, 0.0));
 }
 
-variable_list qk_norm_rotary(const Tensor& q_, const Tensor& k_, const Tensor& q_weight, const Tensor& k_weight,
+std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q_, const Tensor& k_, const Tensor& q_weight, const Tensor& k_weight,
                              const Tensor& positions, PlanPtr plan, double eps) {
   check_qk("qk_norm_rotary", q_, k_, positions, *plan);
   check_norm_weights("qk_norm_rotary", q_weight, k_weight, *plan, eps);
@@ -437,8 +441,8 @@ variable_list qk_norm_rotary(const Tensor& q_, const Tensor& k_, const Tensor& q
   const Tensor q = dense_last(q_), k = dense_last(k_), wq = q_weight.contiguous(), wk = k_weight.contiguous();
   if (at::GradMode::is_enabled() &&
       (q.requires_grad() || k.requires_grad() || wq.requires_grad() || wk.requires_grad()))
-    return QkNormRotaryFunction::apply(q, k, wq, wk, positions, plan, eps);
-  return rotate(q, k, positions, *plan, false, wq, wk, eps);
+    return two(QkNormRotaryFunction::apply(q, k, wq, wk, positions, plan, eps));
+  return two(rotate(q, k, positions, *plan, false, wq, wk, eps));
 }
 
 // Without autograd, for the custom ops.
@@ -583,7 +587,7 @@ Tensor clip_in_place(const std::vector<Tensor>& grads, double max_norm, double e
 PYBIND11_MODULE(_student, m) {
   using torch::wrap_pybind_function_no_gil;
   py::class_<RotaryPlan, PlanPtr>(m, "RotaryPlan")
-      .def(py::init<std::vector<double>, int64_t, bool, double>());
+      .def(py::init<const std::vector<double>&, int64_t, bool, double>());
   m.def("gated_linear_unit", wrap_pybind_function_no_gil(gated_linear_unit));
   m.def("activation_code", torch::wrap_pybind_function(activation_code));
   m.def("glu_forward", wrap_pybind_function_no_gil(glu_forward_op));

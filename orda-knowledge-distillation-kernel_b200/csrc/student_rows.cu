@@ -34,9 +34,7 @@ int check_rotary(const orda_rotary_args_t* a, bool backward) {
     return ORDA_ERR_INVALID_ARGUMENT;
   if (backward && (!a->dweight[0] || !a->dweight[1])) return ORDA_ERR_INVALID_ARGUMENT;
   if (a->batch * a->seq > 0) {
-    if (!a->positions || (a->rotary_dim > 0 && !a->frequencies)) return ORDA_ERR_INVALID_ARGUMENT;
-    for (int i = 0; i < a->rotary_dim / 2; ++i)
-      if (!std::isfinite(a->frequencies[i])) return ORDA_ERR_INVALID_ARGUMENT;
+    if (!a->positions || (a->rotary_dim > 0 && !a->turns)) return ORDA_ERR_INVALID_ARGUMENT;
     for (int i = 0; i < 2; ++i)
       if (a->heads[i] > 0 && (!a->x[i] || !a->out[i] || (backward && !a->dy[i]))) return ORDA_ERR_INVALID_ARGUMENT;
   }
@@ -105,12 +103,7 @@ RotaryPlan plan_rotary(const orda_rotary_args_t* a, bool backward) {
   p.magnitude = a->magnitude;
   p.sin_sign = (a->inverse != 0) != backward ? -1.f : 1.f;
   p.eps = a->eps;
-  const long double two_pi = 6.283185307179586476925286766559L;
-  for (int i = 0; i < a->rotary_dim / 2; ++i) {
-    long double turn = a->frequencies[i] / two_pi;
-    turn -= floorl(turn);
-    p.turns[i] = static_cast<uint64_t>(turn * 18446744073709551616.0L);
-  }
+  for (int i = 0; i < a->rotary_dim / 2; ++i) p.turns[i] = a->turns[i];
   const int slots = static_cast<int>(cdiv(a->head_dim, 2 * r.width));
   p.lanes = 1;
   while (p.lanes < slots && p.lanes < 32) p.lanes *= 2;
@@ -254,6 +247,19 @@ int clip_launches(const orda_tensor_list_t* l, double max_norm, double eps, floa
 }  // namespace
 
 extern "C" {
+
+int32_t orda_rotary_turns(const double* radians, int32_t n, uint64_t* out) {
+  if (n < 0 || (n > 0 && (!radians || !out))) return ORDA_ERR_INVALID_ARGUMENT;
+  const long double two_pi = 6.283185307179586476925286766559L;
+  for (int32_t i = 0; i < n; ++i) {
+    if (!std::isfinite(radians[i])) return ORDA_ERR_INVALID_ARGUMENT;
+    long double turn = radians[i] / two_pi;
+    turn -= floorl(turn);
+    turn *= 18446744073709551616.0L;
+    out[i] = turn < 18446744073709551616.0L ? static_cast<uint64_t>(turn) : 0u;  // (a tiny negative angle rounds to a whole turn)
+  }
+  return ORDA_OK;
+}
 
 int32_t orda_rotary_forward(const orda_rotary_args_t* args, void* stream) {
   const int rc = check_rotary(args, false);

@@ -127,7 +127,7 @@ class RotaryArgs(ctypes.Structure):
         ("dy", _vp * 2), ("dy_stride", _i64 * 6),
         ("positions", _vp), ("position_stride", _i64 * 2),
         ("positions_int64", _i32), ("weight_dtype", _i32),
-        ("frequencies", _vp),
+        ("turns", _vp),
         ("magnitude", _f32), ("eps", _f32),
         ("weight", _vp * 2), ("dweight", _vp * 2),
     ]
@@ -166,6 +166,7 @@ EXPORTED_SYMBOLS = (
     "orda_glu_forward",
     "orda_glu_backward_workspace_bytes",
     "orda_glu_backward",
+    "orda_rotary_turns",
     "orda_rotary_forward",
     "orda_qk_norm_rotary_backward_workspace_bytes",
     "orda_qk_norm_rotary_backward",
@@ -230,6 +231,8 @@ def _declare(lib):
     lib.orda_glu_backward_workspace_bytes.argtypes = [PG]
     lib.orda_glu_backward.restype = _i32
     lib.orda_glu_backward.argtypes = [PG, _vp, ctypes.c_size_t, _vp]
+    lib.orda_rotary_turns.restype = _i32
+    lib.orda_rotary_turns.argtypes = [ctypes.POINTER(ctypes.c_double), _i32, ctypes.POINTER(ctypes.c_uint64)]
     lib.orda_rotary_forward.restype = _i32
     lib.orda_rotary_forward.argtypes = [PR, _vp]
     lib.orda_qk_norm_rotary_backward_workspace_bytes.restype = ctypes.c_size_t

@@ -265,7 +265,7 @@ def rotary_embedding(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     _require_config("rotary_embedding", config)
     if torch.compiler.is_compiling():
         return torch.ops.orda_b200.rotary(q, k, positions, None, None, 0.0, False, *_config_values(config))
-    return tuple((_binding or _bound()).rotary_embedding(q, k, positions, config._plan or _plan(config)))
+    return (_binding or _bound()).rotary_embedding(q, k, positions, config._plan or _plan(config))
 
 
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -280,8 +280,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
     if torch.compiler.is_compiling():
         return torch.ops.orda_b200.rotary(q, k, positions, q_weight, k_weight, float(eps), False,
                                           *_config_values(config))
-    return tuple((_binding or _bound()).qk_norm_rotary(q, k, q_weight, k_weight, positions,
-                                                       config._plan or _plan(config), eps))
+    return (_binding or _bound()).qk_norm_rotary(q, k, q_weight, k_weight, positions, config._plan or _plan(config), eps)
 
 
 # ------------------------------------------------------------------------------------------ gradient norm and clipping

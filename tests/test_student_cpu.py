@@ -208,9 +208,9 @@ def test_c_glu_backward_checks():
 
 
 def _rot(**kw):
-    f = (ctypes.c_double * 4)(1.0, 0.1, 0.01, 0.001)
+    f = (ctypes.c_uint64 * 4)(1, 2, 3, 4)
     a = dict(abi_version=_native.ABI_VERSION, dtype=_native.BF16, batch=1, seq=2, heads=(2, 1), head_dim=8, rotary_dim=8,
-             layout=0, x=(16, 16), out=(16, 16), positions=16, frequencies=ctypes.addressof(f), magnitude=1.0) | kw
+             layout=0, x=(16, 16), out=(16, 16), positions=16, turns=ctypes.addressof(f), magnitude=1.0) | kw
     return _native.RotaryArgs(**a), f
 
 
@@ -218,13 +218,26 @@ def _rot(**kw):
     (dict(abi_version=9), _native.ERR_INVALID_ARGUMENT), (dict(rotary_dim=7), _native.ERR_INVALID_ARGUMENT),
     (dict(rotary_dim=10), _native.ERR_INVALID_ARGUMENT), (dict(layout=2), _native.ERR_INVALID_ARGUMENT),
     (dict(head_dim=1024, rotary_dim=8), _native.ERR_UNSUPPORTED), (dict(positions=None), _native.ERR_INVALID_ARGUMENT),
-    (dict(frequencies=None), _native.ERR_INVALID_ARGUMENT), (dict(x=(16, None)), _native.ERR_INVALID_ARGUMENT),
+    (dict(turns=None), _native.ERR_INVALID_ARGUMENT), (dict(x=(16, None)), _native.ERR_INVALID_ARGUMENT),
     (dict(weight=(16, None)), _native.ERR_INVALID_ARGUMENT), (dict(batch=1 << 20, seq=1 << 20), _native.ERR_UNSUPPORTED),
     (dict(batch=0), _native.OK), (dict(heads=(0, 0)), _native.OK),
 ])
 def test_c_rotary_checks(kw, code):
     a, _f = _rot(**kw)
     assert _native.load().orda_rotary_forward(a, None) == code
+
+
+def test_c_rotary_turns():
+    lib = _native.load()
+    angles = [0.0, 1.0, 2 * math.pi * 0.25, -1.0, 1e-18, -1e-30, 2.5e9]
+    out = (ctypes.c_uint64 * len(angles))()
+    assert lib.orda_rotary_turns((ctypes.c_double * len(angles))(*angles), len(angles), out) == _native.OK
+    for a, t in zip(angles, out):
+        off = (t / 2.0 ** 64 - a / (2 * math.pi)) % 1.0
+        assert min(off, 1.0 - off) <= 2.0 ** -53 * (1 + abs(a)), a
+    for bad in (math.inf, math.nan):
+        assert lib.orda_rotary_turns((ctypes.c_double * 1)(bad), 1, out) == _native.ERR_INVALID_ARGUMENT
+    assert lib.orda_rotary_turns(None, 1, out) == _native.ERR_INVALID_ARGUMENT
 
 
 def test_c_norm_backward_checks():
