@@ -57,8 +57,7 @@ int glu_rows_launch(const orda_glu_args_t* a, cudaStream_t s) {
 template <typename T16>
 int glu_swap_launch(const orda_glu_args_t* a, cudaStream_t s) {
   GluSwapParams p{};
-  int tokens = 16;
-  while (tokens < a->rows && tokens < 128) tokens *= 2;
+  const int tokens = static_cast<int>(std::min<int64_t>(128, cdiv(a->rows, 16) * 16));
   int rc;
   if ((rc = make_map(&p.gate, a->dtype, a->gate, a->hidden, a->ffn, a->ld_gate, 64, kSwapFeatures))) return rc;
   if ((rc = make_map(&p.up, a->dtype, a->up, a->hidden, a->ffn, a->ld_up, 64, kSwapFeatures))) return rc;

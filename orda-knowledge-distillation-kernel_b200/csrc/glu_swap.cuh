@@ -33,7 +33,7 @@ struct GluSwapParams {
   CUtensorMap gate, up, x;  // boxes: 64 x 64 of the weights, 64 x tokens of x
   void *h, *pre_gate, *pre_up;
   int64_t ld_h, ld_pre, ffn, rows;
-  int32_t tokens;           // tokens of a tile: 16, 32, 64 or 128
+  int32_t tokens;           // tokens of a tile: a multiple of 16, at most 128
   int32_t stages, kb, kb_part, act;  // k blocks: all, of one block of the cluster
   int32_t split;            // blocks of the cluster
   uint32_t idesc;
@@ -68,7 +68,8 @@ __global__ void __launch_bounds__(kSwapThreads, 2) glu_swap_kernel(const __grid_
   auto empty_bar = [&](int s) { return bar + 8u * (8 + s); };
   const uint32_t done_bar = bar + 8u * 16;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t tmem_cols = p.tokens < 32 ? 32u : static_cast<uint32_t>(p.tokens);
+  uint32_t tmem_cols = 32;  // a power of two
+  while (tmem_cols < static_cast<uint32_t>(p.tokens)) tmem_cols *= 2;
   const int part = static_cast<int>(blockIdx.x) % p.split;
   const int64_t t0 = static_cast<int64_t>(blockIdx.z) * p.tokens;
   const int64_t f0 = (static_cast<int64_t>(blockIdx.x) / p.split) * kSwapFeatures;
