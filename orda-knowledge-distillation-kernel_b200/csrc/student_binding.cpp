@@ -303,11 +303,13 @@ void check_norm_weights(const char* what, const Tensor& wq, const Tensor& wk, co
 
 Tensor dense_last(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 
+// Element strides of batch, sequence and heads; the stride of a dimension of one means nothing and counts as 0.
 void strides_of(const Tensor& t, int64_t (&out)[3]) {
   const int o = t.dim() == 4;
-  out[0] = o ? t.stride(0) : 0;
-  out[1] = t.stride(o);
-  out[2] = t.stride(o + 1);
+  auto stride = [&](int d) { return t.size(d) > 1 ? t.stride(d) : 0; };
+  out[0] = o ? stride(0) : 0;
+  out[1] = stride(o);
+  out[2] = stride(o + 1);
 }
 
 orda_rotary_args_t rotary_args(const Tensor& q, const Tensor& k, const Tensor& positions, const RotaryPlan& plan,

@@ -512,6 +512,123 @@ def test_clip_refuses_a_gradient_twice():
     assert float(student.grad_norm([p.grad, p.grad])) == pytest.approx(math.sqrt(8.0))
 
 
+def test_clip_offsets_behind_32_bits():
+    g = torch.zeros(2 ** 31 + 77, device="cuda", dtype=BF16)
+    g[-1], g[2 ** 31 - 1], g[5] = 3.0, 4.0, 12.0
+    clipped, norm = student.clip_gradients([g], 6.5, eps=0.0)
+    assert float(norm) == 13.0
+    at = torch.tensor([5, 2 ** 31 - 1, 2 ** 31 + 76], device="cuda")
+    assert clipped[0][at].tolist() == [6.0, 2.0, 1.5] and int((clipped[0] != 0).sum()) == 3
+
+
+# ------------------------------------------------------------------------------------------ calls of every kind
+def test_offsets_behind_32_bits():
+    """Rows, tokens and heads whose element offsets do not fit 32 bits."""
+    far = 2 ** 31 + 64
+    buf = torch.zeros(far + 4096, device="cuda", dtype=BF16)
+    cfg, pos = student.RotaryConfig(64), torch.tensor([[5], [9]], device="cuda")
+    q = torch.as_strided(buf, (2, 1, 3, 64), (far, 64, 64, 1))
+    small = randn(2, 1, 3, 64, seed=1, dtype=BF16)
+    q.copy_(small)
+    w = torch.ones(64, device="cuda")
+    for a, b in zip(student.qk_norm_rotary(q, q, w, w, pos, cfg), student.qk_norm_rotary(small, small, w, w, pos, cfg)):
+        assert torch.equal(a, b)
+    for n in (2, 9, 140):  # each kernel of the feed-forward block
+        ld = (far // (n - 1) + 8) // 8 * 8
+        x = torch.as_strided(torch.zeros(ld * (n - 1) + 64, device="cuda", dtype=BF16), (n, 64), (ld, 1))
+        small = randn(n, 64, seed=2, dtype=BF16)
+        x.copy_(small)
+        _, wg, wu, _ = glu_inputs(1, 64, 72, BF16, 3)
+        assert torch.equal(student.gated_linear_unit(x, wg, wu), student.gated_linear_unit(small, wg, wu))
+
+
+def test_glu_results_behind_32_bits():
+    n, h, f = 270_000, 16, 8192
+    x, wg, wu = randn(n, h, seed=1, dtype=BF16), randn(f, h, seed=2, dtype=BF16), randn(f, h, seed=3, dtype=BF16)
+    leaf = x.detach().requires_grad_(True)
+    y = student.gated_linear_unit(leaf, wg, wu, activation="relu")
+    dh = torch.zeros_like(y)
+    rows = torch.tensor([0, 262_143, 262_144, n - 1], device="cuda")
+    dh[rows] = randn(4, f, seed=4, dtype=BF16)
+    (dx,) = torch.autograd.grad(y, leaf, dh)
+    want = glu64(x[rows], wg, wu, "relu", dh[rows])
+    within(y[rows], *want["h"], "h")
+    within(dx[rows], *want["dx"], "dx")
+    dx[rows] = 0
+    assert not dx.any()
+
+
+def test_second_derivatives_are_refused():
+    x, wg, wu, _ = glu_inputs(6, 16, 24, FP32, 5)
+    q, w = randn(6, 2, 16, seed=6), torch.ones(16, device="cuda")
+    pos, cfg = torch.arange(6, device="cuda"), student.RotaryConfig(16)
+    for leaf, call in ((x, lambda t: student.gated_linear_unit(t, wg, wu)),
+                       (q, lambda t: student.rotary_embedding(t, t, pos, cfg)[0]),
+                       (q, lambda t: student.qk_norm_rotary(t, t, w, w, pos, cfg)[0])):
+        leaf = leaf.detach().requires_grad_(True)
+        (g,) = torch.autograd.grad(call(leaf).square().sum(), leaf, create_graph=True)
+        (plain,) = torch.autograd.grad(call(leaf).square().sum(), leaf)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
+def test_backward_twice_and_kept_graph():
+    x, wg, wu, dh = glu_inputs(40, 64, 72, BF16, 7)
+    leaf = x.detach().requires_grad_(True)
+    y = student.gated_linear_unit(leaf, wg, wu)
+    first = torch.autograd.grad(y, leaf, dh, retain_graph=True)[0]
+    assert torch.equal(first, torch.autograd.grad(y, leaf, dh)[0])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, leaf, dh)
+
+
+def test_mixed_types_inference_mode_and_single_sizes():
+    x, wg, wu, _ = glu_inputs(12, 64, 72, BF16, 8)
+    want = student.gated_linear_unit(x, wg, wu)
+    with torch.inference_mode():
+        assert torch.equal(student.gated_linear_unit(x.float(), wg, wu.float()), want)  # bf16 wins
+    leaf = x.float().requires_grad_(True)
+    student.gated_linear_unit(leaf, wg, wu).sum().backward()
+    assert leaf.grad.dtype == FP32
+    # dimensions of one element may have any stride
+    one = torch.as_strided(x, (1, 64), (7, 1))
+    assert torch.equal(student.gated_linear_unit(one, wg, wu), want[:1])
+    q = torch.as_strided(randn(1, 5, 1, 64, seed=9, dtype=BF16), (1, 5, 1, 64), (3, 64, 1, 1))
+    check_rotary(q, q, torch.arange(5, device="cuda"), student.RotaryConfig(64))
+
+
+def test_calls_from_several_threads():
+    import threading
+
+    x, wg, wu, dh = glu_inputs(40, 64, 72, BF16, 10)
+    grads = [randn(500, seed=i) for i in range(120)]
+    want = student.gated_linear_unit(x, wg, wu)
+    want_clip, want_norm = student.clip_gradients(grads, 1.0)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                leaf = x.detach().requires_grad_(True)
+                y = student.gated_linear_unit(leaf, wg, wu)
+                torch.autograd.grad(y, leaf, dh)
+                clipped, norm = student.clip_gradients(grads, 1.0)
+            stream.synchronize()
+        if not (torch.equal(y, want) and torch.equal(norm, want_norm)
+                and all(torch.equal(a, b) for a, b in zip(clipped, want_clip))):
+            wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 # ------------------------------------------------------------------------------------------ together, streams, graphs
 def _step(x, gate, up, wq, wk, qkv, pos, cfg):
     """Forward, backward and clipping of the operators in a row, as a student's layer would run them."""
