@@ -46,15 +46,23 @@ typedef struct orda_glu_args {
   void* pre_gate; int64_t ld_pre;       /* [N, F] x Wgate^T, written where not NULL          */
   void* pre_up;                         /* [N, F] x Wup^T (both or neither)                  */
   /* backward */
+  int64_t grad_cols;                    /* columns (and row stride) of dx and dweights: H, or fewer where the
+                                           operands' rows end in padding (orda_pad_rows)     */
   const void* dh;                       /* [N, F]                                            */
-  void* dx;                             /* [N, H] row stride hidden, or NULL                 */
-  void* dweights;                       /* [ceil8(F) + F, H] row stride hidden, or NULL: rows 0 .. F-1 the
-                                           gradient of gate, rows ceil8(F) .. that of up; the rows
-                                           between (at most 7) hold no value                 */
+  void* dx;                             /* [N, grad_cols] or NULL                            */
+  void* dweights;                       /* [ceil8(F) + F, grad_cols] or NULL: rows 0 .. F-1 the gradient of
+                                           gate, rows ceil8(F) .. that of up; the rows between (at
+                                           most 7) hold no value                             */
   int32_t* device_status;               /* int32 device word, zero on entry of a forward call; a backward call
                                            clears it. May be NULL for ORDA_F32 and for a forward call of
                                            at most ORDA_GLU_FEW_ROWS rows                    */
 } orda_glu_args_t;
+
+/* Copies of up to three 16-bit matrices (rows of `cols` elements, any alignment, ld[i] elements apart) whose
+ * rows end in zeros at a multiple of 8 elements: operands of the calls below with a hidden size that is
+ * none. dst[i]: [rows[i], ceil8(cols)], 16-byte aligned. HOST arrays of `count`. */
+int32_t orda_pad_rows(int32_t count, const void* const* src, const int64_t* ld, const int64_t* rows, int64_t cols,
+                      void* const* dst, void* stream);
 
 /* h (and, where asked for, the products before the activation, which the backward pass reads). */
 int32_t orda_glu_forward(const orda_glu_args_t* args, void* stream);

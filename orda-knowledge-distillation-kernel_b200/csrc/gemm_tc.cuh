@@ -56,7 +56,8 @@ struct TcGemmParams {
   // wide kernel, store epilogue with st_tma = 1: the 16-bit output [M, N] (64 x 32 boxes, 128-byte
   // swizzle); the epilogue stages each 32-row x 64-column piece in shared memory and stores it by TMA
   CUtensorMap out_map;
-  int32_t st_tma;     // 1: 16-bit output; 2: fp32 partials of a k split, out_map is [split, M, N] in 32 x 32 boxes
+  int32_t st_tma;     // 1: 16-bit output; 2: fp32 partials of a k split, out_map is [split, M, N] in 32 x 32 boxes;
+                      // 3: 16-bit output staged alike, but stored row by row (rows that are not 16-byte aligned)
   // with st_tma and rows routed to peers (st.peers > 0, slab_rows a multiple of 512): map k covers
   // this GPU's slot [slab_rows, N] in peer k's slot buffer
   CUtensorMap peer_maps[ORDA_MAX_PEERS];

@@ -248,6 +248,25 @@ __device__ __forceinline__ void wide_store_tma(const TcGemmParams& p, uint32_t t
   }
 }
 
+// The same 32 x 64 pieces for an output whose rows TMA cannot store: plain stores, a row of a piece at a time.
+template <typename T16>
+__device__ __forceinline__ void wide_store_rows(const TcGemmParams& p, uint32_t tbase, uint32_t staging, int64_t y0,
+                                                int64_t n0, int lane) {
+#pragma unroll 1
+  for (int g = 0; g < kPairBN / 64; ++g) {
+    const int64_t c0 = n0 + g * 64;
+    uint32_t r[2][32];
+    tmem_ld32_async(tbase + g * 64, r[0]);
+    tmem_ld32_async(tbase + g * 64 + 32, r[1]);
+    tmem_wait_ld();
+    if (c0 >= p.st.N || y0 >= p.st.M) continue;  // warp-uniform
+    store_piece_rows(static_cast<T16*>(p.st.out), p.st.ldo, p.st.M, p.st.N, staging, y0, c0, lane, [&](int q, int e) {
+      const int i = (q & 3) * 8 + 2 * e;
+      return pack2<T16>(__uint_as_float(r[q >> 2][i]), __uint_as_float(r[q >> 2][i + 1]));
+    });
+  }
+}
+
 // fp32 partials of k split `ks` through shared memory and TMA: the warp's 32 rows x 256 columns leave as eight
 // 32 x 32 pieces of full 128-byte lines (16-byte stores one row per lane touch 32 lines an instruction).
 __device__ __forceinline__ void wide_store_partial_tma(const TcGemmParams& p, uint32_t tbase, uint32_t staging,
@@ -552,6 +571,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThr
           const int64_t y0 = static_cast<int64_t>(mt) * 512 + j * 256 + rank * 128 + quarter * 32;
           if (p.st_tma == 2) {
             wide_store_partial_tma(p, tbase, staging, y0, n0, ks, lane);
+          } else if (p.st_tma == 3) {
+            wide_store_rows<T16>(p, tbase, staging, y0, n0, lane);
           } else if (p.st_tma) {
             wide_store_tma<T16>(p, tbase, staging, y0, n0, lane);
           } else {

@@ -202,4 +202,46 @@ __global__ void __launch_bounds__(256) glu_grad_kernel(const T* __restrict__ dh,
   }
 }
 
+// Rows of 16-bit elements copied into rows of cols_pad (a multiple of 8) that end in zeros.
+struct PadRowsParams {
+  const uint16_t* src[3];
+  uint16_t* dst[3];
+  int64_t ld[3];
+  int64_t last[3];       // vectors of matrices 0 .. i
+  int64_t cols, cols_pad;
+  int32_t count;
+};
+
+static __global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ PadRowsParams p) {
+  const int64_t vecs = p.cols_pad / 8;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < p.last[p.count - 1];
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    int m = 0;
+    while (i >= p.last[m]) ++m;
+    const int64_t at = i - (m ? p.last[m - 1] : 0), row = at / vecs, c = (at - row * vecs) * 8;
+    const uint16_t* s = p.src[m] + row * p.ld[m] + c;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = c + 2 * j < p.cols ? s[2 * j] : 0u, b = c + 2 * j + 1 < p.cols ? s[2 * j + 1] : 0u;
+      w[j] = a | b << 16;
+    }
+    reinterpret_cast<uint4*>(p.dst[m])[at] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// sum_split_kernel for results whose rows are no multiple of 8: partials [split][rows][cols_pad], out [rows, cols].
+template <typename T>
+__global__ void __launch_bounds__(256) sum_split_rows_kernel(const float* part, int splits, int64_t rows, int64_t cols,
+                                                             int64_t cols_pad, T* out) {
+  const int64_t total = rows * cols;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t row = i / cols, at = row * cols_pad + (i - row * cols);
+    float v = part[at];
+    for (int k = 1; k < splits; ++k) v += part[k * rows * cols_pad + at];
+    out[i] = Conv<T>::from_f(v);
+  }
+}
+
 }  // namespace orda

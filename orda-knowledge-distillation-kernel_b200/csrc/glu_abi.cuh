@@ -25,6 +25,7 @@ int check_glu(const orda_glu_args_t* a, bool backward) {
       ((a->pre_gate || backward) && a->ld_pre < a->ffn))
     return ORDA_ERR_INVALID_ARGUMENT;
   if (backward) {
+    if (a->grad_cols < 1 || a->grad_cols > a->hidden) return ORDA_ERR_INVALID_ARGUMENT;
     if (!a->pre_gate || !a->pre_up || !a->dh) return ORDA_ERR_INVALID_ARGUMENT;
   } else if (!a->h || (a->pre_gate == nullptr) != (a->pre_up == nullptr)) {
     return ORDA_ERR_INVALID_ARGUMENT;
@@ -169,12 +170,13 @@ GluPlan plan_glu_backward(const orda_glu_args_t* a) {
   if (a->dtype != ORDA_F32) {
     size_t part = 0;
     if (a->dx) {
-      p.split_dx = glu_split(a->rows, a->hidden, 2 * cdiv(a->ffn, kBK));
-      if (p.split_dx > 1) part = std::max(part, sizeof(float) * p.split_dx * a->rows * a->hidden);
+      p.split_dx = glu_split(a->rows, a->grad_cols, 2 * cdiv(a->ffn, kBK));
+      if (p.split_dx > 1) part = std::max(part, sizeof(float) * p.split_dx * a->rows * round8(a->grad_cols));
     }
     if (a->dweights) {
-      p.split_dw = glu_split(p.fp + a->ffn, a->hidden, cdiv(a->rows, kBK));
-      if (p.split_dw > 1) part = std::max(part, sizeof(float) * p.split_dw * (p.fp + a->ffn) * a->hidden);
+      p.split_dw = glu_split(p.fp + a->ffn, a->grad_cols, cdiv(a->rows, kBK));
+      if (p.split_dw > 1)
+        part = std::max(part, sizeof(float) * p.split_dw * (p.fp + a->ffn) * round8(a->grad_cols));
     }
     off = align256(off + part);
   }
@@ -201,23 +203,34 @@ template <bool A_MN, bool TWO_SEG, typename T16>
 int glu_grad_gemm(TcGemmParams& prm, int dtype, int64_t M, int64_t N, int split, void* out, uint8_t* part,
                   cudaStream_t s) {
   int rc;
+  const int64_t np = round8(N);
   if (split <= 1) {
     prm.st = StoreEpiParams{out, N, M, N, 0, 0};
-    if ((rc = make_map(&prm.out_map, dtype, out, N, M, N, 64, 32))) return rc;  // (clips a last piece at N)
-    prm.st_tma = 1;
+    if (N == np) {
+      if ((rc = make_map(&prm.out_map, dtype, out, N, M, N, 64, 32))) return rc;  // (clips a last piece at N)
+      prm.st_tma = 1;
+    } else {
+      prm.st_tma = 3;
+    }
     return launch_tc2w<A_MN, true, A_PLAIN, TWO_SEG, EPI_STORE, T16>(prm, cdiv(M, 512), N, s, 4);
   }
   prm.ksplit = split;
   prm.kb_split = static_cast<int32_t>(cdiv(prm.kb0 + prm.kb1, split));
-  prm.split_bytes = static_cast<int64_t>(sizeof(float)) * M * N;
-  prm.st = StoreEpiParams{part, N, M, N, 1, 0};
-  if ((rc = make_partial_map(&prm.out_map, part, N, M, split))) return rc;  // (rows of N floats: 32-byte multiples)
+  prm.split_bytes = static_cast<int64_t>(sizeof(float)) * M * np;
+  prm.st = StoreEpiParams{part, np, M, np, 1, 0};
+  if ((rc = make_partial_map(&prm.out_map, part, np, M, split))) return rc;  // (rows of 32-byte multiples)
   prm.st_tma = 2;
   if ((rc = launch_tc2w<A_MN, true, A_PLAIN, TWO_SEG, EPI_STORE, T16>(prm, cdiv(M, 512), N, s, 4))) return rc;
-  const int64_t count8 = M * N / 8;
   count_launch();
-  sum_split_kernel<T16><<<static_cast<int>(std::min<int64_t>(cdiv(count8, 256), 8 * num_sms())), 256, 0, s>>>(
-      reinterpret_cast<const float*>(part), split, M * N, static_cast<T16*>(out), count8);
+  const float* sums = reinterpret_cast<const float*>(part);
+  if (N == np) {
+    const int64_t count8 = M * N / 8;
+    sum_split_kernel<T16><<<static_cast<int>(std::min<int64_t>(cdiv(count8, 256), 8 * num_sms())), 256, 0, s>>>(
+        sums, split, M * N, static_cast<T16*>(out), count8);
+  } else {
+    sum_split_rows_kernel<T16><<<static_cast<int>(std::min<int64_t>(cdiv(M * N, 256), 16 * num_sms())), 256, 0, s>>>(
+        sums, split, M, N, np, static_cast<T16*>(out));
+  }
   return launch_status();
 }
 
@@ -245,10 +258,10 @@ int glu_backward_tc(const orda_glu_args_t* a, const GluPlan& P, uint8_t* ws, cud
     prm.status = a->device_status;
     if ((rc = make_operand_map(&prm.a0, a->dtype, dgu, false, a->rows, a->ffn, ld, kTileRows))) return rc;
     if ((rc = make_operand_map(&prm.a1, a->dtype, dgu + P.fp, false, a->rows, a->ffn, ld, kTileRows))) return rc;
-    if ((rc = make_operand_map(&prm.b0, a->dtype, a->gate, true, a->hidden, a->ffn, a->ld_gate, 128))) return rc;
-    if ((rc = make_operand_map(&prm.b1, a->dtype, a->up, true, a->hidden, a->ffn, a->ld_up, 128))) return rc;
+    if ((rc = make_operand_map(&prm.b0, a->dtype, a->gate, true, a->grad_cols, a->ffn, a->ld_gate, 128))) return rc;
+    if ((rc = make_operand_map(&prm.b1, a->dtype, a->up, true, a->grad_cols, a->ffn, a->ld_up, 128))) return rc;
     prm.kb0 = prm.kb1 = static_cast<int32_t>(cdiv(a->ffn, kBK));
-    if ((rc = glu_grad_gemm<false, true, T16>(prm, a->dtype, a->rows, a->hidden, P.split_dx, a->dx, part, s)))
+    if ((rc = glu_grad_gemm<false, true, T16>(prm, a->dtype, a->rows, a->grad_cols, P.split_dx, a->dx, part, s)))
       return rc;
   }
   if (a->dweights) {  // [dg | du]^T x: both weights' gradients are one product of fp + ffn rows
@@ -256,9 +269,9 @@ int glu_backward_tc(const orda_glu_args_t* a, const GluPlan& P, uint8_t* ws, cud
     prm.status = a->device_status;
     const int64_t m = P.fp + a->ffn;
     if ((rc = make_operand_map(&prm.a0, a->dtype, dgu, true, m, a->rows, ld, kTileRows))) return rc;
-    if ((rc = make_operand_map(&prm.b0, a->dtype, a->x, true, a->hidden, a->rows, a->ld_x, 128))) return rc;
+    if ((rc = make_operand_map(&prm.b0, a->dtype, a->x, true, a->grad_cols, a->rows, a->ld_x, 128))) return rc;
     prm.kb0 = static_cast<int32_t>(cdiv(a->rows, kBK));
-    if ((rc = glu_grad_gemm<true, false, T16>(prm, a->dtype, m, a->hidden, P.split_dw, a->dweights, part, s)))
+    if ((rc = glu_grad_gemm<true, false, T16>(prm, a->dtype, m, a->grad_cols, P.split_dw, a->dweights, part, s)))
       return rc;
   }
   return ORDA_OK;
@@ -284,12 +297,12 @@ int glu_backward_f32(const orda_glu_args_t* a, const GluPlan& P, uint8_t* ws, cu
   const float* x = static_cast<const float*>(a->x);
   if (a->dx) {
     float* dx = static_cast<float*>(a->dx);
-    simt_gemm(dgu, ld, 1, static_cast<const float*>(a->gate), 1, a->ld_gate, dx, a->hidden, a->rows, a->hidden, a->ffn, 0, s);
-    simt_gemm(dgu + P.fp, ld, 1, static_cast<const float*>(a->up), 1, a->ld_up, dx, a->hidden, a->rows, a->hidden, a->ffn, 1, s);
+    simt_gemm(dgu, ld, 1, static_cast<const float*>(a->gate), 1, a->ld_gate, dx, a->grad_cols, a->rows, a->grad_cols, a->ffn, 0, s);
+    simt_gemm(dgu + P.fp, ld, 1, static_cast<const float*>(a->up), 1, a->ld_up, dx, a->grad_cols, a->rows, a->grad_cols, a->ffn, 1, s);
   }
   if (a->dweights) {
     float* dw = static_cast<float*>(a->dweights);
-    simt_gemm(dgu, 1, ld, x, 1, a->ld_x, dw, a->hidden, P.fp + a->ffn, a->hidden, a->rows, 0, s);
+    simt_gemm(dgu, 1, ld, x, 1, a->ld_x, dw, a->grad_cols, P.fp + a->ffn, a->grad_cols, a->rows, 0, s);
   }
   return launch_status();
 }
@@ -297,6 +310,31 @@ int glu_backward_f32(const orda_glu_args_t* a, const GluPlan& P, uint8_t* ws, cu
 }  // namespace
 
 extern "C" {
+
+int32_t orda_pad_rows(int32_t count, const void* const* src, const int64_t* ld, const int64_t* rows, int64_t cols,
+                      void* const* dst, void* stream) {
+  if (count < 0 || count > 3 || cols < 1) return ORDA_ERR_INVALID_ARGUMENT;
+  if (count > 0 && (!src || !ld || !rows || !dst)) return ORDA_ERR_INVALID_ARGUMENT;
+  PadRowsParams p{};
+  p.cols = cols;
+  p.cols_pad = round8(cols);
+  int64_t total = 0;
+  for (int i = 0; i < count; ++i) {
+    if (rows[i] < 0 || (rows[i] > 0 && (!src[i] || !dst[i] || ld[i] < 0))) return ORDA_ERR_INVALID_ARGUMENT;
+    if ((reinterpret_cast<uintptr_t>(src[i]) & 1u) || (reinterpret_cast<uintptr_t>(dst[i]) & 15u))
+      return ORDA_ERR_ALIGNMENT;
+    p.src[i] = static_cast<const uint16_t*>(src[i]);
+    p.dst[i] = static_cast<uint16_t*>(dst[i]);
+    p.ld[i] = ld[i];
+    p.last[i] = total += rows[i] * (p.cols_pad / 8);
+  }
+  if (total == 0) return ORDA_OK;
+  p.count = count;
+  count_launch();
+  pad_rows_kernel<<<static_cast<int>(std::min<int64_t>(cdiv(total, 256), 16 * num_sms())), 256, 0,
+                    static_cast<cudaStream_t>(stream)>>>(p);
+  return launch_status();
+}
 
 int32_t orda_glu_forward(const orda_glu_args_t* args, void* stream) {
   const int rc = check_glu(args, false);
@@ -320,7 +358,7 @@ int32_t orda_glu_backward(const orda_glu_args_t* args, void* workspace, size_t w
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (args->rows == 0) {
     if (args->dweights &&
-        cudaMemsetAsync(args->dweights, 0, esize(args->dtype) * (round8(args->ffn) + args->ffn) * args->hidden, s) !=
+        cudaMemsetAsync(args->dweights, 0, esize(args->dtype) * (round8(args->ffn) + args->ffn) * args->grad_cols, s) !=
             cudaSuccess)
       return ORDA_ERR_CUDA;
     return ORDA_OK;

@@ -389,9 +389,11 @@ __device__ __forceinline__ void group_sum(float (&v)[N], int lanes) {
   }
 }
 
-// slots a lane may have to hold (1 with 8-element vectors: 32 lanes cover 512 elements)
+// NS: slots of a lane. 32 lanes with one slot each cover 512 elements in 8-element vectors, 128 in pairs and 64
+// in single ones; larger heads of the narrow widths take kRotMaxPairs / (32 V) slots, whose unrolled loops
+// would cost the small heads up to eight times their work.
 template <int V>
-constexpr int rotary_slots_per_lane() {
+constexpr int rotary_most_slots() {
   return kRotMaxPairs / (32 * V);
 }
 
@@ -476,9 +478,8 @@ __device__ __forceinline__ int64_t unit_position(const RotaryParams& p, const Fa
   return token_position(p, b, static_cast<int>(token) - b * static_cast<int>(p.seq.d));
 }
 
-template <typename T, int V, bool NORM, bool IL>
+template <typename T, int V, int NS, bool NORM, bool IL>
 __global__ void __launch_bounds__(32 * kRotWarps, 5) rotary_forward_kernel(const __grid_constant__ RotaryParams p) {
-  constexpr int NS = rotary_slots_per_lane<V>();
   using Ring = PassRing<T, V, 2 * NS>;
   __shared__ __align__(16) Ring ring_all[kRotWarps];
   __shared__ __align__(16) TokenAngles angles_all[kRotWarps];
@@ -606,10 +607,9 @@ __global__ void __launch_bounds__(32 * kRotWarps, 5) rotary_forward_kernel(const
 // norm_weight_grad_kernel adds the blocks' rows, again in a fixed order: the same inputs give the same
 // bits. Angles and weights stay in shared memory: in registers they would leave room for half as many
 // warps.
-template <typename T, int V, bool IL>
+template <typename T, int V, int NS, bool IL>
 __global__ void __launch_bounds__(32 * kRotWarps, 4)
     qk_norm_rotary_backward_kernel(const __grid_constant__ RotaryParams p) {
-  constexpr int NS = rotary_slots_per_lane<V>();
   using Ring = PassRing<T, V, 4 * NS>;  // vector 4 n: x's a, + 1: x's b, + 2, + 3: dy's
   union Shared {
     Ring ring[kRotWarps];

@@ -91,16 +91,45 @@ int32_t activation_code(const std::string& name) {
 // Row stride of a 2-D operand; a single row's stride means nothing, so its length stands for it.
 int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
-// A 2-D operand in the compute dtype that the kernels read in place: contiguous columns (in 16 bits
-// padded to a multiple of 8) and 16-byte aligned rows. Copied only where it is not.
-Tensor operand(Tensor t, at::ScalarType dtype) {
-  if (t.scalar_type() != dtype) t = t.to(dtype);
-  const int64_t unit = dtype == at::kFloat ? 1 : 8;
-  if (t.size(1) % unit) t = at::constant_pad_nd(t, {0, round8(t.size(1)) - t.size(1)});
-  const int64_t ld = row_stride(t);
-  if ((t.stride(1) != 1 && t.size(1) > 1) || ld % unit || ld < t.size(1)) t = t.contiguous();
-  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
-}
+// The operands (one dtype) as the kernels read them: contiguous columns and 16-byte aligned rows, in 16 bits
+// of a multiple of 8 elements. Copied only where they are not; the copies are no part of the autograd graph.
+struct GluOperands {
+  Tensor t[3];  // x, gate, up
+  int64_t hidden;
+
+  GluOperands(const Tensor& x, const Tensor& gate, const Tensor& up) : t{x, gate, up}, hidden(x.size(1)) {
+    at::AutoGradMode off(false);
+    TORCH_CHECK_VALUE(gate.scalar_type() == x.scalar_type() && up.scalar_type() == x.scalar_type(),
+                      "gated_linear_unit: operands must have one dtype, got ", x.scalar_type(), ", ",
+                      gate.scalar_type(), " and ", up.scalar_type());
+    const bool wide = x.scalar_type() == at::kFloat;
+    if (wide || hidden % 8 == 0) {
+      const int64_t unit = wide ? 1 : 8;
+      for (Tensor& o : t) {
+        const int64_t ld = row_stride(o);
+        if ((o.stride(1) != 1 && o.size(1) > 1) || ld % unit || ld < o.size(1)) o = o.contiguous();
+        if (reinterpret_cast<uintptr_t>(o.data_ptr()) % 16) o = o.clone(at::MemoryFormat::Contiguous);
+      }
+      return;
+    }
+    const void* src[3];
+    void* dst[3];
+    int64_t ld[3], rows[3];
+    Tensor padded[3];
+    for (int i = 0; i < 3; ++i) {
+      if (t[i].stride(1) != 1 && hidden > 1) t[i] = t[i].contiguous();
+      padded[i] = new_empty({t[i].size(0), round8(hidden)}, x.scalar_type(), x);
+      src[i] = t[i].data_ptr();
+      dst[i] = padded[i].data_ptr();
+      ld[i] = row_stride(t[i]);
+      rows[i] = t[i].size(0);
+    }
+    c10::cuda::CUDAGuard guard(x.device());
+    check_status(orda_pad_rows(3, src, ld, rows, hidden, dst, at::cuda::getCurrentCUDAStream().stream()),
+                 "orda_pad_rows");
+    for (int i = 0; i < 3; ++i) t[i] = padded[i];
+  }
+};
 
 void check_glu(const Tensor& x, const Tensor& gate, const Tensor& up) {
   TORCH_CHECK_VALUE(gate.dim() == 2 && gate.sizes() == up.sizes(),
@@ -130,6 +159,7 @@ orda_glu_args_t glu_args(const Tensor& x, const Tensor& gate, const Tensor& up, 
   a.ld_up = row_stride(up);
   a.ld_h = a.ffn;
   a.ld_pre = round8(a.ffn);
+  a.grad_cols = a.hidden;
   return a;
 }
 
@@ -152,17 +182,18 @@ std::pair<Tensor, Tensor> glu_forward(const Tensor& x, const Tensor& gate, const
   return {h, pre};
 }
 
-// (dx, gradients of both weights): the latter [ceil8(ffn) + ffn, hidden], gate's from row 0, up's from
-// row ceil8(ffn).
+// (dx, gradients of both weights), `hidden` columns each: the latter [ceil8(ffn) + ffn, hidden], gate's from
+// row 0, up's from row ceil8(ffn).
 std::pair<Tensor, Tensor> glu_backward(Tensor dh, const Tensor& x, const Tensor& gate, const Tensor& up,
-                                       const Tensor& pre, int64_t act, bool need_x, bool need_w) {
+                                       const Tensor& pre, int64_t act, int64_t hidden, bool need_x, bool need_w) {
   c10::cuda::CUDAGuard guard(x.device());
   cudaStream_t s = at::cuda::getCurrentCUDAStream().stream();
   orda_glu_args_t a = glu_args(x, gate, up, act);
   const auto dt = x.scalar_type();
   Tensor dx, dw, ws, status;
-  if (need_x) dx = new_empty({a.rows, a.hidden}, dt, x);
-  if (need_w) dw = new_empty({a.ld_pre + a.ffn, a.hidden}, dt, x);
+  a.grad_cols = hidden;
+  if (need_x) dx = new_empty({a.rows, hidden}, dt, x);
+  if (need_w) dw = new_empty({a.ld_pre + a.ffn, hidden}, dt, x);
   if (a.rows == 0) {
     if (dw.defined()) dw.zero_();
     return {dx, dw};
@@ -183,9 +214,11 @@ std::pair<Tensor, Tensor> glu_backward(Tensor dh, const Tensor& x, const Tensor&
 
 struct GluFunction : torch::autograd::Function<GluFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& up, int64_t act) {
-    auto [h, pre] = glu_forward(x, gate, up, act, true);
-    ctx->save_for_backward({x, gate, up, pre});
+    const GluOperands o(x, gate, up);
+    auto [h, pre] = glu_forward(o.t[0], o.t[1], o.t[2], act, true);
+    ctx->save_for_backward({o.t[0], o.t[1], o.t[2], pre});
     ctx->saved_data["act"] = act;
+    ctx->saved_data["hidden"] = o.hidden;
     return h;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dh) {
@@ -195,7 +228,7 @@ struct GluFunction : torch::autograd::Function<GluFunction> {
     {
       at::AutoGradMode off(false);
       auto [dx, dw] = glu_backward(dh[0], saved[0], saved[1], saved[2], saved[3], ctx->saved_data["act"].toInt(),
-                                   need_x, need_g || need_u);
+                                   ctx->saved_data["hidden"].toInt(), need_x, need_g || need_u);
       const int64_t ffn = saved[1].size(0);
       grads[0] = dx;
       if (need_g) grads[1] = dw.slice(0, 0, ffn);
@@ -222,10 +255,15 @@ Tensor gated_linear_unit(const Tensor& x, const Tensor& gate_weight, const Tenso
   const int64_t act = activation_code(activation);
   check_glu(x, gate_weight, up_weight);
   const auto dt = compute_dtype({&gate_weight, &up_weight, &x});
-  const Tensor flat = operand(x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}), dt);
-  const Tensor gate = operand(gate_weight, dt), up = operand(up_weight, dt);
-  const bool grad = at::GradMode::is_enabled() && (flat.requires_grad() || gate.requires_grad() || up.requires_grad());
-  Tensor h = grad ? GluFunction::apply(flat, gate, up, act) : glu_forward(flat, gate, up, act, false).first;
+  auto cast = [dt](const Tensor& t) { return t.scalar_type() == dt ? t : t.to(dt); };
+  const Tensor flat = cast(x.dim() == 2 ? x : x.reshape({-1, x.size(-1)})), gate = cast(gate_weight), up = cast(up_weight);
+  Tensor h;
+  if (at::GradMode::is_enabled() && (flat.requires_grad() || gate.requires_grad() || up.requires_grad())) {
+    h = GluFunction::apply(flat, gate, up, act);
+  } else {
+    const GluOperands o(flat, gate, up);
+    h = glu_forward(o.t[0], o.t[1], o.t[2], act, false).first;
+  }
   if (x.dim() == 2) return h;
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end() - 1);
   shape.push_back(gate.size(0));
@@ -235,8 +273,8 @@ Tensor gated_linear_unit(const Tensor& x, const Tensor& gate_weight, const Tenso
 // Without autograd, for the custom ops: x any number of dimensions, all tensors in the compute dtype.
 std::tuple<Tensor, Tensor> glu_forward_op(const Tensor& x, const Tensor& gate, const Tensor& up, int64_t act) {
   check_glu(x, gate, up);
-  const auto dt = x.scalar_type();
-  auto [h, pre] = glu_forward(operand(x.reshape({-1, x.size(-1)}), dt), operand(gate, dt), operand(up, dt), act, true);
+  const GluOperands o(x.reshape({-1, x.size(-1)}), gate, up);
+  auto [h, pre] = glu_forward(o.t[0], o.t[1], o.t[2], act, true);
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end() - 1);
   shape.push_back(gate.size(0));
   return {h.view(shape), pre};
@@ -245,13 +283,11 @@ std::tuple<Tensor, Tensor> glu_forward_op(const Tensor& x, const Tensor& gate, c
 std::tuple<Tensor, Tensor, Tensor> glu_backward_op(const Tensor& dh, const Tensor& x, const Tensor& gate,
                                                    const Tensor& up, const Tensor& pre, int64_t act) {
   check_glu(x, gate, up);
-  const auto dt = x.scalar_type();
   const int64_t ffn = gate.size(0), hidden = x.size(-1);
-  auto [dx, dw] = glu_backward(dh.reshape({-1, ffn}), operand(x.reshape({-1, hidden}), dt), operand(gate, dt),
-                               operand(up, dt), pre, act, true, true);
+  const GluOperands o(x.reshape({-1, hidden}), gate, up);
+  auto [dx, dw] = glu_backward(dh.reshape({-1, ffn}), o.t[0], o.t[1], o.t[2], pre, act, hidden, true, true);
   // an op's outputs share no storage
-  return {dx.slice(1, 0, hidden).contiguous().view(x.sizes()), dw.slice(0, 0, ffn).slice(1, 0, hidden).clone(),
-          dw.slice(0, round8(ffn)).slice(1, 0, hidden).clone()};
+  return {dx.view(x.sizes()), dw.slice(0, 0, ffn).clone(), dw.slice(0, round8(ffn)).clone()};
 }
 
 // ------------------------------------------------------------------ rotary positions

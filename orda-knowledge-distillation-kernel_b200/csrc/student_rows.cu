@@ -69,7 +69,7 @@ int rotary_width(const orda_rotary_args_t* a, bool backward) {
 struct RotaryPlan {
   RotaryParams p;
   int width, grid;
-  bool interleaved;
+  bool interleaved, one_slot;  // one_slot: a head's slots fit the 32 lanes
 };
 
 // A unit of work (one warp) is a group of heads of one token. Large calls give a warp all heads of a
@@ -105,6 +105,7 @@ RotaryPlan plan_rotary(const orda_rotary_args_t* a, bool backward) {
   p.eps = a->eps;
   for (int i = 0; i < a->rotary_dim / 2; ++i) p.turns[i] = a->turns[i];
   const int slots = static_cast<int>(cdiv(a->head_dim, 2 * r.width));
+  r.one_slot = slots <= 32;
   p.lanes = 1;
   while (p.lanes < slots && p.lanes < 32) p.lanes *= 2;
   const int at_once = 32 / p.lanes;
@@ -124,43 +125,45 @@ RotaryPlan plan_rotary(const orda_rotary_args_t* a, bool backward) {
   return r;
 }
 
-template <typename T, int V, bool IL>
-int run_rotary(const RotaryPlan& r, bool norm, cudaStream_t s) {
-  count_launch();
-  if (norm) rotary_forward_kernel<T, V, true, IL><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
-  else rotary_forward_kernel<T, V, false, IL><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
-  return launch_status();
+// f(V, NS, IL) of the plan as integral constants. (Single-element slots hold (u, v) in either layout: slot_of
+// alone tells the layouts apart.)
+template <typename F>
+void with_rotary_shape(const RotaryPlan& r, F&& f) {
+  auto layout = [&](auto v, auto ns) {
+    if (r.interleaved) f(v, ns, std::true_type{});
+    else f(v, ns, std::false_type{});
+  };
+  auto slots = [&](auto v) {
+    constexpr int most = rotary_most_slots<decltype(v)::value>();
+    if constexpr (most > 1) {
+      if (r.one_slot) return layout(v, std::integral_constant<int, 1>{});
+    }
+    layout(v, std::integral_constant<int, most>{});
+  };
+  if (r.width == 8) slots(std::integral_constant<int, 8>{});
+  else if (r.width == 2) slots(std::integral_constant<int, 2>{});
+  else slots(std::integral_constant<int, 1>{});
 }
 
-// Single-element slots hold (u, v) in either layout: slot_of alone tells the layouts apart.
 template <typename T>
 int dispatch_rotary(const RotaryPlan& r, bool norm, cudaStream_t s) {
-  switch (r.width * 2 + r.interleaved) {
-    case 16: return run_rotary<T, 8, false>(r, norm, s);
-    case 17: return run_rotary<T, 8, true>(r, norm, s);
-    case 4: return run_rotary<T, 2, false>(r, norm, s);
-    case 5: return run_rotary<T, 2, true>(r, norm, s);
-    case 2: return run_rotary<T, 1, false>(r, norm, s);
-    default: return run_rotary<T, 1, true>(r, norm, s);
-  }
-}
-
-template <typename T, int V, bool IL>
-void run_norm_backward(const RotaryPlan& r, cudaStream_t s) {
-  qk_norm_rotary_backward_kernel<T, V, IL><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
+  count_launch();
+  with_rotary_shape(r, [&](auto v, auto ns, auto il) {
+    constexpr int V = decltype(v)::value, NS = decltype(ns)::value;
+    constexpr bool IL = decltype(il)::value;
+    if (norm) rotary_forward_kernel<T, V, NS, true, IL><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
+    else rotary_forward_kernel<T, V, NS, false, IL><<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
+  });
+  return launch_status();
 }
 
 template <typename T>
 int dispatch_norm_backward(const RotaryPlan& r, cudaStream_t s) {
   count_launch();
-  switch (r.width * 2 + r.interleaved) {
-    case 16: run_norm_backward<T, 8, false>(r, s); break;
-    case 17: run_norm_backward<T, 8, true>(r, s); break;
-    case 4: run_norm_backward<T, 2, false>(r, s); break;
-    case 5: run_norm_backward<T, 2, true>(r, s); break;
-    case 2: run_norm_backward<T, 1, false>(r, s); break;
-    default: run_norm_backward<T, 1, true>(r, s); break;
-  }
+  with_rotary_shape(r, [&](auto v, auto ns, auto il) {
+    qk_norm_rotary_backward_kernel<T, decltype(v)::value, decltype(ns)::value, decltype(il)::value>
+        <<<r.grid, 32 * kRotWarps, 0, s>>>(r.p);
+  });
   return launch_status();
 }
 

@@ -110,7 +110,7 @@ class GluArgs(ctypes.Structure):
         ("rows", _i64), ("hidden", _i64), ("ffn", _i64),
         ("x", _vp), ("ld_x", _i64), ("gate", _vp), ("ld_gate", _i64), ("up", _vp), ("ld_up", _i64),
         ("h", _vp), ("ld_h", _i64), ("pre_gate", _vp), ("ld_pre", _i64), ("pre_up", _vp),
-        ("dh", _vp), ("dx", _vp), ("dweights", _vp),
+        ("grad_cols", _i64), ("dh", _vp), ("dx", _vp), ("dweights", _vp),
         ("device_status", _vp),
     ]
 
@@ -163,6 +163,7 @@ EXPORTED_SYMBOLS = (
     "orda_merge_row_stats",
     "orda_shard_jsd_partials",
     "orda_shard_backward",
+    "orda_pad_rows",
     "orda_glu_forward",
     "orda_glu_backward_workspace_bytes",
     "orda_glu_backward",
@@ -225,6 +226,9 @@ def _declare(lib):
     lib.orda_shard_backward.restype = _i32
     lib.orda_shard_backward.argtypes = [P, _vp, ctypes.c_size_t, _vp, _vp, _vp]
     PG, PR, PT = ctypes.POINTER(GluArgs), ctypes.POINTER(RotaryArgs), ctypes.POINTER(TensorList)
+    lib.orda_pad_rows.restype = _i32
+    lib.orda_pad_rows.argtypes = [_i32, ctypes.POINTER(_vp), ctypes.POINTER(_i64), ctypes.POINTER(_i64), _i64,
+                                  ctypes.POINTER(_vp), _vp]
     lib.orda_glu_forward.restype = _i32
     lib.orda_glu_forward.argtypes = [PG, _vp]
     lib.orda_glu_backward_workspace_bytes.restype = ctypes.c_size_t

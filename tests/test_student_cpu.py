@@ -198,13 +198,26 @@ def test_c_glu_checks(kw, code):
 
 def test_c_glu_backward_checks():
     lib = _native.load()
-    ok = dict(pre_gate=16, pre_up=16, dh=16, dx=16, dweights=16, h=None)
+    ok = dict(pre_gate=16, pre_up=16, dh=16, dx=16, dweights=16, h=None, grad_cols=16)
     size = lib.orda_glu_backward_workspace_bytes(_glu(**ok))
     assert size >= 4 * 16 * 2
     assert lib.orda_glu_backward(_glu(**ok), 256, size - 1, None) == _native.ERR_WORKSPACE
     assert lib.orda_glu_backward(_glu(**ok), None, size, None) == _native.ERR_WORKSPACE
     assert lib.orda_glu_backward(_glu(**ok | dict(dh=None)), 256, size, None) == _native.ERR_INVALID_ARGUMENT
     assert lib.orda_glu_backward(_glu(**ok | dict(dx=8)), 256, size, None) == _native.ERR_ALIGNMENT
+    for cols in (0, 17):
+        assert lib.orda_glu_backward(_glu(**ok | dict(grad_cols=cols)), 256, size, None) == _native.ERR_INVALID_ARGUMENT
+
+
+def test_c_pad_rows_checks():
+    def call(count=1, src=(16,), ld=(3,), rows=(4,), cols=3, dst=(16,)):
+        n = len(src)
+        return _native.load().orda_pad_rows(count, (ctypes.c_void_p * n)(*src), (ctypes.c_int64 * n)(*ld),
+                                            (ctypes.c_int64 * n)(*rows), cols, (ctypes.c_void_p * n)(*dst), None)
+
+    assert call(count=4) == call(cols=0) == call(rows=(-1,)) == call(src=(None,)) == _native.ERR_INVALID_ARGUMENT
+    assert call(src=(17,)) == call(dst=(24,)) == _native.ERR_ALIGNMENT
+    assert call(rows=(0,)) == call(count=0) == _native.OK
 
 
 def _rot(**kw):
