@@ -13,6 +13,9 @@
 // forms its part of the products, then each takes some of the tile's tokens and adds the others' parts
 // up through distributed shared memory, in the blocks' order.
 //
+// Measured in bf16: 64 rows 4096 -> 11264 43 us (4.3 TB/s; the 512-row tiles of the pair GEMM 91, the 256-row
+// ones 60), 64 rows 1024 -> 2816 10.3 us with four blocks a tile, 14.4 with one.
+//
 //   warp 0 : TMA producer    warp 1 : MMA issuer    warps 2..5 : epilogue
 //
 // The bounded waits' status word lives in shared memory, so that the caller has none to clear; a block

@@ -13,8 +13,10 @@
 // 32-bit float product is already off by 0.06 rad at position 1e6). No table and no fp64 arithmetic: a
 // warp computes a token's angles once for the heads that it turns.
 //
-// What bounds it: memory. Each head's values are read and written once, 16-byte vectors, and a lane's
-// cosines, sines and norm weights stay in registers over the heads of the token.
+// What bounds it: memory, and close behind it the issue of instructions (61-67% of the slots). Each head's
+// values are read and written once in 16-byte vectors, a token's angles are formed once. In bf16: 32768 tokens
+// of 10 heads of 128 are rotated in 33.0 us (5.1 TB/s), 16384 of 40 normed and rotated in 60 us (5.6 TB/s), and
+// back in 96 us (5.2 TB/s) and 7 for the weights' sums.
 #pragma once
 
 #include <type_traits>

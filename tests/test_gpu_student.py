@@ -57,6 +57,7 @@ def glu64(x, wg, wu, act, dh=None):
     """{name: (value, tolerance)} of h and, with dh, the gradients."""
     dt, k = x.dtype, x.shape[1]
     hf = half(dt)
+    sub = torch.finfo(dt).smallest_normal * hf  # the same below the normal range: half of the smallest step
     x, wg, wu = x.double(), wg.double(), wu.double()
     g, u = x @ wg.T, x @ wu.T
     eg, eu = (x.abs() @ w.abs().T * (k * 2.0 ** -23) for w in (wg, wu))  # of the products
@@ -69,13 +70,13 @@ def glu64(x, wg, wu, act, dh=None):
         return out
     dh = dh.double()
     # what the backward pass reads: g and u rounded (16-bit types)
-    rg, ru = eg + hf * g.abs(), eu + hf * u.abs()
+    rg, ru = eg + hf * g.abs() + sub, eu + hf * u.abs() + sub
     # |act''| <= 1.13 (relu: its slope jumps within eg of 0)
     ed = 1.13 * rg + 2.0 ** -17 * (1 + g.abs()) if act != "relu" else (g.abs() <= eg).double()
     dg, du = dh * u * d, dh * a
     edg = dh.abs() * (ru * (d.abs() + ed) + u.abs() * ed)
     edu = dh.abs() * (1.13 * rg + 2.0 ** -18 * g.abs())
-    edg, edu = edg + hf * (dg.abs() + edg), edu + hf * (du.abs() + edu)  # dg and du are rounded too
+    edg, edu = edg + hf * (dg.abs() + edg) + sub, edu + hf * (du.abs() + edu) + sub  # dg and du are rounded too
     mg, mu = dg.abs() + edg, du.abs() + edu
 
     def grad(v, err, magnitude, n):
