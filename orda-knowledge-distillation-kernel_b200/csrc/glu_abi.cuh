@@ -124,15 +124,16 @@ int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
   prm.st.N = a->ffn;
   // 512 x 128 or 256 x 128 tiles: the wide kernel moves a quarter less per product, the 256-row one has two
   // accumulator buffers, so that a short K does not wait for the epilogue, and wastes less of a ragged
-  // batch. In clocks of a CTA pair, measured over K = 1024 and 4096: 1050 a k block + 9500 a tile against
-  // 590 + 2300. (8192 x 1024 -> 2816: 94 us wide, 82 us here; 8192 x 4096 -> 11264: 1036 against 1075.)
+  // batch. Estimated clocks of a CTA pair, fitted to K = 1024 ... 4096: 1050 a k block + 9500 a tile against
+  // 620 + 2000. (8192 rows, us wide and 256-row: 1024 -> 2816 94 and 82, 1536 -> 4224 181 and 170, 2048 -> 5632
+  // 284 and 291, 4096 -> 11264 1036 and 1077.)
   const int64_t pairs = std::max(1, num_sms() / 2), f_tiles = cdiv(a->ffn, 128);
   const int64_t wide = cdiv(cdiv(a->rows, 512) * f_tiles, pairs) * (1050 * prm.kb0 + 9500);
-  const int64_t half = cdiv(cdiv(a->rows, 256) * f_tiles, pairs) * (590 * prm.kb0 + 2300);
+  const int64_t half = cdiv(cdiv(a->rows, 256) * f_tiles, pairs) * (620 * prm.kb0 + 2000);
   const int64_t cols = 2 * round8(a->ffn);
   if (half < wide)
     return launch_tc2<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 256), cols, s, 8);
-  return launch_tc2w<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 512), cols, s, 4);
+  return launch_tc2w<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 512), cols, s, 8);
 }
 
 // K split of a gradient GEMM with M x N outputs and `kb` k blocks on the wide kernel: the split whose
