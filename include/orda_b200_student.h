@@ -41,7 +41,7 @@ typedef struct orda_glu_args {
   const void* gate; int64_t ld_gate;    /* [F, H]                                            */
   const void* up; int64_t ld_up;        /* [F, H]                                            */
   /* 16-bit types: hidden and the strides of x, gate, up multiples of 8; ld_pre always. Bases 16-byte aligned,
-     but for h and dh, which may lie anywhere.                                              */
+     but for h and dh, which may start at any element.                                      */
   void* h; int64_t ld_h;                /* [N, F]; ld_h is the row stride of dh too          */
   void* pre_gate; int64_t ld_pre;       /* [N, F] x Wgate^T, written where not NULL          */
   void* pre_up;                         /* [N, F] x Wup^T (both or neither)                  */

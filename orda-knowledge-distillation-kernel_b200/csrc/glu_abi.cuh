@@ -35,6 +35,8 @@ int check_glu(const orda_glu_args_t* a, bool backward) {
   if (a->hidden % unit || a->ld_x % unit || a->ld_gate % unit || a->ld_up % unit ||
       ((a->pre_gate || backward) && a->ld_pre % 8))
     return ORDA_ERR_ALIGNMENT;
+  const uintptr_t es = esize(a->dtype);
+  if (reinterpret_cast<uintptr_t>(a->h) % es || reinterpret_cast<uintptr_t>(a->dh) % es) return ORDA_ERR_ALIGNMENT;
   if (off(a->x) || off(a->gate) || off(a->up) || off(a->pre_gate) || off(a->pre_up) || off(a->dx) || off(a->dweights))
     return ORDA_ERR_ALIGNMENT;
   if (a->dtype == ORDA_F32 && !backward && !a->pre_gate) return ORDA_ERR_INVALID_ARGUMENT;  // its products need a place

@@ -34,7 +34,7 @@ __device__ __forceinline__ void stage_store_piece(const CUtensorMap* map, uint32
 }
 
 // The same piece by plain stores, one row at a time (128 contiguous bytes a warp), for rows that are not 16-byte
-// aligned. Two-element words where the row stride is even, single elements otherwise.
+// aligned. Two-element words where every row starts on their boundary, single elements otherwise.
 template <typename T16, typename Word>
 __device__ __forceinline__ void store_piece_rows(T16* out, int64_t ld, int64_t M, int64_t N, uint32_t staging,
                                                  int64_t y0, int64_t c0, int lane, Word&& w) {
@@ -51,7 +51,7 @@ __device__ __forceinline__ void store_piece_rows(T16* out, int64_t ld, int64_t M
   __syncwarp();
   const int rows = static_cast<int>(M - y0 < 32 ? M - y0 : 32);
   const int64_t col = c0 + 2 * lane;
-  const bool words = (ld & 1) == 0 && col + 1 < N;
+  const bool words = (ld & 1) == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0 && col + 1 < N;
   for (int r = 0; r < rows; ++r) {
     uint32_t v;
     asm volatile("ld.shared.b32 %0, [%1];"

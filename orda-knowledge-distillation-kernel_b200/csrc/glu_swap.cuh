@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kSwapThreads, 2) glu_swap_kernel(const __grid_
       if (!ok) a0 = a1 = nan;
       auto put = [&](void* out, int64_t ld, float x, float y) {
         T16* o = static_cast<T16*>(out) + (t0 + t) * ld + f;
-        if (pair && ld % 2 == 0) {
+        if (pair && (reinterpret_cast<uintptr_t>(o) & 3u) == 0) {
           *reinterpret_cast<uint32_t*>(o) = pack2<T16>(x, y);
         } else {
           o[0] = Conv<T16>::from_f(x);

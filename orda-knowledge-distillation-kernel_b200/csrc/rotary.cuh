@@ -337,22 +337,17 @@ __device__ __forceinline__ void token_angles(const RotaryParams& p, const uint64
   __syncwarp();
 }
 
-// The angles of slot s; (1, 0) where the slot passes through.
+// The angles of slot s. A slot that passes through has none: multiplied by (1, 0) instead, an infinity in one
+// of its values would become NaN in another.
 template <int V>
 struct SlotAngles {
   Vec<V> cos, sin, neg_sin;
 
-  __device__ __forceinline__ void load(const RotaryParams& p, const TokenAngles& t, int s, bool turned) {
-    if (turned) {
-      const int rotated = p.rotary_dim / (2 * V);
-      load_pairs<V>(t.cos, rotated, s, cos);
-      load_pairs<V>(t.sin, rotated, s, sin);
-      load_pairs<V>(t.neg_sin, rotated, s, neg_sin);
-    } else {
-      cos.fill(1.f);
-      sin.fill(0.f);
-      neg_sin.fill(0.f);
-    }
+  __device__ __forceinline__ void load(const RotaryParams& p, const TokenAngles& t, int s) {
+    const int rotated = p.rotary_dim / (2 * V);
+    load_pairs<V>(t.cos, rotated, s, cos);
+    load_pairs<V>(t.sin, rotated, s, sin);
+    load_pairs<V>(t.neg_sin, rotated, s, neg_sin);
   }
   __device__ __forceinline__ void turn(Vec<V>& u, Vec<V>& v) const {
 #pragma unroll
@@ -556,7 +551,8 @@ __global__ void __launch_bounds__(32 * kRotWarps, 5) rotary_forward_kernel(const
       __syncwarp();  // the previous unit's angles have been read
       token_angles<V, IL>(p, turns, position, lane, angles);
 #pragma unroll
-      for (int n = 0; n < NS; ++n) sa[n].load(p, angles, sl + n * p.lanes, slot[n].turned);
+      for (int n = 0; n < NS; ++n)
+        if (slot[n].turned) sa[n].load(p, angles, sl + n * p.lanes);
       // the next unit's position, wanted when this one is done
       if (at.unit + stride < total) position = unit_position(p, p.units[0], at.unit + stride);
     }
@@ -592,7 +588,7 @@ __global__ void __launch_bounds__(32 * kRotWarps, 5) rotary_forward_kernel(const
           v[n].e[i] = mul_v(mul_v(v[n].e[i], r), wv.e[i]);
         }
       }
-      sa[n].turn(u[n], v[n]);
+      if (slot[n].turned) sa[n].turn(u[n], v[n]);
       store_pairs<T, V, IL>(out, slot[n], live, u[n], v[n]);
     }
     at.head += at_once;
@@ -716,9 +712,11 @@ __global__ void __launch_bounds__(32 * kRotWarps, 4)
         ex.fill(0.f);
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-          SlotAngles<V> sa;
-          sa.load(p, angles, sl + n * p.lanes, slot[n].turned);
-          sa.turn(zu[n], zv[n]);
+          if (slot[n].turned) {
+            SlotAngles<V> sa;
+            sa.load(p, angles, sl + n * p.lanes);
+            sa.turn(zu[n], zv[n]);
+          }
           Vec<V> wu, wv;
           load_pairs<V>(weights.u, slots, sl + n * p.lanes, wu);
           load_pairs<V>(weights.v, slots, sl + n * p.lanes, wv);
@@ -732,7 +730,8 @@ __global__ void __launch_bounds__(32 * kRotWarps, 4)
         float sum[2] = {ss.sum(), ex.sum()};
         group_sum(sum, p.lanes);
         const float r = rsqrtf(sum[0] * p.inv_head_dim + p.eps);
-        const float m = -r * r * r * (sum[1] * p.inv_head_dim);  // -r^2 mean(e n)
+        // -r^2 mean(e n), in an order that leaves a head of zeros 0 where r^3 overflows (eps below 1e-25)
+        const float m = -(sum[1] * p.inv_head_dim * r) * r * r;
         const auto r2 = Vec<V>::all(r), m2 = Vec<V>::all(m);
 #pragma unroll
         for (int n = 0; n < NS; ++n) {

@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
@@ -77,6 +78,25 @@ variable_list differentiable_once(variable_list grads) {
     out.push_back((*fn)({g})[0]);
   }
   return out;
+}
+
+// A captured backward pass whose gradients go on to a node of the default stream - a leaf that an eager graph
+// still holds, or a cast made before the capture - would have autograd make that stream wait for the
+// capture, which CUDA forbids and which ends the process. Refused here, before anything is launched.
+void refuse_eager_nodes_in_capture(const char* what) {
+  const auto node = torch::autograd::get_current_node();
+  const auto here = at::cuda::getCurrentCUDAStream();
+  if (!node || here.stream() == nullptr ||
+      at::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None)
+    return;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    if (!node->should_compute_output(i) || !node->task_should_compute_output(i)) continue;
+    const auto stream = node->next_edge(i).function->stream();
+    TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream).stream() != nullptr, what,
+                ": the backward pass is captured into a CUDA graph, but input ", i,
+                " belongs to an autograd graph that was recorded on the default stream and still lives; drop that "
+                "graph (or record it on a side stream) before the capture");
+  }
 }
 
 // ------------------------------------------------------------------ gated feed-forward block
@@ -222,6 +242,7 @@ struct GluFunction : torch::autograd::Function<GluFunction> {
     return h;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dh) {
+    refuse_eager_nodes_in_capture("gated_linear_unit");
     const auto saved = ctx->get_saved_variables();
     const bool need_x = ctx->needs_input_grad(0), need_g = ctx->needs_input_grad(1), need_u = ctx->needs_input_grad(2);
     variable_list grads(4);
@@ -427,6 +448,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     return rotate(q, k, positions, *plan, false, {}, {}, 0.0);
   }
   static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    refuse_eager_nodes_in_capture("rotary_embedding");
     const auto saved = ctx->get_saved_variables();
     const auto plan = c10::static_intrusive_pointer_cast<RotaryPlan>(ctx->saved_data["plan"].toCapsule());
     variable_list g;
@@ -448,6 +470,7 @@ struct QkNormRotaryFunction : torch::autograd::Function<QkNormRotaryFunction> {
     return rotate(q, k, positions, *plan, false, wq, wk, eps);
   }
   static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    refuse_eager_nodes_in_capture("qk_norm_rotary");
     const auto s = ctx->get_saved_variables();
     const auto plan = c10::static_intrusive_pointer_cast<RotaryPlan>(ctx->saved_data["plan"].toCapsule());
     variable_list g;
@@ -559,7 +582,7 @@ Tensor clip_call(const std::vector<Tensor>& src, const std::vector<Tensor>* dst,
 Tensor grad_norm(const std::vector<Tensor>& grads) {
   at::AutoGradMode off(false);
   check_gradients("grad_norm", grads);
-  if (grads.empty()) return at::zeros({});
+  if (grads.empty()) return at::zeros({}, at::kFloat);
   std::vector<Tensor> src;
   src.reserve(grads.size());
   for (const Tensor& g : grads) src.push_back(dense(g));
@@ -570,7 +593,7 @@ std::tuple<std::vector<Tensor>, Tensor> clip_gradients(const std::vector<Tensor>
   at::AutoGradMode off(false);
   check_limits("clip_gradients", max_norm, eps);
   check_gradients("clip_gradients", grads);
-  if (grads.empty()) return std::make_tuple(std::vector<Tensor>(), at::zeros({}));
+  if (grads.empty()) return std::make_tuple(std::vector<Tensor>(), at::zeros({}, at::kFloat));
   std::vector<Tensor> src, out;
   src.reserve(grads.size());
   out.reserve(grads.size());
@@ -605,7 +628,7 @@ Tensor clip_in_place(const std::vector<Tensor>& grads, double max_norm, double e
   const char* what = "clip_grad_norm_";
   check_limits(what, max_norm, eps);
   check_gradients(what, grads);
-  if (grads.empty()) return at::zeros({});
+  if (grads.empty()) return at::zeros({}, at::kFloat);
   std::unordered_set<const void*> seen;
   std::vector<Tensor> src;
   src.reserve(grads.size());
@@ -615,8 +638,10 @@ Tensor clip_in_place(const std::vector<Tensor>& grads, double max_norm, double e
     src.push_back(dense(g));
   }
   Tensor norm = clip_call(src, &src, max_norm, eps);
-  for (size_t i = 0; i < src.size(); ++i)
+  for (size_t i = 0; i < src.size(); ++i) {
     if (!src[i].is_same(grads[i])) grads[i].copy_(src[i]);
+    else if (!grads[i].is_inference()) grads[i].unsafeGetTensorImpl()->bump_version();  // autograd sees the write
+  }
   return norm;
 }
 

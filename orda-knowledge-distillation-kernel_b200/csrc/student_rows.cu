@@ -38,6 +38,13 @@ int check_rotary(const orda_rotary_args_t* a, bool backward) {
     for (int i = 0; i < 2; ++i)
       if (a->heads[i] > 0 && (!a->x[i] || !a->out[i] || (backward && !a->dy[i]))) return ORDA_ERR_INVALID_ARGUMENT;
   }
+  auto off = [](const void* p, size_t element) { return reinterpret_cast<uintptr_t>(p) % element != 0; };
+  const size_t es = esize(a->dtype), ws = norm || backward ? esize(a->weight_dtype) : 1;
+  if (off(a->positions, a->positions_int64 ? 8 : 4)) return ORDA_ERR_ALIGNMENT;
+  for (int i = 0; i < 2; ++i)
+    if (off(a->x[i], es) || off(a->out[i], es) || off(a->weight[i], ws) ||
+        (backward && (off(a->dy[i], es) || off(a->dweight[i], ws))))
+      return ORDA_ERR_ALIGNMENT;
   return ORDA_OK;
 }
 
@@ -295,6 +302,7 @@ int32_t orda_qk_norm_rotary_backward(const orda_rotary_args_t* args, void* works
     return ORDA_OK;
   }
   if (!workspace || workspace_bytes < orda_qk_norm_rotary_backward_workspace_bytes(args)) return ORDA_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15u) return ORDA_ERR_ALIGNMENT;
   RotaryPlan r = plan_rotary(args, true);
   r.p.dw_partial = static_cast<float*>(workspace);
   switch (args->dtype) {
@@ -320,6 +328,7 @@ int32_t orda_clip_gradients(const orda_tensor_list_t* list, double max_norm, dou
   if (rc) return rc;
   if (!norm || !(max_norm >= 0.0) || !(eps >= 0.0)) return ORDA_ERR_INVALID_ARGUMENT;
   if (!workspace || workspace_bytes < orda_clip_workspace_bytes(list)) return ORDA_ERR_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) || (reinterpret_cast<uintptr_t>(norm) & 3u)) return ORDA_ERR_ALIGNMENT;
   double* partial = static_cast<double*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (list->count <= kGradTensorsSmall) return clip_launches<kGradTensorsSmall>(list, max_norm, eps, norm, partial, s);

@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from orda_ce_kernel import student
+from orda_ce_kernel import _native, student
 
 pytestmark = pytest.mark.gpu
 
@@ -170,6 +170,43 @@ def test_glu_leading_dimensions_and_partial_gradients():
     within(leaf.grad, *want["dx"])
 
 
+# each forward kernel: rows at a time, weights first, 256-row and 512-row tiles, fp32
+@pytest.mark.parametrize("n,h,f,dtype", [(5, 64, 72, BF16), (40, 64, 72, BF16), (140, 64, 72, BF16), (140, 64, 71, BF16),
+                                         (512, 4096, 9470, BF16), (20, 64, 72, FP32)])
+def test_c_glu_results_that_start_at_any_element(n, h, f, dtype):
+    """h (and its gradient dh) one element behind a boundary, with even and odd row strides, between values
+    that have to stay."""
+    x, wg, wu, dh = glu_inputs(n, h, f, dtype, 31)
+    leaves = [t.detach().requires_grad_(True) for t in (x, wg, wu)]
+    want = student.gated_linear_unit(*leaves)
+    want_dx, want_dg, want_du = torch.autograd.grad(want, leaves, dh)
+    lib, fp = _native.load(), (f + 7) // 8 * 8
+    code = {BF16: _native.BF16, FP32: _native.F32}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream
+    for ld in (f + f % 2, f + 1 - f % 2):  # even, odd
+        for start in (1, 2):
+            buf, gbuf = (torch.full((start + n * ld + 1,), 7.0, device="cuda", dtype=dtype) for _ in range(2))
+            rows = buf[start:start + n * ld].view(n, ld)
+            gbuf[start:start + n * ld].view(n, ld)[:, :f] = dh
+            pre = torch.empty(2, n, fp, device="cuda", dtype=dtype)
+            status = torch.zeros(1, device="cuda", dtype=torch.int32)
+            dx, dw = torch.empty(n, h, device="cuda", dtype=dtype), torch.empty(fp + f, h, device="cuda", dtype=dtype)
+            size = buf.element_size()
+            a = _native.GluArgs(abi_version=_native.ABI_VERSION, dtype=code, activation=_native.ACT_SILU, rows=n, hidden=h,
+                                ffn=f, x=x.data_ptr(), ld_x=h, gate=wg.data_ptr(), ld_gate=h, up=wu.data_ptr(), ld_up=h,
+                                h=buf.data_ptr() + start * size, ld_h=ld, pre_gate=pre[0].data_ptr(), ld_pre=fp,
+                                pre_up=pre[1].data_ptr(), grad_cols=h, dh=gbuf.data_ptr() + start * size,
+                                dx=dx.data_ptr(), dweights=dw.data_ptr(), device_status=status.data_ptr())
+            assert lib.orda_glu_forward(a, stream) == _native.OK
+            assert torch.equal(rows[:, :f], want) and bool((rows[:, f:] == 7).all())
+            assert bool((buf[:start] == 7).all()) and float(buf[-1]) == 7.0
+            need = lib.orda_glu_backward_workspace_bytes(a)
+            ws = torch.empty(need, device="cuda", dtype=torch.uint8)
+            assert lib.orda_glu_backward(a, ws.data_ptr(), need, stream) == _native.OK
+            assert torch.equal(dx, want_dx) and torch.equal(dw[:f], want_dg) and torch.equal(dw[fp:], want_du)
+            assert not status.any()
+
+
 def test_glu_no_rows():
     wg = randn(24, 16, seed=1, dtype=BF16).requires_grad_(True)
     x = torch.empty(0, 16, device="cuda", dtype=BF16, requires_grad=True)
@@ -324,6 +361,44 @@ def test_rotary_strides():
     assert torch.equal(only, gq)
 
 
+PARTIAL = [dict(head_dim=64, rotary_dim=32), dict(head_dim=80, rotary_dim=20, layout="interleaved"),
+           dict(head_dim=3, rotary_dim=2), dict(head_dim=37, rotary_dim=22, layout="interleaved"),
+           dict(head_dim=512, rotary_dim=6), dict(head_dim=256, rotary_dim=64)]
+
+
+@pytest.mark.parametrize("cfg", PARTIAL, ids=lambda c: "-".join(str(v) for v in c.values()))
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_values_that_are_not_finite_pass_through_alone(cfg, dtype):
+    d, r = cfg["head_dim"], cfg["rotary_dim"]
+    cfg, pos = student.RotaryConfig(**cfg), torch.arange(1, 6, device="cuda")
+    clean = randn(5, 3, d, seed=14, dtype=dtype)
+    x = clean.clone()
+    x[0, 0, r], x[1, 1, d - 1], x[2, 2, (r + d) // 2] = math.inf, -math.inf, math.nan
+    leaf = clean.clone().requires_grad_(True)
+    y, want = student.rotary_embedding(x, x, pos, cfg)[0], student.rotary_embedding(leaf, clean, pos, cfg)[0]
+    assert torch.equal(y[..., :r], want[..., :r])
+    torch.testing.assert_close(y[..., r:], x[..., r:], rtol=0, atol=0, equal_nan=True)
+    (g,) = torch.autograd.grad(want, leaf, x)
+    torch.testing.assert_close(g[..., r:], x[..., r:], rtol=0, atol=0, equal_nan=True)
+    assert bool(torch.isfinite(g[..., :r]).all())
+    # with the norm: a head whose mean square is infinite is zero but for that element
+    w = (1 + randn(d, seed=15, scale=0.1)).requires_grad_(True)
+    bad = clean.clone()
+    bad[0, 0, r] = math.inf
+    y = student.qk_norm_rotary(bad, clean, w, w, pos, cfg)[0].detach()
+    want = student.qk_norm_rotary(clean, clean, w, w, pos, cfg)[0]
+    lost = torch.zeros(5, 3, d, device="cuda", dtype=torch.bool)
+    lost[0, 0, r] = True
+    assert bool(torch.isnan(y[lost]).all()) and not y[0, 0][~lost[0, 0]].any()
+    y[0, 0] = want[0, 0].detach()
+    assert torch.equal(y, want)
+    # a gradient that is not finite reaches one element of the weight's
+    dy = clean.clone()
+    dy[1, 1, d - 1] = math.inf
+    (gw,) = torch.autograd.grad(want, w, dy)
+    assert not bool(torch.isfinite(gw[d - 1])) and bool(torch.isfinite(gw[:d - 1]).all())
+
+
 def test_rotary_no_tokens_and_no_heads():
     cfg = student.RotaryConfig(64)
     q, k = student.rotary_embedding(randn(0, 4, 64, seed=1), randn(0, 2, 64, seed=1),
@@ -393,6 +468,8 @@ def test_qk_norm_strides_and_small_heads():
     q = q.clone()
     q[:, 1] = 0
     check_qk_norm(q, k, w[0, :d], w[1, :d], torch.arange(t, device="cuda"), cfg, eps=1e-2)
+    # the same where the cube of their factor, 1e15, is no fp32 number
+    check_qk_norm(q.float(), k.float(), w[0, :d], w[1, :d], torch.arange(t, device="cuda"), cfg, eps=1e-30)
 
 
 def test_qk_norm_no_tokens():
@@ -511,6 +588,15 @@ def test_clip_refuses_a_gradient_twice():
     with pytest.raises(ValueError, match="twice"):
         student.clip_grad_norm_([p, p], 1.0)
     assert float(student.grad_norm([p.grad, p.grad])) == pytest.approx(math.sqrt(8.0))
+
+
+def test_clip_in_place_is_a_write_that_autograd_sees():
+    p = torch.nn.Parameter(torch.ones(4, device="cuda"))
+    p.grad = torch.full((4,), 3.0, device="cuda")
+    kept = (p * p.grad).sum()  # saves the gradient
+    student.clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
 
 
 def test_clip_offsets_behind_32_bits():
@@ -694,6 +780,50 @@ def test_step_replays_from_two_graphs(n):
     for _, out in captured:
         for a, b in zip(out, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", ["glu", "rotary", "norm"])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_captured_backward_is_refused_while_an_eager_graph_of_its_leaves_lives(which, accumulate):
+    x, wg, wu, _ = glu_inputs(20, 64, 72, BF16, 12)
+    q, w = randn(6, 2, 16, seed=13), torch.ones(16, device="cuda")
+    pos, cfg = torch.arange(6, device="cuda"), student.RotaryConfig(16)
+    call = {"glu": lambda t: student.gated_linear_unit(x, t, wu),
+            "rotary": lambda t: student.rotary_embedding(t, q, pos, cfg)[0],
+            "norm": lambda t: student.qk_norm_rotary(q, t, w, w, pos, cfg)[1]}[which]
+    leaf = (wg if which == "glu" else q).detach().requires_grad_(True)
+
+    def step():
+        y = call(leaf)
+        dy = torch.ones_like(y)
+        if accumulate:
+            y.backward(dy)
+            return leaf.grad
+        return torch.autograd.grad(y, leaf, dy)[0]
+
+    want = step().clone()
+    leaf.grad = None
+    eager = call(leaf)  # recorded on the default stream
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still lives"):
+        with torch.cuda.graph(graph):
+            step()
+    del eager, graph
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        eager = call(leaf)  # a graph of another stream does no harm
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        if accumulate:
+            got.zero_()
+        graph.replay()
+        assert torch.equal(got, want)
+    del eager
 
 
 def test_operators_and_loss_in_one_step():

@@ -209,6 +209,27 @@ def test_c_glu_backward_checks():
         assert lib.orda_glu_backward(_glu(**ok | dict(grad_cols=cols)), 256, size, None) == _native.ERR_INVALID_ARGUMENT
 
 
+def test_c_pointers_inside_an_element_are_refused():
+    lib = _native.load()
+    assert lib.orda_glu_forward(_glu(h=17), None) == _native.ERR_ALIGNMENT
+    assert lib.orda_glu_forward(_glu(dtype=_native.F32, pre_gate=16, pre_up=16, h=18), None) == _native.ERR_ALIGNMENT
+    assert lib.orda_glu_backward(_glu(pre_gate=16, pre_up=16, dh=17, dx=16, grad_cols=16), 256, 1 << 20,
+                                 None) == _native.ERR_ALIGNMENT
+    for kw in (dict(x=(16, 17)), dict(out=(17, 16)), dict(positions=18), dict(positions=20, positions_int64=1),
+               dict(weight=(16, 18), weight_dtype=_native.F32)):
+        a, _f = _rot(**kw)
+        assert lib.orda_rotary_forward(a, None) == _native.ERR_ALIGNMENT, kw
+    full = dict(weight=(16, 16), dweight=(16, 16), dy=(16, 16), weight_dtype=_native.F32)
+    size = lib.orda_qk_norm_rotary_backward_workspace_bytes(_rot(**full)[0])
+    for kw, workspace in ((dict(dy=(17, 16)), 256), (dict(dweight=(16, 18)), 256), ({}, 264)):
+        a, _f = _rot(**full | kw)
+        assert lib.orda_qk_norm_rotary_backward(a, workspace, size, None) == _native.ERR_ALIGNMENT, kw
+    one = _list([16], [4], [0])
+    size = lib.orda_clip_workspace_bytes(one)
+    assert lib.orda_clip_gradients(one, 1.0, 1e-6, 16, 264, size, None) == _native.ERR_ALIGNMENT
+    assert lib.orda_clip_gradients(one, 1.0, 1e-6, 18, 256, size, None) == _native.ERR_ALIGNMENT
+
+
 def test_c_pad_rows_checks():
     def call(count=1, src=(16,), ld=(3,), rows=(4,), cols=3, dst=(16,)):
         n = len(src)
