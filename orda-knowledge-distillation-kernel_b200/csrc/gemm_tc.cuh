@@ -71,6 +71,9 @@ struct TcGemmParams {
   int64_t split_bytes;
   int32_t prof_slot;  // >= 0: accumulate pipeline wait counters into g_tc2_prof[prof_slot] (testing hook)
   int32_t* status;
+  // 16-bit word that a block writes 0x7fff to when it ends with a pipeline wait timed out (may be NULL): the
+  // result's first value (of an fp32 one the upper half), NaN in every type, for callers that read no status
+  uint16_t* poison;
   // EPI_GLU: b0 / b1 are the gate / up weights, out_map stores h, ws_s_map / ws_t_map the products before
   // the activation (glu_save = 1)
   int32_t glu_act, glu_save;

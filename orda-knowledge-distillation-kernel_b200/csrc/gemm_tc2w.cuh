@@ -629,7 +629,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThr
   cluster_sync_all();  // the peer's epilogue and the leader's MMAs are all done before TMEM is freed
   if (warp == 1) {
     tc_fence_after();
-    if (*reinterpret_cast<volatile int32_t*>(p.status) == ORDA_ERR_TIMEOUT) __nanosleep(1000000);
+    if (*reinterpret_cast<volatile int32_t*>(p.status) == ORDA_ERR_TIMEOUT) {
+      if (p.poison && lane == 0) *p.poison = 0x7fffu;
+      __syncwarp();
+      __nanosleep(1000000);
+    }
     tmem_dealloc_pair(tmem_base, kTmemCols);
   }
 }

@@ -115,6 +115,7 @@ int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
     prm.glu_h = a->h;
     prm.st.ldo = a->ld_h;
   }
+  prm.poison = static_cast<uint16_t*>(a->h);
   prm.glu_act = a->activation;
   prm.glu_save = a->pre_gate != nullptr;
   if (prm.glu_save) {
@@ -207,6 +208,7 @@ int glu_grad_gemm(TcGemmParams& prm, int dtype, int64_t M, int64_t N, int split,
                   cudaStream_t s) {
   int rc;
   const int64_t np = round8(N);
+  prm.poison = split <= 1 ? static_cast<uint16_t*>(out) : reinterpret_cast<uint16_t*>(part) + 1;
   if (split <= 1) {
     prm.st = StoreEpiParams{out, N, M, N, 0, 0};
     if (N == np) {
