@@ -16,7 +16,7 @@
 // What bounds it: memory, and close behind it the issue of instructions (61-67% of the slots). Each head's
 // values are read and written once in 16-byte vectors, a token's angles are formed once. In bf16: 32768 tokens
 // of 10 heads of 128 are rotated in 33.0 us (5.1 TB/s), 16384 of 40 normed and rotated in 60 us (5.6 TB/s), and
-// back in 96 us (5.2 TB/s) and 7 for the weights' sums.
+// back in 96 us (5.2 TB/s) and 5 for the weights' sums.
 #pragma once
 
 #include <type_traits>
@@ -788,24 +788,39 @@ __global__ void __launch_bounds__(32 * kRotWarps, 4)
   }
 }
 
-// dweight[which][i] = sum over the blocks' partial rows; one block per 32 columns of one weight, the rows
-// shared out over its 32 warps.
+// dweight[which][i] = sum over the blocks' partial rows, in a fixed order; one block per kNormSumCols columns of one
+// weight, the rows shared out over its threads so that each has its few loads in flight at once (with 32
+// columns a block, a warp a row, this took 7 us: five memory latencies).
+constexpr int kNormSumCols = 8;
+
 static __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* __restrict__ partial, int rows,
                                                                        int head_dim, int dtype, void* dwq, void* dwk) {
-  __shared__ float acc[32][33];
-  const int which = blockIdx.y, lane = threadIdx.x % 32, part = threadIdx.x / 32;
-  const int col = blockIdx.x * 32 + lane;
+  constexpr int kParts = 1024 / kNormSumCols;
+  __shared__ float acc[kNormSumCols][kParts + 1];
+  const int which = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int c = threadIdx.x % kNormSumCols, part = threadIdx.x / kNormSumCols;
+  const int col = blockIdx.x * kNormSumCols + c;
   float v = 0.f;
   if (col < head_dim) {
-#pragma unroll 8
-    for (int r = part; r < rows; r += 32) v += partial[(static_cast<int64_t>(r) * 2 + which) * head_dim + col];
+    constexpr int kBatch = 5;  // all rows of a full grid: 4 x 148
+    for (int r = part; r < rows; r += kBatch * kParts) {
+      float x[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        x[k] = r + k * kParts < rows ? partial[(static_cast<int64_t>(r + k * kParts) * 2 + which) * head_dim + col] : 0.f;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) v += x[k];
+    }
   }
-  acc[part][lane] = v;
+  acc[c][part] = v;
   __syncthreads();
-  v = acc[lane][part];  // warp `part` now adds up column `part`
+  const int out_col = blockIdx.x * kNormSumCols + warp;
+  if (warp >= kNormSumCols || out_col >= head_dim) return;
+  v = 0.f;
+#pragma unroll
+  for (int k = 0; k < kParts / 32; ++k) v += acc[warp][lane + 32 * k];
   for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int out_col = blockIdx.x * 32 + part;
-  if (lane != 0 || out_col >= head_dim) return;
+  if (lane != 0) return;
   void* out = which ? dwk : dwq;
   if (dtype == ORDA_F32) static_cast<float*>(out)[out_col] = v;
   else if (dtype == ORDA_F16) static_cast<__half*>(out)[out_col] = __float2half_rn(v);

@@ -312,7 +312,7 @@ int32_t orda_qk_norm_rotary_backward(const orda_rotary_args_t* args, void* works
   }
   if (rc) return rc;
   count_launch();
-  norm_weight_grad_kernel<<<dim3(static_cast<unsigned>(cdiv(args->head_dim, 32)), 2), 1024, 0, s>>>(
+  norm_weight_grad_kernel<<<dim3(static_cast<unsigned>(cdiv(args->head_dim, kNormSumCols)), 2), 1024, 0, s>>>(
       r.p.dw_partial, r.grid, args->head_dim, args->weight_dtype, args->dweight[0], args->dweight[1]);
   return launch_status();
 }
