@@ -34,8 +34,8 @@ __device__ __forceinline__ void glu_act(float g, float& a, float& d) {
     a = g * s;
     d = s * (1.f + g * (1.f - s));
   } else if constexpr (ACT == ORDA_ACT_RELU) {
-    a = fmaxf(g, 0.f);
-    d = g > 0.f ? 1.f : 0.f;
+    a = g <= 0.f ? 0.f : g;  // a NaN stays one, in the derivative too (fmaxf would return 0)
+    d = g > 0.f ? 1.f : a;
   } else if constexpr (ACT == ORDA_ACT_GELU) {
     float cdf, e;
     if constexpr (EXACT) {

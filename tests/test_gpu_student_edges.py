@@ -1,0 +1,53 @@
+"""GPU tests of ``orda_ce_kernel.student`` at the edges of values, sizes and ways of calling.
+
+Tolerances as in ``test_gpu_student``: worked out per element, ``half`` is one rounding.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from orda_ce_kernel import _native, student
+from test_gpu_student import BF16, FP16, FP32, glu_inputs, half, randn, within
+
+pytestmark = pytest.mark.gpu
+
+ACTS = ["silu", "gelu", "gelu_tanh", "relu"]
+ACT = {"silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu, "relu": torch.relu,
+       "gelu_tanh": lambda g: torch.nn.functional.gelu(g, approximate="tanh")}
+
+
+def glu_pass(x, wg, wu, act, dh):
+    """(h, dx, dgate, dup)"""
+    leaves = [t.detach().requires_grad_(True) for t in (x, wg, wu)]
+    h = student.gated_linear_unit(*leaves, activation=act)
+    return (h.detach(), *torch.autograd.grad(h, leaves, dh))
+
+
+# ------------------------------------------------------------------------------------------ values that are not finite
+# rows: each 16-bit forward kernel (streamed weights, weights first, pair GEMM); fp32
+@pytest.mark.parametrize("n", [5, 40, 300])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("act", ACTS)
+def test_glu_gate_weight_that_is_not_finite_shows(act, dtype, n):
+    """A NaN in one gate row reaches its feature of h and every gradient that reads it, and nothing else;
+    infinite products give what the formula gives."""
+    x, wg, wu, dh = glu_inputs(n, 64, 72, dtype, 11)
+    clean = glu_pass(x, wg, wu, act, dh)
+    others = torch.arange(72, device="cuda") != 7
+    bad = wg.clone()
+    bad[7, 5] = math.nan
+    h, dx, dgate, dup = glu_pass(x, bad, wu, act, dh)
+    for row in (h[:, 7], dx, dgate[7], dup[7]):
+        assert torch.isnan(row).all()
+    assert torch.equal(h[:, others], clean[0][:, others])
+    assert torch.equal(dgate[others], clean[2][others]) and torch.equal(dup[others], clean[3][others])
+    bad[7, 5] = math.inf
+    h = glu_pass(x, bad, wu, act, dh)[0]
+    want = ACT[act](x.double() @ bad.double().T) * (x.double() @ wu.double().T)
+    assert torch.equal(h[:, others], clean[0][:, others])
+    assert torch.equal(torch.isnan(h[:, 7]), torch.isnan(want[:, 7]))
+    keep = ~torch.isnan(want[:, 7])
+    assert bool(keep.any()) and torch.equal(h[keep, 7].double(), want[keep, 7])  # infinities, and zeros of relu
