@@ -138,15 +138,44 @@ static __global__ void __launch_bounds__(256) glu_act_kernel(const float* g, con
   }
 }
 
+// What a product is formed from again: rows of `hidden` elements, a multiple of 8, 16-byte aligned.
+struct GluSources {
+  const void *x, *gate, *up;
+  int64_t ld_x, ld_gate, ld_up, hidden;
+};
+
+// sum a[k] b[k] in fp32
+static __device__ __noinline__ float dot_f16(const __half* a, const __half* b, int64_t n) {
+  float acc[2] = {0.f, 0.f};
+  for (int64_t k = 0; k < n; k += 8) {
+    const uint4 ua = __ldg(reinterpret_cast<const uint4*>(a + k)), ub = __ldg(reinterpret_cast<const uint4*>(b + k));
+    const uint32_t wa[4] = {ua.x, ua.y, ua.z, ua.w}, wb[4] = {ub.x, ub.y, ub.z, ub.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a0, a1, b0, b1;
+      unpack2<__half>(wa[j], a0, a1);
+      unpack2<__half>(wb[j], b0, b1);
+      acc[0] = fmaf(a0, b0, acc[0]);
+      acc[1] = fmaf(a1, b1, acc[1]);
+    }
+  }
+  return acc[0] + acc[1];
+}
+
 // dg and du into the two halves of `out`, rows of 2 * cols_pad: columns [0, cols_pad) dg, the rest du.
 // g, u and out 16-byte aligned, cols_pad and ld (the row stride of g and u) multiples of 8; dh (row stride
 // ld_dh) any, read element by element unless dh_vec. The columns behind `cols` (the padding) are set to
 // zero. One 8-element vector per thread and step; memory-bound (three reads, two writes).
+//
+// fp16: h comes from fp32 products, and may be finite where a product is beyond 65504 and was saved as an
+// infinity (silu(-1e5) is 0). Read as one, it would give inf * 0 = NaN for a gradient that is 0, so a product
+// that is saved as an infinity is formed again in fp32 (and is infinite again if x or a weight is).
 template <typename T>
 __global__ void __launch_bounds__(256) glu_grad_kernel(const T* __restrict__ dh, int64_t ld_dh, int dh_vec,
                                                        const T* __restrict__ g, const T* __restrict__ u,
                                                        T* __restrict__ out, int64_t rows, int64_t cols,
-                                                       int64_t cols_pad, int64_t ld, int act, int32_t* status) {
+                                                       int64_t cols_pad, int64_t ld, int act, int32_t* status,
+                                                       const GluSources src) {
   if (status && blockIdx.x == 0 && threadIdx.x == 0) *status = 0;  // for the gradient GEMMs that follow
   const int64_t vecs = cols_pad / 8, total = rows * vecs;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
@@ -154,6 +183,7 @@ __global__ void __launch_bounds__(256) glu_grad_kernel(const T* __restrict__ dh,
     const int64_t row = i / vecs, c = (i - row * vecs) * 8;
     const int64_t at = row * ld + c;
     float vd[8], vg[8], vu[8];
+    [[maybe_unused]] float largest = 0.f;
     constexpr int Q = sizeof(T) / 2;
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
@@ -172,6 +202,19 @@ __global__ void __launch_bounds__(256) glu_grad_kernel(const T* __restrict__ dh,
           unpack2<T>(wa[j], vd[2 * j], vd[2 * j + 1]);
           unpack2<T>(wb[j], vg[2 * j], vg[2 * j + 1]);
           unpack2<T>(we[j], vu[2 * j], vu[2 * j + 1]);
+        }
+      }
+    }
+    if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) largest = fmaxf(largest, fmaxf(fabsf(vg[j]), fabsf(vu[j])));
+      if (isinf(largest)) {
+        const T* x = static_cast<const T*>(src.x) + row * src.ld_x;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (c + j >= cols) continue;
+          if (isinf(vg[j])) vg[j] = dot_f16(x, static_cast<const T*>(src.gate) + (c + j) * src.ld_gate, src.hidden);
+          if (isinf(vu[j])) vu[j] = dot_f16(x, static_cast<const T*>(src.up) + (c + j) * src.ld_up, src.hidden);
         }
       }
     }

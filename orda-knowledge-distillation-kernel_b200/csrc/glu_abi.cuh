@@ -247,7 +247,8 @@ int glu_grad_launch(const orda_glu_args_t* a, const GluPlan& P, T* out, cudaStre
   const bool dh_vec = a->ffn % 8 == 0 && (a->ld_h * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(a->dh) & 15u) == 0;
   glu_grad_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(a->dh), a->ld_h, dh_vec,
                                           static_cast<const T*>(a->pre_gate), static_cast<const T*>(a->pre_up), out,
-                                          a->rows, a->ffn, P.fp, a->ld_pre, a->activation, a->device_status);
+                                          a->rows, a->ffn, P.fp, a->ld_pre, a->activation, a->device_status,
+                                          GluSources{a->x, a->gate, a->up, a->ld_x, a->ld_gate, a->ld_up, a->hidden});
   return launch_status();
 }
 

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from orda_ce_kernel import _native, student
-from test_gpu_student import BF16, FP16, FP32, glu_inputs, half, randn, within
+from test_gpu_student import BF16, FP16, FP32, glu64, glu_inputs, half, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,24 @@ def test_glu_gate_weight_that_is_not_finite_shows(act, dtype, n):
     assert torch.equal(torch.isnan(h[:, 7]), torch.isnan(want[:, 7]))
     keep = ~torch.isnan(want[:, 7])
     assert bool(keep.any()) and torch.equal(h[keep, 7].double(), want[keep, 7])  # infinities, and zeros of relu
+
+
+@pytest.mark.parametrize("n", [5, 40, 300])
+@pytest.mark.parametrize("act", ACTS)
+def test_glu_fp16_products_behind_the_types_range(act, n):
+    """Gate products of about +-1e5 beside small and large up products: h is formed from fp32 products, and the
+    gradients have to be finite wherever the formula's are."""
+    x, wg, wu, dh = glu_inputs(n, 64, 75, FP16, 21)
+    x, dh = x * 30, (dh * 2e-4).to(FP16)
+    wg, wu = wg / 30, wu / 30
+    wg[:4] *= 1e5  # |x| |w| is about 240 / sqrt(64) / 30 = 1 without these
+    wu[2:6] *= 1e5
+    g, u = x.double() @ wg.double().T, x.double() @ wu.double().T
+    assert bool((g < -65520).any()) and bool((g > 65520).any()) and bool((u.abs() > 65520).any())
+    want = glu64(x, wg, wu, act, dh)
+    h, *grads = glu_pass(x, wg, wu, act, dh)
+    fits = want["h"][0].abs() < 65000
+    within(h[fits], want["h"][0][fits], want["h"][1][fits], "h")
+    for name, got in zip(("dx", "dgate", "dup"), grads):
+        assert float(want[name][0].abs().max()) < 60000
+        within(got, *want[name], name)
