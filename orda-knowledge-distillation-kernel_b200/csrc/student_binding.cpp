@@ -51,6 +51,13 @@ Tensor new_empty(at::IntArrayRef size, at::ScalarType dtype, const Tensor& like)
   return Tensor(at::detail::empty_cuda(size, dtype, like.device(), std::nullopt));
 }
 
+// A tensor that a kernel reads by the sizes of another one.
+void require_like(const char* what, const Tensor& t, at::IntArrayRef size, const Tensor& like) {
+  TORCH_CHECK_VALUE(t.sizes() == size && t.scalar_type() == like.scalar_type() && t.device() == like.device(), what,
+                    " must have shape ", size, ", ", like.scalar_type(), ", on ", like.device(), ", got ", t.sizes(), ", ",
+                    t.scalar_type(), ", on ", t.device());
+}
+
 // A zeroed device word for the kernels' bounded waits.
 Tensor new_status(const Tensor& like, cudaStream_t s) {
   Tensor t = new_empty({1}, at::kInt, like);
@@ -151,7 +158,8 @@ struct GluOperands {
   }
 };
 
-void check_glu(const Tensor& x, const Tensor& gate, const Tensor& up) {
+// Returns the number of rows.
+int64_t check_glu_shapes(const Tensor& x, const Tensor& gate, const Tensor& up) {
   TORCH_CHECK_VALUE(gate.dim() == 2 && gate.sizes() == up.sizes(),
                     "gate_weight and up_weight must have one shape (ffn, hidden), got ", gate.sizes(), " and ", up.sizes());
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == gate.size(1), "x must have shape (..., ", gate.size(1), "), got ",
@@ -160,6 +168,11 @@ void check_glu(const Tensor& x, const Tensor& gate, const Tensor& up) {
   for (const Tensor* t : {&x, &gate, &up})
     TORCH_CHECK_VALUE(supported(t->scalar_type()), "gated_linear_unit: tensors must be float32, float16 or bfloat16, got ",
                       t->scalar_type());
+  return x.numel() / x.size(-1);
+}
+
+void check_glu(const Tensor& x, const Tensor& gate, const Tensor& up) {
+  check_glu_shapes(x, gate, up);
   require_cuda("gated_linear_unit", x, {&gate, &up});
 }
 
@@ -303,8 +316,13 @@ std::tuple<Tensor, Tensor> glu_forward_op(const Tensor& x, const Tensor& gate, c
 
 std::tuple<Tensor, Tensor, Tensor> glu_backward_op(const Tensor& dh, const Tensor& x, const Tensor& gate,
                                                    const Tensor& up, const Tensor& pre, int64_t act) {
-  check_glu(x, gate, up);
-  const int64_t ffn = gate.size(0), hidden = x.size(-1);
+  const int64_t rows = check_glu_shapes(x, gate, up), ffn = gate.size(0), hidden = x.size(-1);
+  const int64_t pre_size[3] = {2, rows, round8(ffn)};
+  require_like("gated_linear_unit: the products of the forward pass", pre, pre_size, x);
+  std::vector<int64_t> dh_size(x.sizes().begin(), x.sizes().end() - 1);
+  dh_size.push_back(ffn);
+  require_like("gated_linear_unit: the gradient", dh, dh_size, x);
+  require_cuda("gated_linear_unit", x, {&gate, &up});
   const GluOperands o(x.reshape({-1, hidden}), gate, up);
   auto [dx, dw] = glu_backward(dh.reshape({-1, ffn}), o.t[0], o.t[1], o.t[2], pre, act, hidden, true, true);
   // an op's outputs share no storage
@@ -511,10 +529,11 @@ std::tuple<Tensor, Tensor> rotary_op(const Tensor& q, const Tensor& k, const Ten
                                      const std::optional<Tensor>& wq, const std::optional<Tensor>& wk, double eps,
                                      bool inverse, PlanPtr plan) {
   check_qk("rotary_embedding", q, k, positions, *plan);
+  TORCH_CHECK_VALUE(wq.has_value() == wk.has_value(), "qk_norm_rotary: q_weight and k_weight belong together");
+  if (wq) check_norm_weights("qk_norm_rotary", *wq, *wk, *plan, eps);
   require_cuda("rotary_embedding", q, {&k, &positions});
   Tensor w[2];
   if (wq) {
-    check_norm_weights("qk_norm_rotary", *wq, *wk, *plan, eps);
     require_cuda("qk_norm_rotary", q, {&*wq, &*wk});
     w[0] = wq->contiguous();
     w[1] = wk->contiguous();
@@ -529,7 +548,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_backward_op(const Tens
                                                                       const Tensor& wk, double eps, PlanPtr plan) {
   check_qk("qk_norm_rotary", q, k, positions, *plan);
   check_norm_weights("qk_norm_rotary", wq, wk, *plan, eps);
-  require_cuda("qk_norm_rotary", q, {&k, &positions, &wq, &wk, &dq, &dk});
+  require_like("qk_norm_rotary: the gradient of the queries", dq, q.sizes(), q);
+  require_like("qk_norm_rotary: the gradient of the keys", dk, k.sizes(), k);
+  require_cuda("qk_norm_rotary", q, {&k, &positions, &wq, &wk});
   auto r = norm_rotate_backward(dq, dk, dense_last(q), dense_last(k), wq.contiguous(), wk.contiguous(), positions, *plan,
                                 eps);
   return {r[0], r[1], r[2], r[3]};

@@ -1,0 +1,57 @@
+"""``orda_ce_kernel.student`` without a GPU, at the edges: refusals that keep a kernel from reading behind a
+tensor, and what the calls do while something traces them."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from orda_ce_kernel import _native, student
+
+OPS = torch.ops.orda_b200
+
+
+# ------------------------------------------------------------------------------------------ custom ops
+def _glu_backward(**change):
+    a = dict(dh=torch.randn(2, 3, 13), x=torch.randn(2, 3, 8), gate=torch.randn(13, 8), up=torch.randn(13, 8),
+             pre=torch.randn(2, 6, 16), act=0) | change
+    return OPS.glu_backward(*a.values())
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(pre=torch.randn(2, 6, 13)), "products"), (dict(pre=torch.randn(2, 5, 16)), "products"),
+    (dict(pre=torch.randn(2, 6, 16).half()), "products"), (dict(pre=torch.randn(192)), "products"),
+    (dict(dh=torch.randn(2, 3, 12)), "gradient"), (dict(dh=torch.randn(2, 2, 13)), "gradient"),
+    (dict(dh=torch.randn(2, 3, 13).bfloat16()), "gradient"), (dict(up=torch.randn(12, 8)), "one shape"),
+])
+def test_glu_backward_op_refuses_tensors_of_other_sizes(change, match):
+    with pytest.raises(ValueError, match=match):
+        _glu_backward(**change)
+
+
+def test_well_formed_custom_ops_reach_the_device_check():
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        _glu_backward()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        _norm_backward()
+
+
+def _norm_backward(**change):
+    q, k, w = torch.randn(4, 2, 8), torch.randn(4, 1, 8), torch.ones(8)
+    a = dict(dq=q, dk=k, q=q, k=k, positions=torch.arange(4), q_weight=w, k_weight=w, eps=1e-6) | change
+    return OPS.qk_norm_rotary_backward(*a.values(), *student._config_values(student.RotaryConfig(8)))
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(dq=torch.randn(3, 2, 8)), "queries"), (dict(dq=torch.randn(4, 1, 8)), "queries"),
+    (dict(dk=torch.randn(4, 1, 6)), "keys"), (dict(dk=torch.randn(4, 1, 8).half()), "keys"),
+])
+def test_norm_backward_op_refuses_gradients_of_other_sizes(change, match):
+    with pytest.raises(ValueError, match=match):
+        _norm_backward(**change)
+
+
+def test_rotary_op_refuses_one_weight():
+    q, k, cfg = torch.randn(4, 2, 8), torch.randn(4, 1, 8), student._config_values(student.RotaryConfig(8))
+    for weights in ((torch.ones(8), None), (None, torch.ones(8))):
+        with pytest.raises(ValueError, match="together"):
+            OPS.rotary(q, k, torch.arange(4), *weights, 1e-6, False, *cfg)
