@@ -76,12 +76,13 @@ int32_t orda_glu_backward(const orda_glu_args_t* args, void* workspace, size_t w
 #define ORDA_ROTARY_HALF 0         /* pairs (i, i + rotary_dim / 2)                          */
 #define ORDA_ROTARY_INTERLEAVED 1  /* pairs (2 i, 2 i + 1)                                   */
 #define ORDA_ROTARY_MAX_DIM 512
+#define ORDA_ROTARY_MAX_HEADS (1 << 29)
 
 typedef struct orda_rotary_args {
   int32_t abi_version;
   int32_t dtype;                 /* of x, out, dy                                            */
   int64_t batch, seq;            /* tokens: [batch, seq]                                     */
-  int32_t heads[2];              /* [0] queries, [1] keys                                    */
+  int32_t heads[2];              /* [0] queries, [1] keys; each <= ORDA_ROTARY_MAX_HEADS     */
   int32_t head_dim;              /* D <= ORDA_ROTARY_MAX_DIM                                 */
   int32_t rotary_dim;            /* even, <= D; the rest of a head is not rotated            */
   int32_t layout;                /* ORDA_ROTARY_*                                            */

@@ -16,6 +16,7 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/custom_class.h>
 
+#include <algorithm>
 #include <unordered_set>
 
 #include "orda_b200_student.h"
@@ -354,6 +355,8 @@ void check_qk(const char* what, const Tensor& q, const Tensor& k, const Tensor& 
                     "tokens, got ", q.sizes(), " and ", k.sizes());
   TORCH_CHECK_VALUE(q.size(-1) == plan.head_dim && k.size(-1) == plan.head_dim, what,
                     ": heads must have config.head_dim=", plan.head_dim, " elements, got ", q.size(-1), " and ", k.size(-1));
+  TORCH_CHECK_VALUE(std::max(q.size(-2), k.size(-2)) <= ORDA_ROTARY_MAX_HEADS, what, ": at most ", ORDA_ROTARY_MAX_HEADS,
+                    " heads each, got ", q.size(-2), " and ", k.size(-2));
   TORCH_CHECK_VALUE(supported(q.scalar_type()) && k.scalar_type() == q.scalar_type(), what,
                     ": q and k must both be float32, float16 or bfloat16, got ", q.scalar_type(), " and ",
                     k.scalar_type());

@@ -21,8 +21,8 @@ int check_rotary(const orda_rotary_args_t* a, bool backward) {
   if (a->batch < 0 || a->seq < 0 || a->heads[0] < 0 || a->heads[1] < 0) return ORDA_ERR_INVALID_ARGUMENT;
   if (a->head_dim < 1 || a->rotary_dim < 0 || a->rotary_dim % 2 || a->rotary_dim > a->head_dim)
     return ORDA_ERR_INVALID_ARGUMENT;
-  // the kernels count units (a token's groups of heads) and step from head to head in 32 bits
-  if (a->head_dim > ORDA_ROTARY_MAX_DIM || a->batch > INT32_MAX || a->seq > INT32_MAX ||
+  // the kernels count units (a token's groups of heads) and heads and step from head to head in 32 bits
+  if (a->head_dim > ORDA_ROTARY_MAX_DIM || a->heads[0] > ORDA_ROTARY_MAX_HEADS || a->heads[1] > ORDA_ROTARY_MAX_HEADS || a->batch > INT32_MAX || a->seq > INT32_MAX ||
       a->batch * a->seq > INT32_MAX)
     return ORDA_ERR_UNSUPPORTED;
   for (int i = 0; i < 2; ++i)

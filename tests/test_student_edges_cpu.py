@@ -55,3 +55,24 @@ def test_rotary_op_refuses_one_weight():
     for weights in ((torch.ones(8), None), (None, torch.ones(8))):
         with pytest.raises(ValueError, match="together"):
             OPS.rotary(q, k, torch.arange(4), *weights, 1e-6, False, *cfg)
+
+
+# ------------------------------------------------------------------------------------------ sizes
+@pytest.mark.parametrize("heads", [2 ** 29 + 1, 2 ** 31, 2 ** 32 + 1])
+def test_head_counts_that_do_not_fit_are_refused(heads):
+    """Heads are counted in 32 bits: 2^32 + 1 broadcast heads must not become one."""
+    one, many, pos = torch.randn(4, 1, 8), torch.randn(4, 1, 8).expand(4, heads, 8), torch.arange(4)
+    cfg, w = student.RotaryConfig(8), torch.ones(8)
+    for q, k in ((many, one), (one, many)):
+        with pytest.raises(ValueError, match="heads each"):
+            student.rotary_embedding(q, k, pos, cfg)
+        with pytest.raises(ValueError, match="heads each"):
+            student.qk_norm_rotary(q, k, w, w, pos, cfg)
+
+
+def test_c_head_counts_are_bounded():
+    lib = _native.load()
+    for heads in ((2 ** 29 + 1, 1), (1, 2 ** 29 + 1), (2 ** 31 - 1, 2 ** 31 - 1)):
+        a = _native.RotaryArgs(abi_version=_native.ABI_VERSION, dtype=_native.BF16, batch=1, seq=1, heads=heads, head_dim=8,
+                               rotary_dim=0, x=(16, 16), out=(16, 16), positions=16, magnitude=1.0)
+        assert lib.orda_rotary_forward(a, None) == _native.ERR_UNSUPPORTED
