@@ -5,6 +5,7 @@
 // decides their speed; filling the C structs from Python through ctypes took 30 us a call for a
 // rotation whose kernel runs 5. The loss, one long call per step, stays on ctypes.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
@@ -17,7 +18,6 @@
 #include <torch/custom_class.h>
 
 #include <algorithm>
-#include <unordered_set>
 
 #include "orda_b200_student.h"
 
@@ -565,13 +565,42 @@ void check_limits(const char* what, double max_norm, double eps) {
   TORCH_CHECK_VALUE(eps >= 0.0, what, ": eps must be >= 0, got ", eps);
 }
 
-void check_gradients(const char* what, const std::vector<Tensor>& grads) {
+// Tensors that are scaled in place must not share memory: a value would be scaled twice, or by two blocks at
+// once. Ones with gaps between their values may lie in each other's gaps; they are scaled as copies, all made
+// before anything is written.
+void refuse_shared_memory(const char* what, const std::vector<Tensor>& grads) {
+  struct Span {
+    const char *first, *end;
+    bool dense;
+  };
+  std::vector<Span> spans;
+  spans.reserve(grads.size());
+  for (const Tensor& g : grads) {
+    if (g.numel() == 0) continue;
+    TORCH_CHECK_VALUE(at::has_internal_overlap(g) != at::MemOverlap::Yes, what, ": a gradient of shape ", g.sizes(),
+                      " holds broadcast values, which cannot be scaled in place");
+    const char* first = static_cast<const char*>(g.data_ptr());
+    spans.push_back({first, first + g.nbytes(), g.is_non_overlapping_and_dense()});
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.first < b.first; });
+  const char *last = nullptr, *dense_end = nullptr;
+  for (const Span& s : spans) {
+    TORCH_CHECK_VALUE(s.first != last, what, ": a gradient appears twice among the parameters");
+    last = s.first;
+    if (!s.dense) continue;
+    TORCH_CHECK_VALUE(s.first >= dense_end, what, ": two gradients share memory");
+    dense_end = s.end;
+  }
+}
+
+void check_gradients(const char* what, const std::vector<Tensor>& grads, bool in_place = false) {
   for (const Tensor& g : grads) {
     TORCH_CHECK_VALUE(supported(g.scalar_type()), what, ": gradients must be float32, float16 or bfloat16, got ",
                       g.scalar_type());
     TORCH_CHECK_VALUE(g.layout() == at::kStrided, what, ": gradients must be strided tensors, got ", g.layout());
     TORCH_CHECK_VALUE(g.device() == grads[0].device(), what, ": tensors are on ", grads[0].device(), " and ", g.device());
   }
+  if (in_place) refuse_shared_memory(what, grads);
   if (!grads.empty()) require_cuda(what, grads[0], {});
 }
 
@@ -651,16 +680,11 @@ Tensor clip_in_place(const std::vector<Tensor>& grads, double max_norm, double e
   at::AutoGradMode off(false);
   const char* what = "clip_grad_norm_";
   check_limits(what, max_norm, eps);
-  check_gradients(what, grads);
+  check_gradients(what, grads, true);
   if (grads.empty()) return at::zeros({}, at::kFloat);
-  std::unordered_set<const void*> seen;
   std::vector<Tensor> src;
   src.reserve(grads.size());
-  for (const Tensor& g : grads) {
-    TORCH_CHECK_VALUE(g.numel() == 0 || seen.insert(g.data_ptr()).second, what,
-                      ": a gradient appears twice among the parameters");
-    src.push_back(dense(g));
-  }
+  for (const Tensor& g : grads) src.push_back(dense(g));
   Tensor norm = clip_call(src, &src, max_norm, eps);
   for (size_t i = 0; i < src.size(); ++i) {
     if (!src[i].is_same(grads[i])) grads[i].copy_(src[i]);

@@ -305,7 +305,7 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
     """``torch.nn.utils.clip_grad_norm_`` for the 2-norm: scales the ``.grad`` of every parameter in place by
     ``min(1, max_norm / (norm + eps))`` and returns the norm (0-dim fp32). Parameters without a gradient are
     skipped; gradients may have different dtypes and strides but must lie on one device, and no two may
-    share memory (a parameter given twice is refused). Only ``error_if_nonfinite`` synchronises: it raises
+    share memory (refused, as is a parameter given twice, and a gradient that holds broadcast values). Only ``error_if_nonfinite`` synchronises: it raises
     before anything is scaled."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]

@@ -72,3 +72,30 @@ def test_glu_fp16_products_behind_the_types_range(act, n):
     for name, got in zip(("dx", "dgate", "dup"), grads):
         assert float(want[name][0].abs().max()) < 60000
         within(got, *want[name], name)
+
+
+# ------------------------------------------------------------------------------------------ clipping in place
+def _params(*grads):
+    params = [torch.nn.Parameter(torch.empty(g.shape, device="cuda", dtype=g.dtype)) for g in grads]
+    for p, g in zip(params, grads):
+        p.grad = g
+    return params
+
+
+def test_clip_refusals_leave_every_gradient_as_it_was():
+    flat = torch.ones(100, device="cuda")
+    first = torch.ones(3, device="cuda")
+    for bad in (flat[10:20], torch.ones(1, 8, device="cuda").expand(4, 8)):
+        with pytest.raises(ValueError):
+            student.clip_grad_norm_(_params(first, flat, bad), 1e-3)
+        assert bool((flat == 1).all()) and bool((first == 1).all()) and bool((bad == 1).all())
+
+
+def test_clip_gradients_between_each_other():
+    flat = randn(101, seed=3)
+    before = flat.double()
+    norm = student.clip_grad_norm_(_params(flat[::2], flat[1::2]), 1.0)
+    want = float(before.square().sum().sqrt())
+    assert float(norm) == pytest.approx(want, rel=2.0 ** -23)
+    # the factor, its product and the value are rounded to fp32
+    within(flat, before / (want + 1e-6), before.abs() / want * 2.0 ** -22)

@@ -76,3 +76,26 @@ def test_c_head_counts_are_bounded():
         a = _native.RotaryArgs(abi_version=_native.ABI_VERSION, dtype=_native.BF16, batch=1, seq=1, heads=heads, head_dim=8,
                                rotary_dim=0, x=(16, 16), out=(16, 16), positions=16, magnitude=1.0)
         assert lib.orda_rotary_forward(a, None) == _native.ERR_UNSUPPORTED
+
+
+# ------------------------------------------------------------------------------------------ clipping in place
+def _clip(*grads):
+    params = []
+    for g in grads:
+        p = torch.nn.Parameter(torch.empty(g.shape, dtype=g.dtype))
+        p.grad = g
+        params.append(p)
+    return student.clip_grad_norm_(params, 1.0)
+
+
+def test_clip_refuses_gradients_that_share_memory():
+    flat = torch.ones(100)
+    for grads, match in (((flat[:60], flat[59:]), "share memory"), ((flat[10:20], flat), "share memory"),
+                         ((flat, flat[50:60], torch.ones(3)), "share memory"), ((flat, flat), "twice"),
+                         ((flat[::2], flat[::2]), "twice"), ((torch.ones(1, 8).expand(4, 8),), "broadcast"),
+                         ((torch.ones(3), torch.ones(()).expand(5)), "broadcast")):
+        with pytest.raises(ValueError, match=match):
+            _clip(*grads)
+    for grads in ((flat[:60], flat[60:]), (flat[::2], flat[1::2]), (flat[:50].view(5, 10).T, flat[50:]), (flat[:0], flat[:0])):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):  # well-formed
+            _clip(*grads)
