@@ -511,7 +511,8 @@ int dw_tc(const orda_distill_args_t* a, const Plan& P, const void* dz0, const vo
 // ------------------------------------------------------------------ fp32 (SIMT) phases
 void simt_gemm(const float* A, int64_t sam, int64_t sak, const float* B, int64_t sbn, int64_t sbk, float* out,
                int64_t ldo, int64_t M, int64_t N, int64_t K, int accumulate, cudaStream_t s) {
-  dim3 grid(static_cast<unsigned>(cdiv(N, kSimtTile)), static_cast<unsigned>(cdiv(M, kSimtTile)));
+  // (2^31 tiles of results would be 35 TB)
+  const unsigned grid = static_cast<unsigned>(cdiv(N, kSimtTile) * cdiv(M, kSimtTile));
   count_launch();
   simt_gemm_f32_kernel<<<grid, 256, 0, s>>>(A, sam, sak, B, sbn, sbk, out, ldo, M, N, K, accumulate);
 }

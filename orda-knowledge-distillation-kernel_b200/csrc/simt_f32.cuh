@@ -10,7 +10,8 @@
 
 namespace orda {
 
-// D[m, n] = sum_k A[m*sam + k*sak] * B[n*sbn + k*sbk];  out[m*ldo + n] (=|+=) D.
+// D[m, n] = sum_k A[m*sam + k*sak] * B[n*sbn + k*sbk];  out[m*ldo + n] (=|+=) D. One block per tile, n fastest, all
+// tiles along the grid's x (its y ends at 65535).
 constexpr int kSimtTile = 64, kSimtK = 16;
 
 __global__ void __launch_bounds__(256) simt_gemm_f32_kernel(const float* __restrict__ A, int64_t sam, int64_t sak,
@@ -19,7 +20,8 @@ __global__ void __launch_bounds__(256) simt_gemm_f32_kernel(const float* __restr
                                                             int64_t N, int64_t K, int accumulate) {
   __shared__ float As[kSimtK][kSimtTile + 4];
   __shared__ float Bs[kSimtK][kSimtTile + 4];
-  const int64_t m0 = (int64_t)blockIdx.y * kSimtTile, n0 = (int64_t)blockIdx.x * kSimtTile;
+  const uint32_t n_tiles = static_cast<uint32_t>((N + kSimtTile - 1) / kSimtTile);
+  const int64_t m0 = (int64_t)(blockIdx.x / n_tiles) * kSimtTile, n0 = (int64_t)(blockIdx.x % n_tiles) * kSimtTile;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   float acc[4][4] = {};
   for (int64_t k0 = 0; k0 < K; k0 += kSimtK) {

@@ -99,3 +99,34 @@ def test_clip_gradients_between_each_other():
     assert float(norm) == pytest.approx(want, rel=2.0 ** -23)
     # the factor, its product and the value are rounded to fp32
     within(flat, before / (want + 1e-6), before.abs() / want * 2.0 ** -22)
+
+
+# ------------------------------------------------------------------------------------------ exact sums
+def integers(*shape, seed, dtype, density):
+    """-1, 0 and 1; `density` of them not 0."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    u = torch.rand(shape, generator=g, device="cuda")
+    return (u < density / 2).to(dtype) - (u > 1 - density / 2).to(dtype)
+
+
+def check_exact(x, wg, wu, dh):
+    """ReLU block on small integers. Products of at most 256 are exact in every type, and so are dg and du; all
+    sums are integers below 2^24, exact in fp32 in any order. Each result is the exact one, rounded once."""
+    dt = x.dtype
+    got = glu_pass(x, wg, wu, "relu", dh)
+    x, wg, wu, dh = (t.double() for t in (x, wg, wu, dh))
+    g, u = x @ wg.T, x @ wu.T
+    assert float(g.abs().max()) <= 256 and float(u.abs().max()) <= 256
+    a, d = g.relu(), (g > 0).double()
+    dg, du = dh * u * d, dh * a
+    for name, y, want in zip(("h", "dx", "dgate", "dup"), got, (a * u, dg @ wg + du @ wu, dg.T @ x, du.T @ x)):
+        assert float(want.abs().max()) < 2 ** 24
+        wrong = y != want.to(dt)
+        assert not bool(wrong.any()), (name, wrong.nonzero()[:3].tolist(), int(wrong.sum()))
+
+
+@pytest.mark.parametrize("n,h,f", [(65535 * 64 + 1, 8, 3), (2, 3, 65535 * 32 + 40)])
+def test_glu_fp32_sizes_of_more_than_65535_tiles(n, h, f):
+    """Rows (h, dx), and features (weight gradients), behind 65535 tiles of 64."""
+    check_exact(integers(n, h, seed=1, dtype=FP32, density=0.7), integers(f, h, seed=2, dtype=FP32, density=0.7),
+                integers(f, h, seed=3, dtype=FP32, density=0.7), integers(n, f, seed=4, dtype=FP32, density=0.1))
