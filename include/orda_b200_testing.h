@@ -43,6 +43,10 @@ int32_t orda_debug_gemm_profile(uint64_t* out, int32_t reset);
  * *waited_ns (device uint64) and the kernel returns, leaving the context usable. */
 int32_t orda_debug_wait_timeout(int32_t* status, uint64_t limit_ns, uint64_t* waited_ns, void* stream);
 
+/* A launch that the CUDA runtime refuses on the host (more threads than a block can have), checked like every
+ * other one: returns ORDA_ERR_CUDA, runs nothing, and leaves no error behind for the thread's next call. */
+int32_t orda_debug_failed_launch(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

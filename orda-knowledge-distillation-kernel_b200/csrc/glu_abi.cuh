@@ -96,7 +96,8 @@ int glu_swap_launch(const orda_glu_args_t* a, cudaStream_t s) {
   cfg.attrs = &cluster;
   cfg.numAttrs = 1;
   count_launch();
-  return cudaLaunchKernelEx(&cfg, glu_swap_kernel<T16>, p) == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  cudaLaunchKernelEx(&cfg, glu_swap_kernel<T16>, p);
+  return launch_status();
 }
 
 template <typename T16>
@@ -363,11 +364,9 @@ int32_t orda_glu_backward(const orda_glu_args_t* args, void* workspace, size_t w
   if (rc) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (args->rows == 0) {
-    if (args->dweights &&
-        cudaMemsetAsync(args->dweights, 0, esize(args->dtype) * (round8(args->ffn) + args->ffn) * args->grad_cols, s) !=
-            cudaSuccess)
-      return ORDA_ERR_CUDA;
-    return ORDA_OK;
+    if (args->dweights)
+      cudaMemsetAsync(args->dweights, 0, esize(args->dtype) * (round8(args->ffn) + args->ffn) * args->grad_cols, s);
+    return launch_status();
   }
   const GluPlan P = plan_glu_backward(args);
   if (!workspace || workspace_bytes < P.total) return ORDA_ERR_WORKSPACE;

@@ -31,6 +31,8 @@ inline int num_sms() {
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline size_t esize(int dtype) { return dtype == ORDA_F32 ? 4 : 2; }
-inline int launch_status() { return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA; }
+// Result of the launches since the last check. It takes the error with it: left pending, a failed launch would
+// be reported again by the thread's next call, whose own launches went well.
+inline int launch_status() { return cudaGetLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA; }
 
 }  // namespace orda

@@ -250,7 +250,7 @@ int launch_tc(TcGemmParams& prm, int64_t M, int64_t N, cudaStream_t stream, int 
   const int grid = static_cast<int>(std::min<int64_t>(tiles, num_sms()));
   count_launch();
   k<<<grid, kGemmThreads, S::kSmemBytes, stream>>>(prm);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 // Pipeline counters of the pair GEMMs are collected when ORDA_GEMM_PROFILE=1 (testing hook; read back
@@ -297,7 +297,7 @@ int launch_tc2(TcGemmParams& prm, int64_t M_tiles, int64_t N, cudaStream_t strea
   const int pairs = static_cast<int>(std::min<int64_t>(tiles, usable / 2));
   count_launch();
   k<<<2 * pairs, S::kThreads, S::kSmemBytes, stream>>>(prm);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 
@@ -319,7 +319,7 @@ int launch_tc2w(TcGemmParams& prm, int64_t M_tiles, int64_t N, cudaStream_t stre
   const int pairs = static_cast<int>(std::min<int64_t>(tiles, usable / 2));
   count_launch();
   k<<<2 * pairs, S::kThreads, S::kSmemBytes, stream>>>(prm);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 
@@ -460,7 +460,7 @@ int dh_tc(const orda_distill_args_t* a, const Plan& P, uint8_t* ws, const void* 
   count_launch();
   sum_split_kernel<T16><<<static_cast<int>(std::min<int64_t>(cdiv(count8, 256), 4 * 148)), 256, 0, s>>>(
       part, P.dh_split, rows * n, static_cast<T16*>(out), count8);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 // dW[V, N] (+)= dZ0^T H0 (+ dZ1^T H1)
@@ -537,7 +537,7 @@ int forward_f32(const orda_distill_args_t* a, const Plan& P, uint8_t* ws, const 
   count_launch();
   if (P.teacher_acc) fwd_stats_gmem_kernel<true><<<grid, 128, 0, s>>>(f);
   else fwd_stats_gmem_kernel<false><<<grid, 128, 0, s>>>(f);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 // ------------------------------------------------------------------ shared row phases
@@ -561,7 +561,7 @@ int row_phases(const orda_distill_args_t* a, const Plan& P, uint8_t* ws, const C
     }
     launch_grad_sweep<WsT>(r, sweep_grid, s);
     row_loss_kernel<<<static_cast<int>(cdiv(c.rows, 256)), 256, 0, s>>>(r);
-    return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+    return launch_status();
   }
   if (do_merge) {
     count_launch();
@@ -572,7 +572,7 @@ int row_phases(const orda_distill_args_t* a, const Plan& P, uint8_t* ws, const C
                                                                               r.row_stats);
     }
   }
-  if (!do_loss_and_sweeps) return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  if (!do_loss_and_sweeps) return launch_status();
   if (row_stats_ext) r.row_stats = const_cast<float*>(row_stats_ext);
   if (P.jsd && !row_sums_ext) {
     count_launch();
@@ -592,7 +592,7 @@ int row_phases(const orda_distill_args_t* a, const Plan& P, uint8_t* ws, const C
     count_launch();
     launch_grad_sweep<WsT>(r, sweep_grid, s);
   }
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 // Records the start / end event of a phase (instrumentation hook; no-op without events).
@@ -642,7 +642,7 @@ int grad_gemms(const orda_distill_args_t* a, const Plan& P, uint8_t* ws, const C
                 static_cast<float*>(a->grad_teacher_weight), a->teacher_hidden, a->vocab, a->teacher_hidden, c.rows,
                 acc, s);
     if (last_chunk && a->dweight_done_event) cudaEventRecord(static_cast<cudaEvent_t>(a->dweight_done_event), s);
-    rc = cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+    rc = launch_status();
   } else {
     int32_t* st = a->device_status;
     auto dhidden = [&]() -> int {
@@ -754,7 +754,7 @@ int run_all(const orda_distill_args_t* a, const Plan& P, uint8_t* ws, cudaStream
   count_launch();
   finalize_kernel<<<1, 1024, 0, s>>>(rl, a->n_rows, a->labels, a->n_rows, a->ignore_index, a->reduction, P.flags,
                                      a->student_ce_weight, a->teacher_ce_weight, a->kl_weight, a->out_reduced);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 int dispatch_all(const orda_distill_args_t* a, const Plan& P, uint8_t* ws, cudaStream_t s) {
@@ -787,7 +787,7 @@ int32_t orda_scale_grad(void* data, int64_t n, int32_t dtype, const float* scale
     case ORDA_F32: scale_grad_kernel<float><<<grid, 256, 0, s>>>(static_cast<float*>(data), n, scale); break;
     default: return ORDA_ERR_INVALID_ARGUMENT;
   }
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 const char* orda_status_string(int32_t status) {
@@ -911,7 +911,7 @@ int32_t orda_peer_reduce_broadcast(const orda_peer_slots_t* peers, int64_t vocab
   count_launch();
   if (dtype == ORDA_BF16) peer_reduce_broadcast_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(q);
   else peer_reduce_broadcast_kernel<__half><<<grid, 256, 0, s>>>(q);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 // ---------------------------------------------------------------- vocab-sharded phases
@@ -937,7 +937,7 @@ int32_t orda_shard_forward(const orda_distill_args_t* args, void* workspace, siz
   }
   if (rc) return rc;
   cudaMemcpyAsync(row_stats, ws + P.off_row_stats, sizeof(float) * kRowStats * args->n_rows, cudaMemcpyDeviceToDevice, s);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 int32_t orda_merge_row_stats(const float* gathered, int32_t world, int64_t n_rows, float* row_stats, void* stream) {
@@ -945,7 +945,7 @@ int32_t orda_merge_row_stats(const float* gathered, int32_t world, int64_t n_row
   const int grid = static_cast<int>(std::min<int64_t>(cdiv(n_rows, 256), 65535));
   count_launch();
   merge_records_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(gathered, world, n_rows, row_stats);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 int32_t orda_shard_jsd_partials(const orda_distill_args_t* args, void* workspace, size_t workspace_bytes,
@@ -967,7 +967,7 @@ int32_t orda_shard_jsd_partials(const orda_distill_args_t* args, void* workspace
     case ORDA_F16: jsd_sweep_kernel<__half><<<grid, 256, 0, s>>>(r, row_sums); break;
     default: jsd_sweep_kernel<float><<<grid, 256, 0, s>>>(r, row_sums); break;
   }
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 int32_t orda_shard_backward(const orda_distill_args_t* args, void* workspace, size_t workspace_bytes,
@@ -1006,7 +1006,7 @@ int32_t orda_shard_backward(const orda_distill_args_t* args, void* workspace, si
   finalize_kernel<<<1, 1024, 0, s>>>(rl, args->n_rows, args->labels, args->n_rows, args->ignore_index,
                                      args->reduction, P.flags, args->student_ce_weight, args->teacher_ce_weight,
                                      args->kl_weight, args->out_reduced);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
 }
 
 // ---------------------------------------------------------------- testing hook
@@ -1157,7 +1157,13 @@ extern "C" int32_t orda_debug_wait_timeout(int32_t* status, uint64_t limit_ns, u
   if (!status || !waited_ns || limit_ns == 0 || limit_ns > ORDA_WAIT_TIMEOUT_NS) return ORDA_ERR_INVALID_ARGUMENT;
   count_launch();
   wait_timeout_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(status, limit_ns, waited_ns);
-  return cudaPeekAtLastError() == cudaSuccess ? ORDA_OK : ORDA_ERR_CUDA;
+  return launch_status();
+}
+
+extern "C" int32_t orda_debug_failed_launch(void* stream) {
+  // refused by the runtime on the host: a block has 1024 threads at most
+  wait_timeout_kernel<<<1, 2048, 0, static_cast<cudaStream_t>(stream)>>>(nullptr, 1, nullptr);
+  return launch_status();
 }
 
 extern "C" int32_t orda_debug_gemm_profile(uint64_t* out, int32_t reset) {

@@ -296,10 +296,8 @@ int32_t orda_qk_norm_rotary_backward(const orda_rotary_args_t* args, void* works
   if (rc) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (args->batch * args->seq == 0 || args->heads[0] + args->heads[1] == 0) {
-    for (int i = 0; i < 2; ++i)
-      if (cudaMemsetAsync(args->dweight[i], 0, esize(args->weight_dtype) * args->head_dim, s) != cudaSuccess)
-        return ORDA_ERR_CUDA;
-    return ORDA_OK;
+    for (int i = 0; i < 2; ++i) cudaMemsetAsync(args->dweight[i], 0, esize(args->weight_dtype) * args->head_dim, s);
+    return launch_status();
   }
   if (!workspace || workspace_bytes < orda_qk_norm_rotary_backward_workspace_bytes(args)) return ORDA_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15u) return ORDA_ERR_ALIGNMENT;

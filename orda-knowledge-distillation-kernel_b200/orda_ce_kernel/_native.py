@@ -178,6 +178,7 @@ EXPORTED_SYMBOLS = (
     "orda_debug_gemm_profile",
     "orda_debug_gemm_wide",
     "orda_debug_wait_timeout",
+    "orda_debug_failed_launch",
 )
 
 _lib = None
@@ -255,6 +256,8 @@ def _declare(lib):
     lib.orda_debug_gemm_wide.argtypes = lib.orda_debug_gemm.argtypes
     lib.orda_debug_gemm_profile.restype = _i32
     lib.orda_debug_gemm_profile.argtypes = [ctypes.c_void_p, _i32]
+    lib.orda_debug_failed_launch.restype = _i32
+    lib.orda_debug_failed_launch.argtypes = [_vp]
     lib.orda_debug_wait_timeout.restype = _i32
     lib.orda_debug_wait_timeout.argtypes = [_vp, ctypes.c_uint64, _vp, _vp]
 

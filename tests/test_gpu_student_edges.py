@@ -130,3 +130,17 @@ def test_glu_fp32_sizes_of_more_than_65535_tiles(n, h, f):
     """Rows (h, dx), and features (weight gradients), behind 65535 tiles of 64."""
     check_exact(integers(n, h, seed=1, dtype=FP32, density=0.7), integers(f, h, seed=2, dtype=FP32, density=0.7),
                 integers(f, h, seed=3, dtype=FP32, density=0.7), integers(n, f, seed=4, dtype=FP32, density=0.1))
+
+
+# ------------------------------------------------------------------------------------------ errors of a launch
+def test_a_failed_launch_is_reported_once():
+    lib, stream = _native.load(), torch.cuda.current_stream().cuda_stream
+    g, q = [torch.ones(4, device="cuda")], randn(3, 2, 16, seed=1)
+    pos, cfg = torch.arange(3, device="cuda"), student.RotaryConfig(16)
+    calls = (lambda: student.grad_norm(g), lambda: student.rotary_embedding(q, q, pos, cfg)[0],
+             lambda: glu_pass(*glu_inputs(40, 64, 72, BF16, 3)[:3], "silu", torch.ones(40, 72, device="cuda", dtype=BF16))[1],
+             lambda: glu_pass(*glu_inputs(300, 64, 72, BF16, 3)[:3], "silu", torch.ones(300, 72, device="cuda", dtype=BF16))[1])
+    want = [c() for c in calls]
+    for call, w in zip(calls, want):
+        assert lib.orda_debug_failed_launch(stream) == _native.ERR_CUDA
+        assert torch.equal(call(), w)
