@@ -56,7 +56,8 @@ typedef struct orda_glu_args {
   int32_t* device_status;               /* int32 device word, zero on entry of a forward call; a backward call
                                            clears it. May be NULL for ORDA_F32 and for a forward call of
                                            at most ORDA_GLU_FEW_ROWS rows. Where it reports a
-                                           timeout, the first value of h, dx or dweights is NaN */
+                                           timeout, the first value of h, dx or of both gradients in
+                                           dweights is NaN */
 } orda_glu_args_t;
 
 /* Copies of up to three 16-bit matrices (rows of `cols` elements, any alignment, ld[i] elements apart) whose

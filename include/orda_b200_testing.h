@@ -6,7 +6,10 @@
 #ifndef ORDA_B200_TESTING_H_
 #define ORDA_B200_TESTING_H_
 
+#include <stddef.h>
 #include <stdint.h>
+
+#include "orda_b200_student.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -42,6 +45,13 @@ int32_t orda_debug_gemm_profile(uint64_t* out, int32_t reset);
  * up, writes ORDA_ERR_TIMEOUT to *status (device int32, zero on entry), stores the time it waited in
  * *waited_ns (device uint64) and the kernel returns, leaving the context usable. */
 int32_t orda_debug_wait_timeout(int32_t* status, uint64_t limit_ns, uint64_t* waited_ns, void* stream);
+
+/* The calls of orda_b200_student.h (16-bit types; forward: more than ORDA_GLU_FEW_ROWS rows), each of whose products
+ * then marks its results by the code that a block runs after a wait that timed out. No wait does: what else is
+ * written is right. */
+int32_t orda_debug_glu_forward_marked(const orda_glu_args_t* args, void* stream);
+int32_t orda_debug_glu_backward_marked(const orda_glu_args_t* args, void* workspace, size_t workspace_bytes,
+                                       void* stream);
 
 /* A launch that the CUDA runtime refuses on the host (more threads than a block can have), checked like every
  * other one: returns ORDA_ERR_CUDA, runs nothing, and leaves no error behind for the thread's next call. */

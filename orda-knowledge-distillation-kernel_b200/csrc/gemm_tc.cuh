@@ -71,9 +71,10 @@ struct TcGemmParams {
   int64_t split_bytes;
   int32_t prof_slot;  // >= 0: accumulate pipeline wait counters into g_tc2_prof[prof_slot] (testing hook)
   int32_t* status;
-  // 16-bit word that a block writes 0x7fff to when it ends with a pipeline wait timed out (may be NULL): the
-  // result's first value (of an fp32 one the upper half), NaN in every type, for callers that read no status
-  uint16_t* poison;
+  // 16-bit words that a block writes 0x7fff to when it ends with a pipeline wait timed out (may be NULL): the
+  // first value of each result (of an fp32 one the upper half; two where the product is two weights'
+  // gradients), NaN in every type, for callers that read no status
+  uint16_t* poison[2];
   // EPI_GLU: b0 / b1 are the gate / up weights, out_map stores h, ws_s_map / ws_t_map the products before
   // the activation (glu_save = 1)
   int32_t glu_act, glu_save;
@@ -81,6 +82,14 @@ struct TcGemmParams {
   FwdEpiParams fwd;
   StoreEpiParams st;
 };
+
+// By one thread, after its block's own stores: of two blocks that write a marked value the one that ends last
+// has seen the status, or the other one has.
+__device__ __forceinline__ void mark_timeout(const TcGemmParams& p) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (p.poison[i]) *p.poison[i] = 0x7fffu;
+}
 
 template <int BN>
 struct GemmShape {

@@ -630,7 +630,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape<EPI>::kThr
   if (warp == 1) {
     tc_fence_after();
     if (*reinterpret_cast<volatile int32_t*>(p.status) == ORDA_ERR_TIMEOUT) {
-      if (p.poison && lane == 0) *p.poison = 0x7fffu;
+      if (lane == 0) mark_timeout(p);
       __syncwarp();
       __nanosleep(1000000);
     }

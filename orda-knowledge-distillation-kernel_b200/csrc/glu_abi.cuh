@@ -100,6 +100,17 @@ int glu_swap_launch(const orda_glu_args_t* a, cudaStream_t s) {
   return launch_status();
 }
 
+// Testing hook (orda_debug_glu_*_marked): every product of the thread's calls ends as if a wait had timed out.
+thread_local bool t_mark_products = false;
+
+__global__ void mark_timeout_kernel(const __grid_constant__ TcGemmParams p) { mark_timeout(p); }
+
+int mark_if_testing(const TcGemmParams& prm, cudaStream_t s) {
+  if (!t_mark_products) return ORDA_OK;
+  mark_timeout_kernel<<<1, 1, 0, s>>>(prm);
+  return launch_status();
+}
+
 template <typename T16>
 int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
   if (a->rows <= 8) return glu_rows_launch<T16>(a, s);
@@ -116,7 +127,7 @@ int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
     prm.glu_h = a->h;
     prm.st.ldo = a->ld_h;
   }
-  prm.poison = static_cast<uint16_t*>(a->h);
+  prm.poison[0] = static_cast<uint16_t*>(a->h);
   prm.glu_act = a->activation;
   prm.glu_save = a->pre_gate != nullptr;
   if (prm.glu_save) {
@@ -135,9 +146,9 @@ int glu_forward_tc(const orda_glu_args_t* a, cudaStream_t s) {
   const int64_t wide = cdiv(cdiv(a->rows, 512) * f_tiles, pairs) * (1050 * prm.kb0 + 9500);
   const int64_t half = cdiv(cdiv(a->rows, 256) * f_tiles, pairs) * (620 * prm.kb0 + 2000);
   const int64_t cols = 2 * round8(a->ffn);
-  if (half < wide)
-    return launch_tc2<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 256), cols, s, 8);
-  return launch_tc2w<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 512), cols, s, 8);
+  rc = half < wide ? launch_tc2<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 256), cols, s, 8)
+                   : launch_tc2w<false, false, A_PLAIN, false, EPI_GLU, T16>(prm, cdiv(a->rows, 512), cols, s, 8);
+  return rc ? rc : mark_if_testing(prm, s);
 }
 
 // K split of a gradient GEMM with M x N outputs and `kb` k blocks on the wide kernel: the split whose
@@ -203,13 +214,15 @@ int make_partial_map(CUtensorMap* m, void* base, int64_t N, int64_t M, int split
 }
 
 // Destination of a gradient GEMM: `out` itself, or fp32 partials added in a fixed order by sum_split_kernel;
-// both leave by TMA stores.
+// both leave by TMA stores. `second`: the row where another result starts (0: none), marked of its own on a timeout.
 template <bool A_MN, bool TWO_SEG, typename T16>
-int glu_grad_gemm(TcGemmParams& prm, int dtype, int64_t M, int64_t N, int split, void* out, uint8_t* part,
-                  cudaStream_t s) {
+int glu_grad_gemm(TcGemmParams& prm, int dtype, int64_t M, int64_t N, int64_t second, int split, void* out,
+                  uint8_t* part, cudaStream_t s) {
   int rc;
   const int64_t np = round8(N);
-  prm.poison = split <= 1 ? static_cast<uint16_t*>(out) : reinterpret_cast<uint16_t*>(part) + 1;
+  for (int i = 0; i < (second ? 2 : 1); ++i)
+    prm.poison[i] = split <= 1 ? static_cast<uint16_t*>(out) + i * second * N
+                               : reinterpret_cast<uint16_t*>(part) + 2 * i * second * np + 1;
   if (split <= 1) {
     prm.st = StoreEpiParams{out, N, M, N, 0, 0};
     if (N == np) {
@@ -218,7 +231,8 @@ int glu_grad_gemm(TcGemmParams& prm, int dtype, int64_t M, int64_t N, int split,
     } else {
       prm.st_tma = 3;
     }
-    return launch_tc2w<A_MN, true, A_PLAIN, TWO_SEG, EPI_STORE, T16>(prm, cdiv(M, 512), N, s, 4);
+    rc = launch_tc2w<A_MN, true, A_PLAIN, TWO_SEG, EPI_STORE, T16>(prm, cdiv(M, 512), N, s, 4);
+    return rc ? rc : mark_if_testing(prm, s);
   }
   prm.ksplit = split;
   prm.kb_split = static_cast<int32_t>(cdiv(prm.kb0 + prm.kb1, split));
@@ -227,6 +241,7 @@ int glu_grad_gemm(TcGemmParams& prm, int dtype, int64_t M, int64_t N, int split,
   if ((rc = make_partial_map(&prm.out_map, part, np, M, split))) return rc;  // (rows of 32-byte multiples)
   prm.st_tma = 2;
   if ((rc = launch_tc2w<A_MN, true, A_PLAIN, TWO_SEG, EPI_STORE, T16>(prm, cdiv(M, 512), N, s, 4))) return rc;
+  if ((rc = mark_if_testing(prm, s))) return rc;
   count_launch();
   const float* sums = reinterpret_cast<const float*>(part);
   if (N == np) {
@@ -268,7 +283,7 @@ int glu_backward_tc(const orda_glu_args_t* a, const GluPlan& P, uint8_t* ws, cud
     if ((rc = make_operand_map(&prm.b0, a->dtype, a->gate, true, a->grad_cols, a->ffn, a->ld_gate, 128))) return rc;
     if ((rc = make_operand_map(&prm.b1, a->dtype, a->up, true, a->grad_cols, a->ffn, a->ld_up, 128))) return rc;
     prm.kb0 = prm.kb1 = static_cast<int32_t>(cdiv(a->ffn, kBK));
-    if ((rc = glu_grad_gemm<false, true, T16>(prm, a->dtype, a->rows, a->grad_cols, P.split_dx, a->dx, part, s)))
+    if ((rc = glu_grad_gemm<false, true, T16>(prm, a->dtype, a->rows, a->grad_cols, 0, P.split_dx, a->dx, part, s)))
       return rc;
   }
   if (a->dweights) {  // [dg | du]^T x: both weights' gradients are one product of fp + ffn rows
@@ -278,7 +293,7 @@ int glu_backward_tc(const orda_glu_args_t* a, const GluPlan& P, uint8_t* ws, cud
     if ((rc = make_operand_map(&prm.a0, a->dtype, dgu, true, m, a->rows, ld, kTileRows))) return rc;
     if ((rc = make_operand_map(&prm.b0, a->dtype, a->x, true, a->grad_cols, a->rows, a->ld_x, 128))) return rc;
     prm.kb0 = static_cast<int32_t>(cdiv(a->rows, kBK));
-    if ((rc = glu_grad_gemm<true, false, T16>(prm, a->dtype, m, a->grad_cols, P.split_dw, a->dweights, part, s)))
+    if ((rc = glu_grad_gemm<true, false, T16>(prm, a->dtype, m, a->grad_cols, P.fp, P.split_dw, a->dweights, part, s)))
       return rc;
   }
   return ORDA_OK;
@@ -377,6 +392,20 @@ int32_t orda_glu_backward(const orda_glu_args_t* args, void* workspace, size_t w
     case ORDA_F16: return glu_backward_tc<__half>(args, P, ws, s);
     default: return glu_backward_f32(args, P, ws, s);
   }
+}
+
+int32_t orda_debug_glu_forward_marked(const orda_glu_args_t* args, void* stream) {
+  t_mark_products = true;
+  const int32_t rc = orda_glu_forward(args, stream);
+  t_mark_products = false;
+  return rc;
+}
+
+int32_t orda_debug_glu_backward_marked(const orda_glu_args_t* args, void* workspace, size_t workspace_bytes, void* stream) {
+  t_mark_products = true;
+  const int32_t rc = orda_glu_backward(args, workspace, workspace_bytes, stream);
+  t_mark_products = false;
+  return rc;
 }
 
 }  // extern "C"

@@ -179,6 +179,8 @@ EXPORTED_SYMBOLS = (
     "orda_debug_gemm_wide",
     "orda_debug_wait_timeout",
     "orda_debug_failed_launch",
+    "orda_debug_glu_forward_marked",
+    "orda_debug_glu_backward_marked",
 )
 
 _lib = None
@@ -256,6 +258,10 @@ def _declare(lib):
     lib.orda_debug_gemm_wide.argtypes = lib.orda_debug_gemm.argtypes
     lib.orda_debug_gemm_profile.restype = _i32
     lib.orda_debug_gemm_profile.argtypes = [ctypes.c_void_p, _i32]
+    lib.orda_debug_glu_forward_marked.restype = _i32
+    lib.orda_debug_glu_forward_marked.argtypes = [PG, _vp]
+    lib.orda_debug_glu_backward_marked.restype = _i32
+    lib.orda_debug_glu_backward_marked.argtypes = [PG, _vp, ctypes.c_size_t, _vp]
     lib.orda_debug_failed_launch.restype = _i32
     lib.orda_debug_failed_launch.argtypes = [_vp]
     lib.orda_debug_wait_timeout.restype = _i32

@@ -144,3 +144,35 @@ def test_a_failed_launch_is_reported_once():
     for call, w in zip(calls, want):
         assert lib.orda_debug_failed_launch(stream) == _native.ERR_CUDA
         assert torch.equal(call(), w)
+
+
+# one product each, K-split products, rows of a multiple of 8 and not (grad_cols)
+@pytest.mark.parametrize("n,h,cols,f", [(300, 64, 64, 75), (2048, 1024, 1024, 2816), (1111, 1000, 997, 2730)])
+def test_c_glu_results_marked_by_a_timeout(n, h, cols, f):
+    """The marks of a wait that timed out make the first value of h, of dx and of each weight's gradient NaN,
+    whether the gradients come from one product or from partial sums, and nothing else."""
+    x, wg, wu, dh = glu_inputs(n, h, f, BF16, 61)
+    lib, fp = _native.load(), (f + 7) // 8 * 8
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def run(forward, backward):
+        y, pre = torch.empty(n, f, device="cuda", dtype=BF16), torch.empty(2, n, fp, device="cuda", dtype=BF16)
+        dx, dw = torch.empty(n, cols, device="cuda", dtype=BF16), torch.zeros(fp + f, cols, device="cuda", dtype=BF16)
+        status = torch.zeros(1, device="cuda", dtype=torch.int32)
+        a = _native.GluArgs(abi_version=_native.ABI_VERSION, dtype=_native.BF16, activation=_native.ACT_SILU, rows=n, hidden=h,
+                            ffn=f, x=x.data_ptr(), ld_x=h, gate=wg.data_ptr(), ld_gate=h, up=wu.data_ptr(), ld_up=h,
+                            h=y.data_ptr(), ld_h=f, pre_gate=pre[0].data_ptr(), ld_pre=fp, pre_up=pre[1].data_ptr(),
+                            grad_cols=cols, dh=dh.data_ptr(), dx=dx.data_ptr(), dweights=dw.data_ptr(),
+                            device_status=status.data_ptr())
+        assert forward(a, stream) == _native.OK
+        need = lib.orda_glu_backward_workspace_bytes(a)
+        ws = torch.empty(need, device="cuda", dtype=torch.uint8)
+        assert backward(a, ws.data_ptr(), need, stream) == _native.OK
+        return y, dx, dw[:f], dw[fp:]
+
+    want = run(lib.orda_glu_forward, lib.orda_glu_backward)
+    got = run(lib.orda_debug_glu_forward_marked, lib.orda_debug_glu_backward_marked)
+    for a, b in zip(got, want):
+        assert bool(torch.isnan(a[0, 0])) and bool(torch.isfinite(b).all())
+        a[0, 0] = b[0, 0]
+        assert torch.equal(a, b)
