@@ -59,6 +59,11 @@ void require_like(const char* what, const Tensor& t, at::IntArrayRef size, const
                     t.scalar_type(), ", on ", t.device());
 }
 
+// There is no forward-mode derivative; a result without a tangent would count as a constant.
+void refuse_tangent(const char* what, const Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivative, and an input carries a tangent");
+}
+
 // A zeroed device word for the kernels' bounded waits.
 Tensor new_status(const Tensor& like, cudaStream_t s) {
   Tensor t = new_empty({1}, at::kInt, like);
@@ -286,8 +291,9 @@ at::ScalarType compute_dtype(std::initializer_list<const Tensor*> tensors) {
 }
 
 Tensor gated_linear_unit(const Tensor& x, const Tensor& gate_weight, const Tensor& up_weight,
-                         const std::string& activation) {
+                                        const std::string& activation) {
   const int64_t act = activation_code(activation);
+  for (const Tensor* t : {&x, &gate_weight, &up_weight}) refuse_tangent("gated_linear_unit", *t);
   check_glu(x, gate_weight, up_weight);
   const auto dt = compute_dtype({&gate_weight, &up_weight, &x});
   auto cast = [dt](const Tensor& t) { return t.scalar_type() == dt ? t : t.to(dt); };
@@ -506,8 +512,10 @@ struct QkNormRotaryFunction : torch::autograd::Function<QkNormRotaryFunction> {
 
 std::tuple<Tensor, Tensor> two(const variable_list& v) { return {v[0], v[1]}; }
 
-std::tuple<Tensor, Tensor> rotary_embedding(const Tensor& q_, const Tensor& k_, const Tensor& positions, PlanPtr plan) {
+std::tuple<Tensor, Tensor> rotary_embedding(const Tensor& q_, const Tensor& k_, const Tensor& positions,
+                                                           PlanPtr plan) {
   check_qk("rotary_embedding", q_, k_, positions, *plan);
+  for (const Tensor* t : {&q_, &k_}) refuse_tangent("rotary_embedding", *t);
   require_cuda("rotary_embedding", q_, {&k_, &positions});
   const Tensor q = dense_last(q_), k = dense_last(k_);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad()))
@@ -515,10 +523,12 @@ std::tuple<Tensor, Tensor> rotary_embedding(const Tensor& q_, const Tensor& k_, 
   return two(rotate(q, k, positions, *plan, false, {}, {}, 0.0));
 }
 
-std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q_, const Tensor& k_, const Tensor& q_weight, const Tensor& k_weight,
-                             const Tensor& positions, PlanPtr plan, double eps) {
+std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q_, const Tensor& k_, const Tensor& q_weight,
+                                                         const Tensor& k_weight, const Tensor& positions, PlanPtr plan,
+                                                         double eps) {
   check_qk("qk_norm_rotary", q_, k_, positions, *plan);
   check_norm_weights("qk_norm_rotary", q_weight, k_weight, *plan, eps);
+  for (const Tensor* t : {&q_, &k_, &q_weight, &k_weight}) refuse_tangent("qk_norm_rotary", *t);
   require_cuda("qk_norm_rotary", q_, {&k_, &positions, &q_weight, &k_weight});
   const Tensor q = dense_last(q_), k = dense_last(k_), wq = q_weight.contiguous(), wk = k_weight.contiguous();
   if (at::GradMode::is_enabled() &&
@@ -595,6 +605,7 @@ void refuse_shared_memory(const char* what, const std::vector<Tensor>& grads) {
 
 void check_gradients(const char* what, const std::vector<Tensor>& grads, bool in_place = false) {
   for (const Tensor& g : grads) {
+    refuse_tangent(what, g);
     TORCH_CHECK_VALUE(supported(g.scalar_type()), what, ": gradients must be float32, float16 or bfloat16, got ",
                       g.scalar_type());
     TORCH_CHECK_VALUE(g.layout() == at::kStrided, what, ": gradients must be strided tensors, got ", g.layout());

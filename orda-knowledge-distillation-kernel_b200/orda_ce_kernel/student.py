@@ -7,8 +7,8 @@ and training loop of ``test/benchmark/src/core.py:106-138`` and ``_train.py:102-
 * :func:`qk_norm_rotary` - per-head RMS norms of queries and keys, rotated in the same pass;
 * :func:`grad_norm`, :func:`clip_gradients`, :func:`clip_grad_norm_` - the global gradient norm and clipping.
 
-The first three back-propagate (once; no double backward) and trace into one custom op each under
-``torch.compile``. As for the loss there is no CPU fallback: CUDA tensors on a B200 are required. Every call
+The first three back-propagate (once; no double backward, no forward-mode derivative: an input that carries a
+tangent is refused) and trace into one custom op each under ``torch.compile``. As for the loss there is no CPU fallback: CUDA tensors on a B200 are required. Every call
 runs on the current stream of its tensors' device, takes its workspace from the caching allocator and
 does not synchronise, so it can be captured into a CUDA graph; a captured backward pass is refused while an
 eager autograd graph of the default stream still holds one of its leaves.

@@ -99,3 +99,27 @@ def test_clip_refuses_gradients_that_share_memory():
     for grads in ((flat[:60], flat[60:]), (flat[::2], flat[1::2]), (flat[:50].view(5, 10).T, flat[50:]), (flat[:0], flat[:0])):
         with pytest.raises(RuntimeError, match="no CPU fallback"):  # well-formed
             _clip(*grads)
+
+
+# ------------------------------------------------------------------------------------------ tangents and recorders
+def test_inputs_that_carry_a_tangent_are_refused():
+    """A result without one would count as a constant."""
+    from torch.autograd import forward_ad
+
+    x, w, v, pos, cfg = torch.randn(4, 2, 8), torch.randn(12, 8), torch.ones(8), torch.arange(4), student.RotaryConfig(8)
+    g = torch.ones(3)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        p = torch.nn.Parameter(torch.ones(3))
+        p.grad = dual(g)
+        for call in (lambda: student.gated_linear_unit(dual(x), w, w), lambda: student.gated_linear_unit(x, dual(w), w),
+                     lambda: student.gated_linear_unit(x, w, dual(w)), lambda: student.rotary_embedding(dual(x), x, pos, cfg),
+                     lambda: student.rotary_embedding(x, dual(x), pos, cfg),
+                     lambda: student.qk_norm_rotary(dual(x), x, v, v, pos, cfg),
+                     lambda: student.qk_norm_rotary(x, x, v, dual(v), pos, cfg),
+                     lambda: student.grad_norm([g, dual(g)]), lambda: student.clip_gradients([dual(g)], 1.0),
+                     lambda: student.clip_grad_norm_([p], 1.0)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
