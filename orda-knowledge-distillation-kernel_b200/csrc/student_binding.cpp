@@ -10,10 +10,13 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/custom_class.h>
 
@@ -57,6 +60,22 @@ void require_like(const char* what, const Tensor& t, at::IntArrayRef size, const
   TORCH_CHECK_VALUE(t.sizes() == size && t.scalar_type() == like.scalar_type() && t.device() == like.device(), what,
                     " must have shape ", size, ", ", like.scalar_type(), ", on ", like.device(), ", got ", t.sizes(), ", ",
                     t.scalar_type(), ", on ", t.device());
+}
+
+// Something records the calls that pass through PyTorch's dispatcher: these do not, and take the custom ops instead
+// (an empty result tells the caller to).
+bool recorded() {
+  return c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+         c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) || torch::jit::tracer::isTracing();
+}
+
+// For the calls that have no custom op: a graph would hold their results of this run as constants. (Modes that
+// only watch, such as a FLOP counter, do no harm.)
+void refuse_graph_recording(const char* what) {
+  TORCH_CHECK(!c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY) &&
+                  !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) &&
+                  !torch::jit::tracer::isTracing(),
+              what, " cannot be recorded into a graph; call it outside of the traced function");
 }
 
 // There is no forward-mode derivative; a result without a tangent would count as a constant.
@@ -290,10 +309,11 @@ at::ScalarType compute_dtype(std::initializer_list<const Tensor*> tensors) {
   return at::kFloat;
 }
 
-Tensor gated_linear_unit(const Tensor& x, const Tensor& gate_weight, const Tensor& up_weight,
+std::optional<Tensor> gated_linear_unit(const Tensor& x, const Tensor& gate_weight, const Tensor& up_weight,
                                         const std::string& activation) {
   const int64_t act = activation_code(activation);
   for (const Tensor* t : {&x, &gate_weight, &up_weight}) refuse_tangent("gated_linear_unit", *t);
+  if (recorded()) return std::nullopt;
   check_glu(x, gate_weight, up_weight);
   const auto dt = compute_dtype({&gate_weight, &up_weight, &x});
   auto cast = [dt](const Tensor& t) { return t.scalar_type() == dt ? t : t.to(dt); };
@@ -512,10 +532,11 @@ struct QkNormRotaryFunction : torch::autograd::Function<QkNormRotaryFunction> {
 
 std::tuple<Tensor, Tensor> two(const variable_list& v) { return {v[0], v[1]}; }
 
-std::tuple<Tensor, Tensor> rotary_embedding(const Tensor& q_, const Tensor& k_, const Tensor& positions,
+std::optional<std::tuple<Tensor, Tensor>> rotary_embedding(const Tensor& q_, const Tensor& k_, const Tensor& positions,
                                                            PlanPtr plan) {
   check_qk("rotary_embedding", q_, k_, positions, *plan);
   for (const Tensor* t : {&q_, &k_}) refuse_tangent("rotary_embedding", *t);
+  if (recorded()) return std::nullopt;
   require_cuda("rotary_embedding", q_, {&k_, &positions});
   const Tensor q = dense_last(q_), k = dense_last(k_);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad()))
@@ -523,12 +544,13 @@ std::tuple<Tensor, Tensor> rotary_embedding(const Tensor& q_, const Tensor& k_, 
   return two(rotate(q, k, positions, *plan, false, {}, {}, 0.0));
 }
 
-std::tuple<Tensor, Tensor> qk_norm_rotary(const Tensor& q_, const Tensor& k_, const Tensor& q_weight,
+std::optional<std::tuple<Tensor, Tensor>> qk_norm_rotary(const Tensor& q_, const Tensor& k_, const Tensor& q_weight,
                                                          const Tensor& k_weight, const Tensor& positions, PlanPtr plan,
                                                          double eps) {
   check_qk("qk_norm_rotary", q_, k_, positions, *plan);
   check_norm_weights("qk_norm_rotary", q_weight, k_weight, *plan, eps);
   for (const Tensor* t : {&q_, &k_, &q_weight, &k_weight}) refuse_tangent("qk_norm_rotary", *t);
+  if (recorded()) return std::nullopt;
   require_cuda("qk_norm_rotary", q_, {&k_, &positions, &q_weight, &k_weight});
   const Tensor q = dense_last(q_), k = dense_last(k_), wq = q_weight.contiguous(), wk = k_weight.contiguous();
   if (at::GradMode::is_enabled() &&
@@ -604,6 +626,7 @@ void refuse_shared_memory(const char* what, const std::vector<Tensor>& grads) {
 }
 
 void check_gradients(const char* what, const std::vector<Tensor>& grads, bool in_place = false) {
+  refuse_graph_recording(what);
   for (const Tensor& g : grads) {
     refuse_tangent(what, g);
     TORCH_CHECK_VALUE(supported(g.scalar_type()), what, ": gradients must be float32, float16 or bfloat16, got ",

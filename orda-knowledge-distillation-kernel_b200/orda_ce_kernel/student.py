@@ -8,10 +8,12 @@ and training loop of ``test/benchmark/src/core.py:106-138`` and ``_train.py:102-
 * :func:`grad_norm`, :func:`clip_gradients`, :func:`clip_grad_norm_` - the global gradient norm and clipping.
 
 The first three back-propagate (once; no double backward, no forward-mode derivative: an input that carries a
-tangent is refused) and trace into one custom op each under ``torch.compile``. As for the loss there is no CPU fallback: CUDA tensors on a B200 are required. Every call
-runs on the current stream of its tensors' device, takes its workspace from the caching allocator and
-does not synchronise, so it can be captured into a CUDA graph; a captured backward pass is refused while an
-eager autograd graph of the default stream still holds one of its leaves.
+tangent is refused) and become one custom op each under ``torch.compile`` and whatever else records calls
+(``make_fx``, ``torch.jit.trace``, dispatch modes); the last three refuse to be recorded into a graph. As for
+the loss there is no CPU fallback: CUDA tensors on a B200 are required. Every call runs on the current stream of
+its tensors' device, takes its workspace from the caching allocator and does not synchronise, so it can be
+captured into a CUDA graph; a captured backward pass is refused while an eager autograd graph of the default
+stream still holds one of its leaves.
 """
 from __future__ import annotations
 
@@ -98,13 +100,16 @@ def gated_linear_unit(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: tor
     cores' speed. Back-propagates into all three; the backward pass keeps the two products in the compute
     dtype. Inputs with a hidden size that is no multiple of 8 are copied into padded rows first.
     """
-    if torch.compiler.is_compiling():
+    h = None
+    if not torch.compiler.is_compiling():
+        h = (_binding or _bound()).gated_linear_unit(x, gate_weight, up_weight, activation)
+    if h is None:  # recorded: through the custom op
         if activation not in _ACT_CODE:
             raise ValueError(f"activation must be one of {sorted(_ACT_CODE)}, got {activation!r}")
         dtype = default_compute_dtype(gate_weight, up_weight, x)
-        return torch.ops.orda_b200.glu_forward(x.to(dtype), gate_weight.to(dtype), up_weight.to(dtype),
-                                               _ACT_CODE[activation])[0]
-    return (_binding or _bound()).gated_linear_unit(x, gate_weight, up_weight, activation)
+        h = torch.ops.orda_b200.glu_forward(x.to(dtype), gate_weight.to(dtype), up_weight.to(dtype),
+                                            _ACT_CODE[activation])[0]
+    return h
 
 
 # ------------------------------------------------------------------------------------------ rotary positions
@@ -264,9 +269,12 @@ def rotary_embedding(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     positions lose nothing. Back-propagates into ``q`` and ``k``.
     """
     _require_config("rotary_embedding", config)
-    if torch.compiler.is_compiling():
-        return torch.ops.orda_b200.rotary(q, k, positions, None, None, 0.0, False, *_config_values(config))
-    return (_binding or _bound()).rotary_embedding(q, k, positions, config._plan or _plan(config))
+    out = None
+    if not torch.compiler.is_compiling():
+        out = (_binding or _bound()).rotary_embedding(q, k, positions, config._plan or _plan(config))
+    if out is None:  # recorded: through the custom op
+        out = torch.ops.orda_b200.rotary(q, k, positions, None, None, 0.0, False, *_config_values(config))
+    return out
 
 
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -278,10 +286,13 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
     gradients are summed over tokens and heads in a fixed order.
     """
     _require_config("qk_norm_rotary", config)
-    if torch.compiler.is_compiling():
-        return torch.ops.orda_b200.rotary(q, k, positions, q_weight, k_weight, float(eps), False,
-                                          *_config_values(config))
-    return (_binding or _bound()).qk_norm_rotary(q, k, q_weight, k_weight, positions, config._plan or _plan(config), eps)
+    out = None
+    if not torch.compiler.is_compiling():
+        out = (_binding or _bound()).qk_norm_rotary(q, k, q_weight, k_weight, positions, config._plan or _plan(config), eps)
+    if out is None:  # recorded: through the custom op
+        out = torch.ops.orda_b200.rotary(q, k, positions, q_weight, k_weight, float(eps), False,
+                                         *_config_values(config))
+    return out
 
 
 # ------------------------------------------------------------------------------------------ gradient norm and clipping

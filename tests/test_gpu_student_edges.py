@@ -176,3 +176,54 @@ def test_c_glu_results_marked_by_a_timeout(n, h, cols, f):
         assert bool(torch.isnan(a[0, 0])) and bool(torch.isfinite(b).all())
         a[0, 0] = b[0, 0]
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------ recorders
+def _block(x, wg, wu, q, k, wq, wk, pos):
+    cfg = student.RotaryConfig(64)
+    a, b = student.qk_norm_rotary(q, k, wq, wk, pos, cfg)
+    return student.gated_linear_unit(x, wg, wu), *student.rotary_embedding(a, b, pos, cfg)
+
+
+def _block_inputs(seed):
+    x, wg, wu, _ = glu_inputs(40, 64, 72, BF16, seed)
+    q, k = randn(40, 2, 64, seed=seed + 4, dtype=BF16), randn(40, 1, 64, seed=seed + 5, dtype=BF16)
+    return x, wg, wu, q, k, randn(64, seed=seed + 6), randn(64, seed=seed + 7), torch.arange(40, device="cuda") + seed
+
+
+@pytest.mark.parametrize("how", ["make_fx", "jit"])
+def test_recorded_graphs_compute_from_their_inputs(how):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    first, second = _block_inputs(1), _block_inputs(50)
+    graph = make_fx(_block)(*first) if how == "make_fx" else torch.jit.trace(_block, first)
+    for ins in (first, second):
+        for a, b in zip(graph(*ins), _block(*ins)):
+            assert torch.equal(a, b)
+
+
+def test_calls_under_a_dispatch_mode_are_seen_and_differentiated():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    def run():
+        *leaves, pos = _block_inputs(7)
+        leaves = [t.requires_grad_(True) for t in leaves]
+        out = _block(*leaves, pos)
+        grads = torch.autograd.grad(sum(o.float().square().sum() for o in out), leaves)
+        clipped, norm = student.clip_gradients(grads, 1.0)
+        return [*out, *clipped, norm]
+
+    want = run()
+    assert not seen
+    with Watch():
+        got = run()
+    assert sum("orda_b200.glu" in s for s in seen) == 2 and sum("orda_b200.rotary" in s for s in seen) == 3
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

@@ -123,3 +123,42 @@ def test_inputs_that_carry_a_tangent_are_refused():
                      lambda: student.clip_grad_norm_([p], 1.0)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+def _graph_ops(graph):
+    return [str(n.target).split(".")[1] for n in graph.graph.nodes if "orda_b200" in str(n.target)]
+
+
+@pytest.mark.parametrize("pre_dispatch", [False, True])
+def test_recorded_calls_are_custom_ops_of_the_graph(pre_dispatch):
+    """make_fx sees what passes through the dispatcher only: a call around it would be a constant of the graph."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    with FakeTensorMode():
+        x, w = torch.empty(3, 16, device="cuda"), torch.empty(24, 16, device="cuda")
+        q, k, v = (torch.empty(*s, device="cuda") for s in ((3, 2, 8), (3, 1, 8), (8,)))
+        pos = torch.empty(3, device="cuda", dtype=torch.long)
+    cfg = student.RotaryConfig(8)
+
+    def step(x, w, q, k, v, pos):
+        q, k = student.qk_norm_rotary(q, k, v, v, pos, cfg)
+        return student.gated_linear_unit(x, w, w), *student.rotary_embedding(q, k, pos, cfg)
+
+    graph = make_fx(step, pre_dispatch=pre_dispatch)(x, w, q, k, v, pos)
+    assert _graph_ops(graph) == ["rotary", "glu_forward", "rotary"]
+    for call in (lambda x: student.grad_norm([x]), lambda x: student.clip_gradients([x], 1.0)):
+        with pytest.raises(RuntimeError, match="recorded into a graph"):
+            make_fx(call, pre_dispatch=pre_dispatch)(x)
+    with pytest.raises(RuntimeError, match="recorded into a graph"):
+        torch.jit.trace(lambda x: student.grad_norm([x]), (torch.ones(3),), check_trace=False)
+
+
+def test_recorded_calls_have_the_shapes_of_plain_ones():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x, w = (torch.empty(*s, device="cuda", dtype=torch.bfloat16) for s in ((2, 3, 16), (24, 16)))
+        assert student.gated_linear_unit(x, w, w).shape == (2, 3, 24)
+        with pytest.raises(ValueError, match="activation"):
+            student.gated_linear_unit(x, w, w, activation="tanh")
