@@ -31,6 +31,7 @@ Layout = Literal["half", "interleaved"]
 Scaling = Literal["none", "linear", "ntk", "yarn"]
 
 _LAYOUTS = ("half", "interleaved")
+_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 _binding = None
 
 
@@ -106,6 +107,9 @@ def gated_linear_unit(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: tor
     if h is None:  # recorded: through the custom op
         if activation not in _ACT_CODE:
             raise ValueError(f"activation must be one of {sorted(_ACT_CODE)}, got {activation!r}")
+        for t in (x, gate_weight, up_weight):
+            if t.dtype not in _DTYPES:
+                raise ValueError(f"gated_linear_unit: tensors must be float32, float16 or bfloat16, got {t.dtype}")
         dtype = default_compute_dtype(gate_weight, up_weight, x)
         h = torch.ops.orda_b200.glu_forward(x.to(dtype), gate_weight.to(dtype), up_weight.to(dtype),
                                             _ACT_CODE[activation])[0]

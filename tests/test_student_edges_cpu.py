@@ -160,5 +160,13 @@ def test_recorded_calls_have_the_shapes_of_plain_ones():
     with FakeTensorMode():
         x, w = (torch.empty(*s, device="cuda", dtype=torch.bfloat16) for s in ((2, 3, 16), (24, 16)))
         assert student.gated_linear_unit(x, w, w).shape == (2, 3, 24)
+        with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+            student.gated_linear_unit(x.double(), w.double(), w.double())
         with pytest.raises(ValueError, match="activation"):
             student.gated_linear_unit(x, w, w, activation="tanh")
+
+
+def test_compiled_block_refuses_types_as_the_plain_one_does():
+    x, w = torch.randn(4, 16, dtype=torch.float64), torch.randn(24, 16, dtype=torch.float64)
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        torch.compile(lambda x: student.gated_linear_unit(x, w, w), backend="eager")(x)
