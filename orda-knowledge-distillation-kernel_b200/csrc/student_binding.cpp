@@ -83,6 +83,12 @@ void refuse_tangent(const char* what, const Tensor& t) {
   TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivative, and an input carries a tangent");
 }
 
+// The tensor with its values in memory: not a view that stands for their negatives, nor a zero tensor without any.
+Tensor plain(const Tensor& t) {
+  if (t._is_zerotensor()) return t.clone();
+  return t.is_neg() ? t.resolve_neg() : t;
+}
+
 // A zeroed device word for the kernels' bounded waits.
 Tensor new_status(const Tensor& like, cudaStream_t s) {
   Tensor t = new_empty({1}, at::kInt, like);
@@ -256,7 +262,7 @@ std::pair<Tensor, Tensor> glu_backward(Tensor dh, const Tensor& x, const Tensor&
     if (dw.defined()) dw.zero_();
     return {dx, dw};
   }
-  dh = dh.contiguous();
+  dh = plain(dh).contiguous();
   a.pre_gate = pre.data_ptr();
   a.pre_up = static_cast<char*>(pre.data_ptr()) + a.rows * a.ld_pre * pre.element_size();
   a.dh = dh.data_ptr();
@@ -316,7 +322,7 @@ std::optional<Tensor> gated_linear_unit(const Tensor& x, const Tensor& gate_weig
   if (recorded()) return std::nullopt;
   check_glu(x, gate_weight, up_weight);
   const auto dt = compute_dtype({&gate_weight, &up_weight, &x});
-  auto cast = [dt](const Tensor& t) { return t.scalar_type() == dt ? t : t.to(dt); };
+  auto cast = [dt](const Tensor& t) { return plain(t.scalar_type() == dt ? t : t.to(dt)); };
   const Tensor flat = cast(x.dim() == 2 ? x : x.reshape({-1, x.size(-1)})), gate = cast(gate_weight), up = cast(up_weight);
   Tensor h;
   if (at::GradMode::is_enabled() && (flat.requires_grad() || gate.requires_grad() || up.requires_grad())) {
@@ -334,7 +340,7 @@ std::optional<Tensor> gated_linear_unit(const Tensor& x, const Tensor& gate_weig
 // Without autograd, for the custom ops: x any number of dimensions, all tensors in the compute dtype.
 std::tuple<Tensor, Tensor> glu_forward_op(const Tensor& x, const Tensor& gate, const Tensor& up, int64_t act) {
   check_glu(x, gate, up);
-  const GluOperands o(x.reshape({-1, x.size(-1)}), gate, up);
+  const GluOperands o(plain(x.reshape({-1, x.size(-1)})), plain(gate), plain(up));
   auto [h, pre] = glu_forward(o.t[0], o.t[1], o.t[2], act, true);
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end() - 1);
   shape.push_back(gate.size(0));
@@ -350,7 +356,7 @@ std::tuple<Tensor, Tensor, Tensor> glu_backward_op(const Tensor& dh, const Tenso
   dh_size.push_back(ffn);
   require_like("gated_linear_unit: the gradient", dh, dh_size, x);
   require_cuda("gated_linear_unit", x, {&gate, &up});
-  const GluOperands o(x.reshape({-1, hidden}), gate, up);
+  const GluOperands o(plain(x.reshape({-1, hidden})), plain(gate), plain(up));
   auto [dx, dw] = glu_backward(dh.reshape({-1, ffn}), o.t[0], o.t[1], o.t[2], pre, act, hidden, true, true);
   // an op's outputs share no storage
   return {dx.view(x.sizes()), dw.slice(0, 0, ffn).clone(), dw.slice(0, round8(ffn)).clone()};
@@ -405,7 +411,7 @@ void check_norm_weights(const char* what, const Tensor& wq, const Tensor& wk, co
   TORCH_CHECK_VALUE(eps >= 0.0, what, ": eps must be >= 0, got ", eps);
 }
 
-Tensor dense_last(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+Tensor dense_last(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? plain(t) : plain(t.contiguous()); }
 
 // Element strides of batch, sequence and heads; the stride of a dimension of one means nothing and counts as 0.
 void strides_of(const Tensor& t, int64_t (&out)[3]) {
@@ -532,27 +538,28 @@ struct QkNormRotaryFunction : torch::autograd::Function<QkNormRotaryFunction> {
 
 std::tuple<Tensor, Tensor> two(const variable_list& v) { return {v[0], v[1]}; }
 
-std::optional<std::tuple<Tensor, Tensor>> rotary_embedding(const Tensor& q_, const Tensor& k_, const Tensor& positions,
+std::optional<std::tuple<Tensor, Tensor>> rotary_embedding(const Tensor& q_, const Tensor& k_, const Tensor& positions_,
                                                            PlanPtr plan) {
-  check_qk("rotary_embedding", q_, k_, positions, *plan);
+  check_qk("rotary_embedding", q_, k_, positions_, *plan);
   for (const Tensor* t : {&q_, &k_}) refuse_tangent("rotary_embedding", *t);
   if (recorded()) return std::nullopt;
-  require_cuda("rotary_embedding", q_, {&k_, &positions});
-  const Tensor q = dense_last(q_), k = dense_last(k_);
+  require_cuda("rotary_embedding", q_, {&k_, &positions_});
+  const Tensor q = dense_last(q_), k = dense_last(k_), positions = plain(positions_);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad()))
     return two(RotaryFunction::apply(q, k, positions, plan));
   return two(rotate(q, k, positions, *plan, false, {}, {}, 0.0));
 }
 
 std::optional<std::tuple<Tensor, Tensor>> qk_norm_rotary(const Tensor& q_, const Tensor& k_, const Tensor& q_weight,
-                                                         const Tensor& k_weight, const Tensor& positions, PlanPtr plan,
+                                                         const Tensor& k_weight, const Tensor& positions_, PlanPtr plan,
                                                          double eps) {
-  check_qk("qk_norm_rotary", q_, k_, positions, *plan);
+  check_qk("qk_norm_rotary", q_, k_, positions_, *plan);
   check_norm_weights("qk_norm_rotary", q_weight, k_weight, *plan, eps);
   for (const Tensor* t : {&q_, &k_, &q_weight, &k_weight}) refuse_tangent("qk_norm_rotary", *t);
   if (recorded()) return std::nullopt;
-  require_cuda("qk_norm_rotary", q_, {&k_, &positions, &q_weight, &k_weight});
-  const Tensor q = dense_last(q_), k = dense_last(k_), wq = q_weight.contiguous(), wk = k_weight.contiguous();
+  require_cuda("qk_norm_rotary", q_, {&k_, &positions_, &q_weight, &k_weight});
+  const Tensor q = dense_last(q_), k = dense_last(k_), positions = plain(positions_), wq = plain(q_weight).contiguous(),
+               wk = plain(k_weight).contiguous();
   if (at::GradMode::is_enabled() &&
       (q.requires_grad() || k.requires_grad() || wq.requires_grad() || wk.requires_grad()))
     return two(QkNormRotaryFunction::apply(q, k, wq, wk, positions, plan, eps));
@@ -570,10 +577,10 @@ std::tuple<Tensor, Tensor> rotary_op(const Tensor& q, const Tensor& k, const Ten
   Tensor w[2];
   if (wq) {
     require_cuda("qk_norm_rotary", q, {&*wq, &*wk});
-    w[0] = wq->contiguous();
-    w[1] = wk->contiguous();
+    w[0] = plain(*wq).contiguous();
+    w[1] = plain(*wk).contiguous();
   }
-  auto r = rotate(dense_last(q), dense_last(k), positions, *plan, inverse, w[0], w[1], eps);
+  auto r = rotate(dense_last(q), dense_last(k), plain(positions), *plan, inverse, w[0], w[1], eps);
   return {r[0], r[1]};
 }
 
@@ -586,7 +593,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_backward_op(const Tens
   require_like("qk_norm_rotary: the gradient of the queries", dq, q.sizes(), q);
   require_like("qk_norm_rotary: the gradient of the keys", dk, k.sizes(), k);
   require_cuda("qk_norm_rotary", q, {&k, &positions, &wq, &wk});
-  auto r = norm_rotate_backward(dq, dk, dense_last(q), dense_last(k), wq.contiguous(), wk.contiguous(), positions, *plan,
+  auto r = norm_rotate_backward(dq, dk, dense_last(q), dense_last(k), plain(wq).contiguous(),
+                                plain(wk).contiguous(), plain(positions), *plan,
                                 eps);
   return {r[0], r[1], r[2], r[3]};
 }
@@ -639,7 +647,7 @@ void check_gradients(const char* what, const std::vector<Tensor>& grads, bool in
 }
 
 // A tensor whose values fill one gapless stretch of memory: itself, or a contiguous copy.
-Tensor dense(const Tensor& t) { return t.is_non_overlapping_and_dense() ? t : t.contiguous(); }
+Tensor dense(const Tensor& t) { return plain(t.is_non_overlapping_and_dense() ? t : t.contiguous()); }
 
 // Norm of `src` (0-dim fp32); `dst` (may be null) receives the clipped values. All dense, one device.
 Tensor clip_call(const std::vector<Tensor>& src, const std::vector<Tensor>* dst, double max_norm, double eps) {

@@ -227,3 +227,32 @@ def test_calls_under_a_dispatch_mode_are_seen_and_differentiated():
     assert sum("orda_b200.glu" in s for s in seen) == 2 and sum("orda_b200.rotary" in s for s in seen) == 3
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------ lazily negated and zero tensors
+def test_tensors_whose_values_are_not_in_memory_as_such():
+    """Views that stand for the negatives of what they point at (the imaginary part of a conjugate), and zero
+    tensors without memory, as inputs and as gradients."""
+    def neg(t):
+        return torch._neg_view((-t).clone())
+
+    x, wg, wu, q, k, wq, wk, pos = ins = _block_inputs(3)
+    want = _block(*ins)
+    for a, b in zip(_block(*(neg(t) for t in ins)), want):
+        assert torch.equal(a, b)
+    leaves = [t.detach().requires_grad_(True) for t in ins[:-1]]
+    dy = [randn(*o.shape, seed=9 + i, dtype=BF16) for i, o in enumerate(want)]
+    plain = torch.autograd.grad(_block(*leaves, pos), leaves, dy)
+    for a, b in zip(torch.autograd.grad(_block(*leaves, pos), leaves, [neg(d) for d in dy]), plain):
+        assert torch.equal(a, b)
+    part = torch.conj(torch.complex(q.float(), q.float())).imag[..., :1]  # dense: one element a head
+    assert part.is_neg()
+    for t in (part, neg(wg), x):
+        clipped, norm = student.clip_gradients([t], 1.0)
+        assert torch.equal(norm, student.grad_norm([t.clone()]))
+        assert torch.equal(clipped[0], student.clip_gradients([t.clone()], 1.0)[0][0])
+    g = neg(wg)
+    norm = student.clip_grad_norm_(_params(g), 1.0)
+    assert torch.equal(g.clone(), student.clip_gradients([wg], 1.0)[0][0])
+    zero = torch._efficientzerotensor((40, 64), device="cuda", dtype=BF16)
+    assert not student.gated_linear_unit(zero, wg, wu).any() and float(student.grad_norm([zero, wg])) == float(norm)
