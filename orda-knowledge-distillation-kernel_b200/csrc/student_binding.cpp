@@ -249,7 +249,7 @@ std::pair<Tensor, Tensor> glu_forward(const Tensor& x, const Tensor& gate, const
 // (dx, gradients of both weights), `hidden` columns each: the latter [ceil8(ffn) + ffn, hidden], gate's from
 // row 0, up's from row ceil8(ffn).
 std::pair<Tensor, Tensor> glu_backward(Tensor dh, const Tensor& x, const Tensor& gate, const Tensor& up,
-                                       const Tensor& pre, int64_t act, int64_t hidden, bool need_x, bool need_w) {
+                                       Tensor pre, int64_t act, int64_t hidden, bool need_x, bool need_w) {
   c10::cuda::CUDAGuard guard(x.device());
   cudaStream_t s = at::cuda::getCurrentCUDAStream().stream();
   orda_glu_args_t a = glu_args(x, gate, up, act);
@@ -263,6 +263,7 @@ std::pair<Tensor, Tensor> glu_backward(Tensor dh, const Tensor& x, const Tensor&
     return {dx, dw};
   }
   dh = plain(dh).contiguous();
+  pre = plain(pre).contiguous();
   a.pre_gate = pre.data_ptr();
   a.pre_up = static_cast<char*>(pre.data_ptr()) + a.rows * a.ld_pre * pre.element_size();
   a.dh = dh.data_ptr();
@@ -292,9 +293,15 @@ struct GluFunction : torch::autograd::Function<GluFunction> {
     variable_list grads(4);
     {
       at::AutoGradMode off(false);
-      auto [dx, dw] = glu_backward(dh[0], saved[0], saved[1], saved[2], saved[3], ctx->saved_data["act"].toInt(),
+      // what a saved-tensor hook returns may lie in memory in another way, and must be looked at again
+      check_glu(saved[0], saved[1], saved[2]);
+      const GluOperands o(plain(saved[0]), plain(saved[1]), plain(saved[2]));
+      const int64_t ffn = saved[1].size(0), pre_size[3] = {2, saved[0].size(0), round8(ffn)};
+      require_like("gated_linear_unit: the products of the forward pass", saved[3], pre_size, saved[0]);
+      const int64_t dh_size[2] = {saved[0].size(0), ffn};
+      require_like("gated_linear_unit: the gradient", dh[0], dh_size, saved[0]);
+      auto [dx, dw] = glu_backward(dh[0], o.t[0], o.t[1], o.t[2], saved[3], ctx->saved_data["act"].toInt(),
                                    ctx->saved_data["hidden"].toInt(), need_x, need_g || need_u);
-      const int64_t ffn = saved[1].size(0);
       grads[0] = dx;
       if (need_g) grads[1] = dw.slice(0, 0, ffn);
       if (need_u) grads[2] = dw.slice(0, round8(ffn));
@@ -493,6 +500,19 @@ variable_list norm_rotate_backward(const Tensor& dq, const Tensor& dk, const Ten
   return {gq, gk, gwq, gwk};
 }
 
+// The same of tensors that come from outside: a custom op's arguments, or what a saved-tensor hook returned.
+variable_list checked_norm_rotate_backward(const Tensor& dq, const Tensor& dk, const Tensor& q, const Tensor& k,
+                                           const Tensor& wq, const Tensor& wk, const Tensor& positions,
+                                           const RotaryPlan& plan, double eps) {
+  check_qk("qk_norm_rotary", q, k, positions, plan);
+  check_norm_weights("qk_norm_rotary", wq, wk, plan, eps);
+  require_like("qk_norm_rotary: the gradient of the queries", dq, q.sizes(), q);
+  require_like("qk_norm_rotary: the gradient of the keys", dk, k.sizes(), k);
+  require_cuda("qk_norm_rotary", q, {&k, &positions, &wq, &wk});
+  return norm_rotate_backward(dq, dk, dense_last(q), dense_last(k), plain(wq).contiguous(),
+                              plain(wk).contiguous(), plain(positions), plan, eps);
+}
+
 struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& positions,
                                PlanPtr plan) {
@@ -507,7 +527,9 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     variable_list g;
     {
       at::AutoGradMode off(false);
-      g = rotate(dense_last(dy[0]), dense_last(dy[1]), saved[0], *plan, true, {}, {}, 0.0);
+      check_qk("rotary_embedding", dy[0], dy[1], saved[0], *plan);
+      require_cuda("rotary_embedding", dy[0], {&dy[1], &saved[0]});
+      g = rotate(dense_last(dy[0]), dense_last(dy[1]), plain(saved[0]), *plan, true, {}, {}, 0.0);
     }
     g.resize(4);
     return differentiable_once(std::move(g));
@@ -529,7 +551,8 @@ struct QkNormRotaryFunction : torch::autograd::Function<QkNormRotaryFunction> {
     variable_list g;
     {
       at::AutoGradMode off(false);
-      g = norm_rotate_backward(dy[0], dy[1], s[0], s[1], s[2], s[3], s[4], *plan, ctx->saved_data["eps"].toDouble());
+      g = checked_norm_rotate_backward(dy[0], dy[1], s[0], s[1], s[2], s[3], s[4], *plan,
+                                       ctx->saved_data["eps"].toDouble());
     }
     g.resize(7);
     return differentiable_once(std::move(g));
@@ -588,14 +611,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_backward_op(const Tens
                                                                       const Tensor& q, const Tensor& k,
                                                                       const Tensor& positions, const Tensor& wq,
                                                                       const Tensor& wk, double eps, PlanPtr plan) {
-  check_qk("qk_norm_rotary", q, k, positions, *plan);
-  check_norm_weights("qk_norm_rotary", wq, wk, *plan, eps);
-  require_like("qk_norm_rotary: the gradient of the queries", dq, q.sizes(), q);
-  require_like("qk_norm_rotary: the gradient of the keys", dk, k.sizes(), k);
-  require_cuda("qk_norm_rotary", q, {&k, &positions, &wq, &wk});
-  auto r = norm_rotate_backward(dq, dk, dense_last(q), dense_last(k), plain(wq).contiguous(),
-                                plain(wk).contiguous(), plain(positions), *plan,
-                                eps);
+  const auto r = checked_norm_rotate_backward(dq, dk, q, k, wq, wk, positions, *plan, eps);
   return {r[0], r[1], r[2], r[3]};
 }
 

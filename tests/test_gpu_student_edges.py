@@ -256,3 +256,52 @@ def test_tensors_whose_values_are_not_in_memory_as_such():
     assert torch.equal(g.clone(), student.clip_gradients([wg], 1.0)[0][0])
     zero = torch._efficientzerotensor((40, 64), device="cuda", dtype=BF16)
     assert not student.gated_linear_unit(zero, wg, wu).any() and float(student.grad_norm([zero, wg])) == float(norm)
+
+
+# ------------------------------------------------------------------------------------------ saved-tensor hooks
+def _reversed_strides(t):
+    """The same values in memory in the opposite order of dimensions."""
+    dims = list(range(t.ndim))[::-1]
+    return t.permute(dims).contiguous().permute(dims)
+
+
+def _behind_a_boundary(t):
+    """The same values starting one element behind a 16-byte boundary."""
+    return torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+
+
+@pytest.mark.parametrize("unpack", [_reversed_strides, _behind_a_boundary, lambda t: t.cpu().cuda()])
+@pytest.mark.parametrize("n,h", [(40, 64), (300, 66)])
+def test_saved_tensors_that_come_back_with_other_strides(unpack, n, h):
+    x, wg, wu, dh = glu_inputs(n, h, 75, BF16, 71)
+    *_, q, k, wq, wk, pos = _block_inputs(5)
+    cfg = student.RotaryConfig(64, rotary_dim=32)
+    leaves = [t.detach().requires_grad_(True) for t in (x, wg, wu, q, k, wq, wk)]
+    dq, dk = randn(*q.shape, seed=6, dtype=BF16), randn(*k.shape, seed=7, dtype=BF16)
+
+    def run():
+        a, b = student.qk_norm_rotary(*leaves[3:], pos, cfg)
+        a, b = student.rotary_embedding(a, b, pos, cfg)
+        out = (student.gated_linear_unit(*leaves[:3]), a, b)
+        return torch.autograd.grad(out, leaves, (dh, dq, dk))
+
+    want = run()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        got = run()
+    for a, b in zip(got, want):
+        # weight gradients of the norms are added up in another order where heads are read in narrower vectors
+        torch.testing.assert_close(a, b, rtol=2 * half(b.dtype) if b.dtype != FP32 else 1e-5, atol=1e-5)
+
+
+def test_saved_tensors_that_come_back_as_others_are_refused():
+    x, wg, wu, dh = glu_inputs(40, 64, 72, BF16, 71)
+    *_, q, k, wq, wk, pos = _block_inputs(5)
+    for call, leaf in ((lambda t: student.gated_linear_unit(t, wg, wu), x),
+                       (lambda t: student.qk_norm_rotary(t, k, wq, wk, pos, student.RotaryConfig(64))[0], q),
+                       (lambda t: student.rotary_embedding(t, k, pos, student.RotaryConfig(64))[0], q)):
+        for unpack in (lambda t: t.cpu(), lambda t: t[1:], lambda t: t[..., :1]):
+            leaf = leaf.detach().requires_grad_(True)
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                y = call(leaf)
+            with pytest.raises((ValueError, RuntimeError)):
+                y.sum().backward()
