@@ -264,6 +264,7 @@ std::pair<Tensor, Tensor> glu_backward(Tensor dh, const Tensor& x, const Tensor&
   }
   dh = plain(dh).contiguous();
   pre = plain(pre).contiguous();
+  if (reinterpret_cast<uintptr_t>(pre.data_ptr()) % 16) pre = pre.clone();
   a.pre_gate = pre.data_ptr();
   a.pre_up = static_cast<char*>(pre.data_ptr()) + a.rows * a.ld_pre * pre.element_size();
   a.dh = dh.data_ptr();
