@@ -305,3 +305,24 @@ def test_saved_tensors_that_come_back_as_others_are_refused():
                 y = call(leaf)
             with pytest.raises((ValueError, RuntimeError)):
                 y.sum().backward()
+
+
+# ------------------------------------------------------------------------------------------ large finite values
+@pytest.mark.parametrize("n", [5, 40, 300])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("act", ACTS)
+def test_glu_gates_whose_square_is_infinite(act, dtype, n):
+    """Gates of +-1.6e21: activations and derivatives are at their limits (g and 1, or 0), and finite."""
+    x = torch.full((n, 16), 1e10, device="cuda", dtype=dtype)
+    wg = torch.full((24, 16), 1e10, device="cuda", dtype=dtype)
+    wg[::2] *= -1
+    wu, dh = torch.full_like(wg, 1e-10), torch.full((n, 24), 1e-20, device="cuda", dtype=dtype)
+    got = glu_pass(x, wg, wu, act, dh)
+    x, wg, wu, dh = (t.double() for t in (x, wg, wu, dh))
+    g, u = x @ wg.T, x @ wu.T
+    a, d = g.relu(), (g > 0).double()
+    dg, du = dh * u * d, dh * a
+    # nothing cancels: the products, dg and du, and the result are each rounded once, sums lose 2^-23 a step
+    rel = 3.5 * half(dtype) + (16 + n + 48) * 2.0 ** -23
+    for name, y, want in zip(("h", "dx", "dgate", "dup"), got, (a * u, dg @ wg + du @ wu, dg.T @ x, du.T @ x)):
+        within(y, want, rel * want.abs(), name)
