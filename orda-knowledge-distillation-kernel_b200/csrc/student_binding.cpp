@@ -89,6 +89,14 @@ Tensor plain(const Tensor& t) {
   return t.is_neg() ? t.resolve_neg() : t;
 }
 
+// A tensor in the memory of `whole` that is no view of it: writes to one part do not count as writes to another.
+Tensor part_of(const Tensor& whole, at::IntArrayRef size, at::IntArrayRef stride, int64_t offset, caffe2::TypeMeta dtype) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()),
+                                                      c10::DispatchKeySet(c10::DispatchKey::CUDA), dtype);
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(size, stride, offset);
+  return t;
+}
+
 // A zeroed device word for the kernels' bounded waits.
 Tensor new_status(const Tensor& like, cudaStream_t s) {
   Tensor t = new_empty({1}, at::kInt, like);
@@ -304,8 +312,9 @@ struct GluFunction : torch::autograd::Function<GluFunction> {
       auto [dx, dw] = glu_backward(dh[0], o.t[0], o.t[1], o.t[2], saved[3], ctx->saved_data["act"].toInt(),
                                    ctx->saved_data["hidden"].toInt(), need_x, need_g || need_u);
       grads[0] = dx;
-      if (need_g) grads[1] = dw.slice(0, 0, ffn);
-      if (need_u) grads[2] = dw.slice(0, round8(ffn));
+      const int64_t size[2] = {ffn, ctx->saved_data["hidden"].toInt()}, stride[2] = {size[1], 1};
+      if (need_g) grads[1] = part_of(dw, size, stride, 0, dw.dtype());
+      if (need_u) grads[2] = part_of(dw, size, stride, round8(ffn) * size[1], dw.dtype());
     }
     return differentiable_once(std::move(grads));
   }
@@ -721,10 +730,7 @@ std::tuple<std::vector<Tensor>, Tensor> clip_gradients(const std::vector<Tensor>
     const Tensor all = new_empty({bytes}, at::kByte, grads[0]);
     int64_t at = 0;
     for (const Tensor& d : src) {
-      Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()),
-                                                          c10::DispatchKeySet(c10::DispatchKey::CUDA), d.dtype());
-      t.unsafeGetTensorImpl()->set_sizes_and_strides(d.sizes(), d.strides(), at / d.element_size());
-      out.push_back(std::move(t));
+      out.push_back(part_of(all, d.sizes(), d.strides(), at / d.element_size(), d.dtype()));
       at += (d.nbytes() + 255) / 256 * 256;
     }
   } else {

@@ -326,3 +326,19 @@ def test_glu_gates_whose_square_is_infinite(act, dtype, n):
     rel = 3.5 * half(dtype) + (16 + n + 48) * 2.0 ** -23
     for name, y, want in zip(("h", "dx", "dgate", "dup"), got, (a * u, dg @ wg + du @ wu, dg.T @ x, du.T @ x)):
         within(y, want, rel * want.abs(), name)
+
+
+# ------------------------------------------------------------------------------------------ results in one allocation
+def test_writes_to_one_result_are_none_to_another():
+    """The two weights' gradients, and the results of clip_gradients, share an allocation."""
+    x, wg, wu, dh = glu_inputs(40, 64, 75, BF16, 81)
+    gate, up = (t.detach().requires_grad_(True) for t in (wg, wu))
+    student.gated_linear_unit(x, gate, up).backward(dh)
+    clipped, _ = student.clip_gradients([gate.grad, up.grad], 1e9)
+    for a, b in ((gate.grad, up.grad), clipped):
+        kept = b.clone()
+        p = torch.ones_like(b).requires_grad_(True)
+        y = (p * b).sum()  # saves b
+        a.add_(1)
+        y.backward()
+        assert torch.equal(p.grad, kept) and torch.equal(b, kept) and b._version == 0
