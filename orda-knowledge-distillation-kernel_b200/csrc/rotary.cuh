@@ -9,9 +9,10 @@
 //
 // Angles: theta_i / 2 pi is held as a 64-bit fraction of a turn, and the low 64 bits of its product with
 // the position are the angle modulo one turn, off by |p| 2^-65 turns plus the rounding of theta_i. The
-// top 32 of them go to fp32, so the angle is off by less than 2e-7 rad at any position below 2^31 (a
-// 32-bit float product is already off by 0.06 rad at position 1e6). No table and no fp64 arithmetic: a
-// warp computes a token's angles once for the heads that it turns.
+// top 32 of them go to fp32, so the angle is off by less than 1e-7 rad at any position below 2^31 (a
+// 32-bit float product is already off by 0.06 rad at position 1e6); for fp32 tensors, where a sine near zero
+// would show it, cosine and sine are corrected by the rest. No table and no fp64 arithmetic: a warp computes a
+// token's angles once for the heads that it turns.
 //
 // What bounds it: memory, and close behind it the issue of instructions (61-67% of the slots). Each head's
 // values are read and written once in 16-byte vectors, a token's angles are formed once. In bf16: 32768 tokens
@@ -319,15 +320,24 @@ struct TokenAngles {
   float cos[kRotMaxPairs], sin[kRotMaxPairs], neg_sin[kRotMaxPairs];
 };
 
-// `turns`: the block's copy of p.turns (lanes that read different constants wait for one another).
-template <int V, bool IL>
+// `turns`: the block's copy of p.turns (lanes that read different constants wait for one another). FINE (32-bit
+// tensors): the part of the angle that its rounding to fp32 lost, at most 1e-7, turns cosine and sine once more, to first order.
+template <int V, bool IL, bool FINE>
 __device__ __forceinline__ void token_angles(const RotaryParams& p, const uint64_t* turns, int64_t position, int lane,
                                              TokenAngles& out) {
   for (int i = lane; i < p.rotary_dim / 2; i += 32) {
     const uint64_t turn = static_cast<uint64_t>(position) * turns[i];
     float s, c;
     // the top 32 bits as a signed number: units of 2^-31 half turns
-    sincospif(static_cast<float>(static_cast<int32_t>(turn >> 32)) * 4.656612873077393e-10f, &s, &c);
+    const float top = static_cast<float>(static_cast<int32_t>(turn >> 32));
+    sincospif(top * 4.656612873077393e-10f, &s, &c);
+    if constexpr (FINE) {
+      const uint64_t rest = turn - (static_cast<uint64_t>(static_cast<int64_t>(top)) << 32);  // (modulo a turn)
+      const float angle = static_cast<float>(static_cast<int64_t>(rest)) * 3.4061215800865545e-19f;  // 2 pi / 2^64
+      const float fine = fmaf(angle, c, s);
+      c = fmaf(-angle, s, c);
+      s = fine;
+    }
     s *= p.magnitude * p.sin_sign;
     const int at = pair_at<V, IL>(p, i);
     out.cos[at] = p.magnitude * c;
@@ -549,7 +559,7 @@ __global__ void __launch_bounds__(32 * kRotWarps, 5) rotary_forward_kernel(const
       oq = static_cast<T*>(p.out[0]) + at.b * p.os[0][0] + at.t * p.os[0][1];
       ok = static_cast<T*>(p.out[1]) + at.b * p.os[1][0] + at.t * p.os[1][1];
       __syncwarp();  // the previous unit's angles have been read
-      token_angles<V, IL>(p, turns, position, lane, angles);
+      token_angles<V, IL, sizeof(T) == 4>(p, turns, position, lane, angles);
 #pragma unroll
       for (int n = 0; n < NS; ++n)
         if (slot[n].turned) sa[n].load(p, angles, sl + n * p.lanes);
@@ -694,7 +704,7 @@ __global__ void __launch_bounds__(32 * kRotWarps, 4)
         if (fresh) {
           out_token = static_cast<T*>(p.out[which]) + at.b * p.os[which][0] + at.t * p.os[which][1];
           __syncwarp();  // the previous unit's angles have been read
-          token_angles<V, IL>(p, turns, position, lane, angles);
+          token_angles<V, IL, sizeof(T) == 4>(p, turns, position, lane, angles);
           if (at.unit + stride < total) position = unit_position(p, p.units[which], at.unit + stride);
         }
         Ring::wait();

@@ -342,3 +342,24 @@ def test_writes_to_one_result_are_none_to_another():
         a.add_(1)
         y.backward()
         assert torch.equal(p.grad, kept) and torch.equal(b, kept) and b._version == 0
+
+
+# ------------------------------------------------------------------------------------------ angles of fp32 tensors
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,head", [(2, 3), (16, 16), (128, 128)])
+def test_rotary_fp32_keeps_small_sines(dim, head, layout):
+    """Positions whose angles lie close to multiples of pi / 2 (355, 710, 103993, ... for one radian a position):
+    cosines and sines near zero are as exact, relatively, as others."""
+    cfg = student.RotaryConfig(head, rotary_dim=dim, layout=layout)
+    pos = torch.tensor([0, 1, 11, 22, 44, 355, 710, 1065, -355, 103993, 104348, 833719, 1000003], device="cuda")
+    q = randn(13, 4, head, seed=1)
+    got = student.rotary_embedding(q, q[:, :1], pos, cfg)[0].double()
+    angle = pos.double()[:, None, None] * torch.tensor(cfg.frequencies(), dtype=torch.float64, device="cuda")
+    ia, ib = ((slice(0, dim // 2), slice(dim // 2, dim)) if layout == "half" else (slice(0, dim, 2), slice(1, dim, 2)))
+    a, b, cos, sin = q.double()[..., ia], q.double()[..., ib], angle.cos(), angle.sin()
+    # cosine and sine: one unit in the last place, and half of one for the correction; one product is rounded. The
+    # frequencies' own rounding and the correction's second order: |p| 2^-52 and 1e-14
+    rel, off = 1.5 * 2.0 ** -23 + 2.0 ** -24, pos.double().abs()[:, None, None] * 2.0 ** -52 + 1e-14
+    for at, u, v in ((ia, a * cos, -b * sin), (ib, b * cos, a * sin)):
+        tol = half(FP32) * (u + v).abs() + rel * (u.abs() + v.abs()) + off * (a.abs() + b.abs())
+        assert bool(((got[..., at] - (u + v)).abs() <= tol).all())
