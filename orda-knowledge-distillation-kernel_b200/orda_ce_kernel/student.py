@@ -29,6 +29,7 @@ from ._runtime import default_compute_dtype
 Activation = Literal["silu", "gelu", "gelu_tanh", "relu"]
 Layout = Literal["half", "interleaved"]
 Scaling = Literal["none", "linear", "ntk", "yarn"]
+Ramp = Literal["turns", "index"]
 
 _LAYOUTS = ("half", "interleaved")
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -126,8 +127,13 @@ class RotaryConfig:
     * ``scaling`` - contexts ``factor`` times as long: ``"linear"`` divides every angle by ``factor``;
       ``"ntk"`` raises ``base`` to ``base * factor^(d / (d - 2))``; ``"yarn"`` divides the angles of pairs
       that turn less than ``beta_slow`` times within ``original_positions``, keeps those that turn more than
-      ``beta_fast`` times, blends in between, and multiplies the rotated values by
+      ``beta_fast`` times, blends in between (``ramp``), and multiplies the rotated values by
       ``0.1 ln(factor) + 1`` (or ``magnitude``).
+    * ``ramp`` - the part of a pair's own angle in YaRN's blend. ``"turns"``: linear in its turns within
+      ``original_positions``, 0 at ``beta_slow`` and 1 at ``beta_fast``, as the paper has it. ``"index"``: linear
+      in the pair's index ``i``, 1 up to the last pair that turns ``beta_fast`` times and 0 from the first that
+      turns ``beta_slow`` times or less, as published checkpoints mostly have it. The two differ by up to 57% in a
+      pair's angle (128 elements, factor 8), so a checkpoint needs the one it was trained with.
     """
 
     head_dim: int
@@ -140,6 +146,7 @@ class RotaryConfig:
     beta_fast: float = 32.0
     beta_slow: float = 1.0
     magnitude: float | None = None
+    ramp: Ramp = "turns"
 
     def __post_init__(self):
         if not 1 <= self.head_dim <= _native.ROTARY_MAX_DIM:
@@ -159,6 +166,10 @@ class RotaryConfig:
             raise ValueError("scaling='ntk' needs rotary_dim > 2")
         if self.scaling == "yarn" and not (self.beta_fast > self.beta_slow and self.original_positions > 0):
             raise ValueError("scaling='yarn' needs beta_fast > beta_slow and original_positions > 0")
+        if self.ramp not in ("turns", "index"):
+            raise ValueError(f"ramp must be 'turns' or 'index', got {self.ramp!r}")
+        if self.scaling == "yarn" and self.ramp == "index" and not (self.base > 1.0 and self.beta_slow > 0.0):
+            raise ValueError("scaling='yarn' with ramp='index' needs base > 1 and beta_slow > 0")
         object.__setattr__(self, "_plan", None)
 
     @property
@@ -174,13 +185,29 @@ class RotaryConfig:
         if self.scaling == "linear":
             return [t / self.factor for t in theta]
         if self.scaling == "yarn":
-            out = []
-            for t in theta:
-                turns = self.original_positions * t / (2.0 * math.pi)
-                keep = min(1.0, max(0.0, (turns - self.beta_slow) / (self.beta_fast - self.beta_slow)))
-                out.append(t / self.factor * (1.0 - keep) + t * keep)
-            return out
+            return [t / self.factor * (1.0 - keep) + t * keep for t, keep in zip(theta, self._kept(theta))]
         return theta
+
+    def _kept(self, theta: list[float]) -> list[float]:
+        """YaRN: the part of each pair's own angle in the blend."""
+        if self.ramp == "turns":
+            def at(i):
+                return self.original_positions * theta[i] / (2.0 * math.pi)
+
+            slow, fast = self.beta_slow, self.beta_fast
+        else:
+            def index(turns):  # of the pair that turns so often; not a whole number
+                return self.dim * math.log(self.original_positions / (2.0 * math.pi * turns)) / (2.0 * math.log(self.base))
+
+            def at(i):
+                return i
+
+            fast, slow = max(0, math.floor(index(self.beta_fast))), min(self.dim - 1, math.ceil(index(self.beta_slow)))
+            if slow <= 0:  # no pair turns that often
+                return [0.0] * len(theta)
+            if slow <= fast:
+                slow = fast + 0.001  # a step
+        return [min(1.0, max(0.0, (at(i) - slow) / (fast - slow))) for i in range(len(theta))]
 
     @property
     def value_scale(self) -> float:
@@ -204,43 +231,44 @@ def _plan(config: RotaryConfig):
 # The custom ops take the configuration as plain values.
 def _config_values(c: RotaryConfig):
     return [c.head_dim, c.dim, c.original_positions], [c.base, c.factor, c.beta_fast, c.beta_slow, c.value_scale], \
-        c.layout, c.scaling
+        c.layout, c.scaling, c.ramp
 
 
-def _config_from(ints, floats, layout, scaling) -> RotaryConfig:
-    return RotaryConfig(ints[0], ints[1], floats[0], layout, scaling, floats[1], ints[2], floats[2], floats[3], floats[4])
+def _config_from(ints, floats, layout, scaling, ramp) -> RotaryConfig:
+    return RotaryConfig(ints[0], ints[1], floats[0], layout, scaling, floats[1], ints[2], floats[2], floats[3], floats[4],
+                        ramp)
 
 
 @torch.library.custom_op("orda_b200::rotary", mutates_args=())
 def _rotary_op(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, q_weight: Optional[torch.Tensor],
                k_weight: Optional[torch.Tensor], eps: float, inverse: bool, ints: list[int], floats: list[float],
-               layout: str, scaling: str) -> tuple[torch.Tensor, torch.Tensor]:
-    plan = _plan(_config_from(ints, floats, layout, scaling))
+               layout: str, scaling: str, ramp: str) -> tuple[torch.Tensor, torch.Tensor]:
+    plan = _plan(_config_from(ints, floats, layout, scaling, ramp))
     return _bound().rotary(q, k, positions, q_weight, k_weight, eps, inverse, plan)
 
 
 @_rotary_op.register_fake
-def _(q, k, positions, q_weight, k_weight, eps, inverse, ints, floats, layout, scaling):
+def _(q, k, positions, q_weight, k_weight, eps, inverse, ints, floats, layout, scaling, ramp):
     return q.new_empty(q.shape), k.new_empty(k.shape)
 
 
 @torch.library.custom_op("orda_b200::qk_norm_rotary_backward", mutates_args=())
 def _qk_norm_rotary_backward_op(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
                                 positions: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
-                                ints: list[int], floats: list[float], layout: str,
-                                scaling: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    plan = _plan(_config_from(ints, floats, layout, scaling))
+                                ints: list[int], floats: list[float], layout: str, scaling: str,
+                                ramp: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    plan = _plan(_config_from(ints, floats, layout, scaling, ramp))
     return _bound().qk_norm_rotary_backward(dq, dk, q, k, positions, q_weight, k_weight, eps, plan)
 
 
 @_qk_norm_rotary_backward_op.register_fake
-def _(dq, dk, q, k, positions, q_weight, k_weight, eps, ints, floats, layout, scaling):
+def _(dq, dk, q, k, positions, q_weight, k_weight, eps, ints, floats, layout, scaling, ramp):
     return q.new_empty(q.shape), k.new_empty(k.shape), q_weight.new_empty(q_weight.shape), k_weight.new_empty(k_weight.shape)
 
 
 def _rotary_setup(ctx, inputs, output):
-    q, k, positions, q_weight, k_weight, eps, inverse, ints, floats, layout, scaling = inputs
-    ctx.normed, ctx.eps, ctx.inverse, ctx.config = q_weight is not None, eps, inverse, (ints, floats, layout, scaling)
+    q, k, positions, q_weight, k_weight, eps, inverse, *config = inputs
+    ctx.normed, ctx.eps, ctx.inverse, ctx.config = q_weight is not None, eps, inverse, config
     ctx.save_for_backward(positions, *((q, k, q_weight, k_weight) if ctx.normed else ()))
 
 
@@ -249,9 +277,9 @@ def _rotary_op_backward(ctx, dq, dk):
         positions, q, k, q_weight, k_weight = ctx.saved_tensors
         gq, gk, gwq, gwk = torch.ops.orda_b200.qk_norm_rotary_backward(dq, dk, q, k, positions, q_weight, k_weight,
                                                                        ctx.eps, *ctx.config)
-        return (gq, gk, None, gwq, gwk, *([None] * 6))
+        return (gq, gk, None, gwq, gwk, *([None] * 7))
     gq, gk = torch.ops.orda_b200.rotary(dq, dk, ctx.saved_tensors[0], None, None, 0.0, not ctx.inverse, *ctx.config)
-    return (gq, gk, *([None] * 9))
+    return (gq, gk, *([None] * 10))
 
 
 _rotary_op.register_autograd(_rotary_op_backward, setup_context=_rotary_setup)

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from orda_ce_kernel import _native, student
-from test_gpu_student import BF16, FP16, FP32, glu64, glu_inputs, half, randn, within
+from test_gpu_student import BF16, FP16, FP32, check_rotary, glu64, glu_inputs, half, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -363,3 +363,21 @@ def test_rotary_fp32_keeps_small_sines(dim, head, layout):
     for at, u, v in ((ia, a * cos, -b * sin), (ib, b * cos, a * sin)):
         tol = half(FP32) * (u + v).abs() + rel * (u.abs() + v.abs()) + off * (a.abs() + b.abs())
         assert bool(((got[..., at] - (u + v)).abs() <= tol).all())
+
+
+def test_ramp_in_the_pair_index_eager_and_compiled():
+    cfg = student.RotaryConfig(64, scaling="yarn", factor=8.0, ramp="index")
+    q, k = randn(9, 4, 64, seed=1, dtype=BF16), randn(9, 2, 64, seed=2, dtype=BF16)
+    pos = torch.arange(9, device="cuda") * 1000
+    check_rotary(q, k, pos, cfg)
+    fn = lambda q, k: student.rotary_embedding(q, k, pos, cfg)  # noqa: E731
+    dy = [randn(*t.shape, seed=3, dtype=BF16) for t in (q, k)]
+    results = []
+    for f in (fn, torch.compile(fn, fullgraph=True)):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k)]
+        out = f(*leaves)
+        results.append([*out, *torch.autograd.grad(out, leaves, dy)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    other = student.rotary_embedding(q, k, pos, student.RotaryConfig(64, scaling="yarn", factor=8.0))
+    assert not torch.equal(results[0][0], other[0])

@@ -170,3 +170,42 @@ def test_compiled_block_refuses_types_as_the_plain_one_does():
     x, w = torch.randn(4, 16, dtype=torch.float64), torch.randn(24, 16, dtype=torch.float64)
     with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
         torch.compile(lambda x: student.gated_linear_unit(x, w, w), backend="eager")(x)
+
+
+# ------------------------------------------------------------------------------------------ YaRN's two ramps
+def _yarn(**kw):
+    return student.RotaryConfig(128, scaling="yarn", factor=8.0, original_positions=4096, **kw).frequencies()
+
+
+def test_yarn_ramp_in_the_pair_index():
+    """128 elements, base 10^4, 4096 positions: a pair turns 4096 / (2 pi) 10^(-i / 16) times, 32 times at
+    i = 20.9 and once at i = 45.0; the ramp runs from pair 20 to pair 46."""
+    own = student.RotaryConfig(128).frequencies()
+    got = _yarn(ramp="index")
+    for i, (f, y) in enumerate(zip(own, got)):
+        keep = min(1.0, max(0.0, 1.0 - (i - 20) / 26))
+        assert y == pytest.approx(f * (keep + (1.0 - keep) / 8), rel=1e-14), i
+    assert got[33] == pytest.approx(own[33] * 9 / 16, rel=1e-14)
+    turns = _yarn()  # the default: linear in a pair's turns
+    assert turns == _yarn(ramp="turns")
+    assert min(t / y for t, y in zip(turns, got)) == pytest.approx(0.434, abs=1e-3)
+    t33 = 4096 * own[33] / 6.283185307179586
+    assert turns[33] == pytest.approx(own[33] * (1 / 8 + 7 / 8 * (t33 - 1) / 31), rel=1e-12)
+
+
+def test_yarn_ramp_at_its_ends():
+    many = student.RotaryConfig(16, scaling="yarn", factor=4.0, original_positions=10 ** 9, ramp="index")
+    assert many.frequencies() == student.RotaryConfig(16).frequencies()  # every pair turns often
+    few = student.RotaryConfig(16, scaling="yarn", factor=4.0, original_positions=2, ramp="index")
+    assert few.frequencies() == pytest.approx([f / 4 for f in student.RotaryConfig(16).frequencies()])
+    with pytest.raises(ValueError, match="ramp"):
+        student.RotaryConfig(16, ramp="pairs")
+    for kw in (dict(base=1.0), dict(base=0.5), dict(beta_slow=0.0)):
+        with pytest.raises(ValueError, match="ramp='index'"):
+            student.RotaryConfig(16, scaling="yarn", factor=4.0, ramp="index", **kw)
+
+
+def test_ramp_reaches_the_custom_op():
+    c = student.RotaryConfig(64, scaling="yarn", factor=8.0, ramp="index")
+    assert student._config_from(*student._config_values(c)) == student.RotaryConfig(
+        64, 64, scaling="yarn", factor=8.0, ramp="index", magnitude=c.value_scale)
