@@ -76,7 +76,7 @@ class Attention(nn.Module):
         self.qkv = nn.Linear(d, (q_heads + 2 * kv_heads) * self.dh, bias=False)
         self.proj = nn.Linear(d, d, bias=False)
         self.q_norm, self.k_norm = (RMSNorm(self.dh), RMSNorm(self.dh)) if qk_norm else (None, None)
-        self.rotary = RotaryConfig(self.dh)
+        self.rotary = RotaryConfig(self.dh) if ops else None
         self.register_buffer("positions", torch.arange(seq), persistent=False)
         cos, sin = rotary_tables(self.dh, seq)
         self.register_buffer("cos", cos, persistent=False)

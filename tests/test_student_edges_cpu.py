@@ -209,3 +209,14 @@ def test_ramp_reaches_the_custom_op():
     c = student.RotaryConfig(64, scaling="yarn", factor=8.0, ramp="index")
     assert student._config_from(*student._config_values(c)) == student.RotaryConfig(
         64, 64, scaling="yarn", factor=8.0, ramp="index", magnitude=c.value_scale)
+
+
+# ------------------------------------------------------------------------------------------ the training benchmark's model
+def test_benchmark_model_without_operators_takes_heads_that_they_refuse():
+    from orda_ce_kernel.benchmarks import train_step
+
+    cfg = dict(dim=520, q_heads=1, kv_heads=1, n_layers=1, ffn_dim=16)  # heads of more than 512 elements
+    ids = torch.randint(0, 11, (1, 3))
+    assert train_step.TinyLM(11, cfg, 4).hidden(ids).shape == (1, 3, 520)
+    with pytest.raises(ValueError, match="head_dim"):
+        train_step.TinyLM(11, cfg, 4, ops=True)
