@@ -3,13 +3,15 @@
     python orda-knowledge-distillation-kernel_b200/build.py [--force]
 
 and ``orda_ce_kernel/_student.so``, the Python binding of the student-step operators, with g++ against the
-installed torch.
+installed torch (where there is none, the library alone, which C programs link to).
 
-Rebuilds only when a source under csrc/ or include/ is newer than a library.
+Rebuilds only when a source under csrc/ or include/ is newer than a library; ``--force`` for a binding that was
+built against another torch.
 """
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -45,10 +47,15 @@ def sources() -> list[str]:
                   + glob.glob(os.path.join(CSRC, "*.cpp")) + glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
+def has_torch() -> bool:
+    return importlib.util.find_spec("torch") is not None
+
+
 def needs_build() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(BINDING):
+    outputs = [LIB, BINDING] if has_torch() else [LIB]
+    if not all(os.path.exists(o) for o in outputs):
         return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(BINDING))
+    t = min(os.path.getmtime(o) for o in outputs)
     return any(os.path.getmtime(s) > t for s in sources())
 
 
@@ -73,6 +80,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB
     nvcc = _nvcc()
+    flags = _binding_flags() if has_torch() else None
     with tempfile.TemporaryDirectory(dir=os.path.dirname(LIB)) as tmp:
         # the translation units compile side by side
         objects, running = [], []
@@ -82,21 +90,23 @@ def build(force: bool = False, verbose: bool = False) -> str:
             if verbose:
                 print(" ".join(cmd))
             running.append((cmd, subprocess.Popen(cmd)))
-        compile_flags, link_flags = _binding_flags()
-        binding_object = os.path.join(tmp, "student_binding.o")
-        cmd = ["g++", *compile_flags, "-c", os.path.join(CSRC, "student_binding.cpp"), "-o", binding_object]
-        if verbose:
-            print(" ".join(cmd))
-        running.append((cmd, subprocess.Popen(cmd)))
+        if flags:
+            binding_object = os.path.join(tmp, "student_binding.o")
+            cmd = ["g++", *flags[0], "-c", os.path.join(CSRC, "student_binding.cpp"), "-o", binding_object]
+            if verbose:
+                print(" ".join(cmd))
+            running.append((cmd, subprocess.Popen(cmd)))
         failed = [cmd for cmd, p in running if p.wait() != 0]
         if failed:
             raise subprocess.CalledProcessError(1, failed[0])
         lib = os.path.join(tmp, LIB_NAME)
         subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", lib, *objects], check=True)
         binding = os.path.join(tmp, "_student.so")
-        subprocess.run(["g++", "-shared", "-o", binding, binding_object, "-L", tmp, *link_flags], check=True)
+        if flags:
+            subprocess.run(["g++", "-shared", "-o", binding, binding_object, "-L", tmp, *flags[1]], check=True)
         os.replace(lib, LIB)
-        os.replace(binding, BINDING)
+        if flags:
+            os.replace(binding, BINDING)
     return LIB
 
 

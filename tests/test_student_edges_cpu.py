@@ -220,3 +220,48 @@ def test_benchmark_model_without_operators_takes_heads_that_they_refuse():
     assert train_step.TinyLM(11, cfg, 4).hidden(ids).shape == (1, 3, 520)
     with pytest.raises(ValueError, match="head_dim"):
         train_step.TinyLM(11, cfg, 4, ops=True)
+
+
+# ------------------------------------------------------------------------------------------ build
+def _build_module():
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                        "orda-knowledge-distillation-kernel_b200", "build.py")
+    spec = importlib.util.spec_from_file_location("orda_build", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+@pytest.mark.parametrize("torch_installed", [True, False])
+def test_the_library_builds_without_torch(torch_installed, tmp_path, monkeypatch):
+    """The commands of a build, recorded instead of run: the binding is compiled where torch is installed only."""
+    import os
+
+    b, commands = _build_module(), []
+
+    def run(cmd, check=False):
+        commands.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+
+    class Popen:
+        def __init__(self, cmd):
+            run(cmd)
+
+        def wait(self):
+            return 0
+
+    monkeypatch.setattr(b, "has_torch", lambda: torch_installed)
+    monkeypatch.setattr(b, "_nvcc", lambda: "nvcc")
+    monkeypatch.setattr(b, "_binding_flags", lambda: (["-O2"], ["-ltorch"]))
+    monkeypatch.setattr(b, "LIB", str(tmp_path / b.LIB_NAME))
+    monkeypatch.setattr(b, "BINDING", str(tmp_path / "_student.so"))
+    monkeypatch.setattr(b.subprocess, "run", run)
+    monkeypatch.setattr(b.subprocess, "Popen", Popen)
+    assert b.needs_build()
+    b.build()
+    assert not b.needs_build()
+    assert sorted(os.listdir(tmp_path)) == (["_student.so"] if torch_installed else []) + [b.LIB_NAME]
+    assert any(c[0] == "g++" for c in commands) == torch_installed
