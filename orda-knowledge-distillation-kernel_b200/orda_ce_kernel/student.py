@@ -45,7 +45,7 @@ def _bound():
             from . import _student
         except ImportError as exc:
             raise RuntimeError("orda_ce_kernel/_student.so is not built for this torch (run "
-                               f"orda-knowledge-distillation-kernel_b200/build.py): {exc}") from exc
+                               f"orda-knowledge-distillation-kernel_b200/build.py --force): {exc}") from exc
         _binding = _student
     return _binding
 

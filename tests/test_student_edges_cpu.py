@@ -265,3 +265,13 @@ def test_the_library_builds_without_torch(torch_installed, tmp_path, monkeypatch
     assert not b.needs_build()
     assert sorted(os.listdir(tmp_path)) == (["_student.so"] if torch_installed else []) + [b.LIB_NAME]
     assert any(c[0] == "g++" for c in commands) == torch_installed
+
+
+def test_a_binding_that_does_not_load_names_a_command_that_rebuilds_it(monkeypatch):
+    import sys
+
+    monkeypatch.setattr(student, "_binding", None)
+    monkeypatch.setitem(sys.modules, "orda_ce_kernel._student", None)  # an import of it fails
+    monkeypatch.delattr(sys.modules["orda_ce_kernel"], "_student", raising=False)
+    with pytest.raises(RuntimeError, match=r"build.py --force"):
+        student.gated_linear_unit(torch.ones(1, 8), torch.ones(8, 8), torch.ones(8, 8))
