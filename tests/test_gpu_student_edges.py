@@ -381,3 +381,59 @@ def test_ramp_in_the_pair_index_eager_and_compiled():
         assert torch.equal(a, b)
     other = student.rotary_embedding(q, k, pos, student.RotaryConfig(64, scaling="yarn", factor=8.0))
     assert not torch.equal(results[0][0], other[0])
+
+
+# ------------------------------------------------------------------------------------------ no term of a sum is lost
+# every forward kernel, whole and partial tiles; one product and K-split ones, whose ranges end inside and at tiles;
+# sizes that are no multiple of a tile, a k block, a 16-byte row
+@pytest.mark.parametrize("n,h,f", [
+    (1, 1000, 2730), (8, 4096, 512), (9, 72, 64), (24, 4096, 1408), (37, 1024, 2816), (64, 4096, 11264), (128, 520, 333),
+    (129, 8, 8), (300, 4096, 264), (513, 136, 1025), (1111, 1000, 2730), (1724, 306, 811), (2048, 1024, 2816),
+    (4096, 256, 512), (8192, 1024, 2816)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_glu_sums_are_exact_on_integers(n, h, f, dtype):
+    check_exact(integers(n, h, seed=1, dtype=dtype, density=0.5), integers(f, h, seed=2, dtype=dtype, density=0.25),
+                integers(f, h, seed=3, dtype=dtype, density=0.25), integers(n, f, seed=4, dtype=dtype, density=0.5))
+
+
+@pytest.mark.parametrize("n,h,f", [(1, 70, 90), (130, 33, 65), (700, 257, 300)])
+def test_glu_fp32_sums_are_exact_on_integers(n, h, f):
+    check_exact(integers(n, h, seed=1, dtype=FP32, density=0.5), integers(f, h, seed=2, dtype=FP32, density=0.5),
+                integers(f, h, seed=3, dtype=FP32, density=0.5), integers(n, f, seed=4, dtype=FP32, density=0.5))
+
+
+# gates at which e^g (GELU: e^{-g^2 / 2}) stays above the smallest normal number of bf16 and fp32
+TAILS = {"silu": 80.0, "gelu": 12.8, "gelu_tanh": 10.0}
+
+
+@pytest.mark.parametrize("act", list(TAILS))
+@pytest.mark.parametrize("n", [5, 40, 300])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_glu_activation_and_derivative_in_their_tails(dtype, n, act):
+    """act(g) and act'(g) alone: one element of x is 1, the up product 1. Relative to their values, however small."""
+    end = TAILS[act]
+    g = torch.cat([torch.linspace(-end, -3, 300, device="cuda"), torch.linspace(3, end, 100, device="cuda")]).to(dtype)
+    x = torch.zeros(n, 8, device="cuda", dtype=dtype)
+    x[0, 0] = 1
+    wg, wu = torch.zeros(2, 400, 8, device="cuda", dtype=dtype)
+    wg[:, 0], wu[:, 0] = g, 1
+    dh = torch.zeros(n, 400, device="cuda", dtype=dtype)
+    dh[0] = 1
+    h, _, dgate, dup = glu_pass(x, wg, wu, act, dh)
+    v = g.double()
+    if act == "silu":
+        s = 1 / (1 + torch.exp(-v))
+        a, d = v * s, s * (1 + v * (1 - s))
+    elif act == "gelu":
+        cdf = torch.special.erfc(-v / math.sqrt(2)) / 2
+        a, d = v * cdf, cdf + v * torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)
+    else:
+        z = 2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)
+        s, t = 1 / (1 + torch.exp(-z)), 1 / (1 + torch.exp(z))
+        a, d = v * s, s + v * s * t * 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * v * v)
+    # e^x of |x| <= 88 in fp32: x and x log2(e) are each rounded (2^-18 of 88 or 127), z of three more roundings;
+    # in d the two terms may cancel down to a tenth of the larger
+    rel = half(dtype) + 2.0 ** -15
+    within(h[0], a, rel * a.abs(), "act")
+    within(dgate[:, 0], d, (half(dtype) + 2.0 ** -14) * d.abs(), "derivative")
+    within(dup[:, 0], a, rel * a.abs(), "act in the backward pass")
