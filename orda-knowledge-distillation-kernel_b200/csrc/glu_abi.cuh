@@ -60,13 +60,13 @@ int glu_rows_launch(const orda_glu_args_t* a, cudaStream_t s) {
 template <typename T16>
 int glu_swap_launch(const orda_glu_args_t* a, cudaStream_t s) {
   GluSwapParams p{};
-  const int tokens = static_cast<int>(std::min<int64_t>(128, cdiv(a->rows, 16) * 16));
+  const int tokens = static_cast<int>(cdiv(a->rows, 16) * 16);  // at most 128: ORDA_GLU_FEW_ROWS
   int rc;
   if ((rc = make_map(&p.gate, a->dtype, a->gate, a->hidden, a->ffn, a->ld_gate, 64, kSwapFeatures))) return rc;
   if ((rc = make_map(&p.up, a->dtype, a->up, a->hidden, a->ffn, a->ld_up, 64, kSwapFeatures))) return rc;
   if ((rc = make_map(&p.x, a->dtype, a->x, a->hidden, a->rows, a->ld_x, 64, static_cast<uint32_t>(tokens)))) return rc;
   p.h = a->h; p.pre_gate = a->pre_gate; p.pre_up = a->pre_up;
-  p.ld_h = a->ld_h; p.ld_pre = a->ld_pre; p.ffn = a->ffn; p.rows = a->rows;
+  p.ld_h = a->ld_h; p.ld_pre = a->ld_pre; p.ffn = a->ffn; p.rows = static_cast<int32_t>(a->rows);
   p.tokens = tokens;
   p.kb = static_cast<int32_t>(cdiv(a->hidden, kBK));
   p.act = a->activation;
@@ -79,13 +79,13 @@ int glu_swap_launch(const orda_glu_args_t* a, cudaStream_t s) {
   set_smem(glu_swap_kernel<T16>, smem);
   // Blocks that share a tile's K: as many as fit beside the other tiles, two blocks an SM, each with at least
   // four k blocks (one round of stages).
-  const int64_t f_tiles = cdiv(a->ffn, kSwapFeatures), t_tiles = cdiv(a->rows, tokens);
-  int64_t split = std::min<int64_t>({8, 2 * num_sms() / (f_tiles * t_tiles), p.kb / 4});
+  const int64_t f_tiles = cdiv(a->ffn, kSwapFeatures);
+  int64_t split = std::min<int64_t>({8, 2 * num_sms() / f_tiles, p.kb / 4});
   split = std::max<int64_t>(split, 1);
   p.kb_part = static_cast<int32_t>(cdiv(p.kb, split));
   p.split = static_cast<int32_t>(cdiv(p.kb, p.kb_part));  // no block without a k block
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(f_tiles * p.split), 1, static_cast<unsigned>(t_tiles));
+  cfg.gridDim = dim3(static_cast<unsigned>(f_tiles * p.split));
   cfg.blockDim = dim3(kSwapThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;

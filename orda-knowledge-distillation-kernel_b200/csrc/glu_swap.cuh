@@ -4,7 +4,7 @@
 //
 // The operands change places: the weights are the M side of the tensor-core product, the tokens its N
 // side, so a tile costs what its tokens cost. A block multiplies 64 gate rows and the same 64 up rows
-// (M = 128: TMEM lanes 0..63 gate, 64..127 up) by up to 128 tokens; both products meet in shared memory,
+// (M = 128: TMEM lanes 0..63 gate, 64..127 up) by all tokens, at most 128; both products meet in shared memory,
 // from where the activation and the product go out in whole rows. One tile a block, no persistence: two
 // blocks fit an SM, so one's epilogue runs under the other's loads, and 8 stages of weights are on
 // their way per SM. What bounds it: reading the weights.
@@ -35,8 +35,9 @@ constexpr uint32_t kSwapSmem = 113 * 1024;  // of a block: two fit an SM
 struct GluSwapParams {
   CUtensorMap gate, up, x;  // boxes: 64 x 64 of the weights, 64 x tokens of x
   void *h, *pre_gate, *pre_up;
-  int64_t ld_h, ld_pre, ffn, rows;
-  int32_t tokens;           // tokens of a tile: a multiple of 16, at most 128
+  int64_t ld_h, ld_pre, ffn;
+  int32_t rows;
+  int32_t tokens;           // tokens of a tile (all rows): a multiple of 16, at most 128
   int32_t stages, kb, kb_part, act;  // k blocks: all, of one block of the cluster
   int32_t split;            // blocks of the cluster
   uint32_t idesc;
@@ -74,7 +75,6 @@ __global__ void __launch_bounds__(kSwapThreads, 2) glu_swap_kernel(const __grid_
   uint32_t tmem_cols = 32;  // a power of two
   while (tmem_cols < static_cast<uint32_t>(p.tokens)) tmem_cols *= 2;
   const int part = static_cast<int>(blockIdx.x) % p.split;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.z) * p.tokens;
   const int64_t f0 = (static_cast<int64_t>(blockIdx.x) / p.split) * kSwapFeatures;
   const int kb0 = part * p.kb_part, kbs = min(p.kb_part, p.kb - kb0);  // at least one
 
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kSwapThreads, 2) glu_swap_kernel(const __grid_
         mbar_arrive_expect_tx(full_bar(s), stage_bytes);
         tma_load_2d(a, &p.gate, full_bar(s), (kb0 + kb) * kBK, static_cast<int32_t>(f0));
         tma_load_2d(a + kATileBytes / 2, &p.up, full_bar(s), (kb0 + kb) * kBK, static_cast<int32_t>(f0));
-        tma_load_2d(a + kATileBytes, &p.x, full_bar(s), (kb0 + kb) * kBK, static_cast<int32_t>(t0));
+        tma_load_2d(a + kATileBytes, &p.x, full_bar(s), (kb0 + kb) * kBK, 0);
       }
     }
   } else if (warp == 1) {
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kSwapThreads, 2) glu_swap_kernel(const __grid_
     const uint32_t sg = smem_u32(exchange), su = sg + p.tokens * kSwapFeatures * 4;
     const int64_t f = f0 + 2 * lane;
     const bool pair = f + 1 < p.ffn;
-    for (int t = part * 4 + warp - 2; t < p.tokens && t0 + t < p.rows; t += 4 * p.split) {
+    for (int t = part * 4 + warp - 2; t < p.rows; t += 4 * p.split) {
       if (f >= p.ffn) break;
       const float nan = __int_as_float(0x7fffffff);
       const uint32_t at_pair = (t * kSwapFeatures + 2 * lane) * 4;
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kSwapThreads, 2) glu_swap_kernel(const __grid_
       });
       if (!ok) a0 = a1 = nan;
       auto put = [&](void* out, int64_t ld, float x, float y) {
-        T16* o = static_cast<T16*>(out) + (t0 + t) * ld + f;
+        T16* o = static_cast<T16*>(out) + t * ld + f;
         if (pair && (reinterpret_cast<uintptr_t>(o) & 3u) == 0) {
           *reinterpret_cast<uint32_t*>(o) = pack2<T16>(x, y);
         } else {

@@ -24,7 +24,6 @@ constexpr int kGradThreads = 256;
 
 template <int N>
 struct GradTable {
-  static constexpr int kCapacity = N;
   const void* src[N];
   void* dst[N];
   int64_t numel[N];

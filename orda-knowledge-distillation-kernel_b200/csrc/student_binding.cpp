@@ -765,7 +765,6 @@ PYBIND11_MODULE(_student, m) {
   py::class_<RotaryPlan, PlanPtr>(m, "RotaryPlan")
       .def(py::init<const std::vector<double>&, int64_t, bool, double>());
   m.def("gated_linear_unit", wrap_pybind_function_no_gil(gated_linear_unit));
-  m.def("activation_code", torch::wrap_pybind_function(activation_code));
   m.def("glu_forward", wrap_pybind_function_no_gil(glu_forward_op));
   m.def("glu_backward", wrap_pybind_function_no_gil(glu_backward_op));
   m.def("rotary_embedding", wrap_pybind_function_no_gil(rotary_embedding));
