@@ -126,7 +126,7 @@ __device__ __forceinline__ double chunk_squares(const T* p, int64_t n) {
 }
 
 template <typename T>
-__device__ __forceinline__ void chunk_scale(const T* p, T* d, int64_t n, float c) {
+__device__ __forceinline__ void chunk_scale(const T* p, T* d, int64_t n, float c, float c2) {
   constexpr int V = 16 / sizeof(T);
   int64_t done = 0;
   if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(d)) & 15u) == 0) {
@@ -143,7 +143,7 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* d, int64_t n, float c
         float v[V];
         unpack16<T>(u[k], v);
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] *= c;
+        for (int e = 0; e < V; ++e) v[e] = v[e] * c * c2;
         o[i + k * kGradThreads] = pack16<T>(v);
       }
     }
@@ -151,12 +151,12 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* d, int64_t n, float c
       float v[V];
       unpack16<T>(q[i], v);
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] *= c;
+      for (int e = 0; e < V; ++e) v[e] = v[e] * c * c2;
       o[i] = pack16<T>(v);
     }
     done = vecs * V;
   }
-  for (int64_t i = done + threadIdx.x; i < n; i += kGradThreads) d[i] = Conv<T>::from_f(Conv<T>::to_f(p[i]) * c);
+  for (int64_t i = done + threadIdx.x; i < n; i += kGradThreads) d[i] = Conv<T>::from_f(Conv<T>::to_f(p[i]) * c * c2);
 }
 
 template <int N>
@@ -198,7 +198,10 @@ __global__ void __launch_bounds__(kGradThreads) grad_scale_kernel(const __grid_c
   const double s = norm_of(partial, parts, shared);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(s);
   const double ratio = max_norm / (s + eps);
-  const float factor = ratio >= 1.0 ? 1.f : static_cast<float>(ratio);  // NaN stays NaN
+  // below fp32's normal range the factor would lose bits that the values have: it is taken in two steps
+  const bool tiny = ratio < 0x1p-126;
+  const float factor = ratio >= 1.0 ? 1.f : static_cast<float>(tiny ? ratio * 0x1p64 : ratio);  // NaN stays NaN
+  const float rest = tiny ? 0x1p-64f : 1.f;
   const int chunks = g.first_chunk[g.count];
   for (int c = chunks - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= static_cast<int>(gridDim.x)) {
     const int t = tensor_of(g, c);
@@ -206,12 +209,12 @@ __global__ void __launch_bounds__(kGradThreads) grad_scale_kernel(const __grid_c
     const int64_t at = static_cast<int64_t>(c - g.first_chunk[t]) * g.chunk;
     const int64_t n = min(static_cast<int64_t>(g.chunk), g.numel[t] - at);
     if (g.dtype[t] == ORDA_F32)
-      chunk_scale(static_cast<const float*>(g.src[t]) + at, static_cast<float*>(g.dst[t]) + at, n, factor);
+      chunk_scale(static_cast<const float*>(g.src[t]) + at, static_cast<float*>(g.dst[t]) + at, n, factor, rest);
     else if (g.dtype[t] == ORDA_F16)
-      chunk_scale(static_cast<const __half*>(g.src[t]) + at, static_cast<__half*>(g.dst[t]) + at, n, factor);
+      chunk_scale(static_cast<const __half*>(g.src[t]) + at, static_cast<__half*>(g.dst[t]) + at, n, factor, rest);
     else
       chunk_scale(static_cast<const __nv_bfloat16*>(g.src[t]) + at, static_cast<__nv_bfloat16*>(g.dst[t]) + at, n,
-                  factor);
+                  factor, rest);
   }
 }
 

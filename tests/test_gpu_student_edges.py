@@ -437,3 +437,17 @@ def test_glu_activation_and_derivative_in_their_tails(dtype, n, act):
     within(h[0], a, rel * a.abs(), "act")
     within(dgate[:, 0], d, (half(dtype) + 2.0 ** -14) * d.abs(), "derivative")
     within(dup[:, 0], a, rel * a.abs(), "act in the backward pass")
+
+
+@pytest.mark.parametrize("value,max_norm", [(1e37, 1e-2), (3e38, 0.1), (1e38, 1e-6), (1e38, 0.0)])
+def test_clip_by_factors_below_the_normal_range(value, max_norm):
+    """A diverged step's gradients: the factor is no normal fp32 number, the clipped values are."""
+    for dtype in (FP32, BF16):
+        g = torch.full((1000,), value, device="cuda", dtype=dtype)
+        g[::3] *= -0.5
+        want = g.double() * (max_norm / (float(g.double().square().sum().sqrt()) + 1e-6))
+        clipped, _ = student.clip_gradients([g], max_norm)
+        # the factor, two products (the second by a power of two), the value
+        within(clipped[0], want, (half(dtype) + 2 * half(FP32)) * want.abs())
+        student.clip_grad_norm_(_params(g), max_norm)
+        assert torch.equal(g, clipped[0])
