@@ -359,6 +359,9 @@ std::tuple<Tensor, Tensor> glu_forward_op(const Tensor& x, const Tensor& gate, c
   check_glu(x, gate, up);
   const GluOperands o(plain(x.reshape({-1, x.size(-1)})), plain(gate), plain(up));
   auto [h, pre] = glu_forward(o.t[0], o.t[1], o.t[2], act, true);
+  // an op's outputs are compared and kept whole: no memory behind the last feature that holds anything
+  const int64_t ffn = gate.size(0);
+  if (pre.size(2) > ffn) pre.slice(2, ffn).zero_();
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end() - 1);
   shape.push_back(gate.size(0));
   return {h.view(shape), pre};

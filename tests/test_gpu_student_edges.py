@@ -451,3 +451,24 @@ def test_clip_by_factors_below_the_normal_range(value, max_norm):
         within(clipped[0], want, (half(dtype) + 2 * half(FP32)) * want.abs())
         student.clip_grad_norm_(_params(g), max_norm)
         assert torch.equal(g, clipped[0])
+
+
+# ------------------------------------------------------------------------------------------ the custom ops as such
+def _custom_op_calls():
+    ops = torch.ops.orda_b200
+    for n, h, f in ((40, 64, 72), (3, 66, 75), (0, 64, 72), (300, 64, 71)):
+        x, wg, wu, _ = glu_inputs(n, h, f, BF16, 5)
+        yield ops.glu_forward, (*(t.requires_grad_(True) for t in (x, wg, wu)), 0)
+    cfg = student._config_values(student.RotaryConfig(64, rotary_dim=32))
+    q, k, pos = randn(2, 5, 4, 64, seed=1), randn(2, 2, 5, 64, seed=2).transpose(1, 2), torch.arange(5, device="cuda")
+    w = [randn(64, seed=3 + i).requires_grad_(True) for i in range(2)]
+    q, k = q.requires_grad_(True), k.requires_grad_(True)
+    yield ops.rotary, (q, k, pos, None, None, 0.0, False, *cfg)
+    yield ops.rotary, (q, k, pos, *w, 1e-6, False, *cfg)
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_custom_ops_keep_the_rules_of_custom_ops(which):
+    """Schema, shapes without data, autograd registration, and tracing with dynamic shapes."""
+    op, args = list(_custom_op_calls())[which]
+    torch.library.opcheck(op, args)
