@@ -767,6 +767,7 @@ PYBIND11_MODULE(_student, m) {
   using torch::wrap_pybind_function_no_gil;
   py::class_<RotaryPlan, PlanPtr>(m, "RotaryPlan")
       .def(py::init<const std::vector<double>&, int64_t, bool, double>());
+  m.def("refuse_eager_nodes_in_capture", wrap_pybind_function_no_gil(refuse_eager_nodes_in_capture));
   m.def("gated_linear_unit", wrap_pybind_function_no_gil(gated_linear_unit));
   m.def("glu_forward", wrap_pybind_function_no_gil(glu_forward_op));
   m.def("glu_backward", wrap_pybind_function_no_gil(glu_backward_op));

@@ -13,7 +13,7 @@ tangent is refused) and become one custom op each under ``torch.compile`` and wh
 the loss there is no CPU fallback: CUDA tensors on a B200 are required. Every call runs on the current stream of
 its tensors' device, takes its workspace from the caching allocator and does not synchronise, so it can be
 captured into a CUDA graph; a captured backward pass is refused while an eager autograd graph of the default
-stream still holds one of its leaves.
+stream still holds one of its leaves (a compiled one is PyTorch's own node, and is not: drop such graphs first).
 """
 from __future__ import annotations
 
@@ -81,6 +81,7 @@ def _glu_setup(ctx, inputs, output):
 
 
 def _glu_op_backward(ctx, dh, _dpre):
+    _bound().refuse_eager_nodes_in_capture("gated_linear_unit")
     return (*torch.ops.orda_b200.glu_backward(dh, *ctx.saved_tensors, ctx.act), None)
 
 
@@ -273,6 +274,7 @@ def _rotary_setup(ctx, inputs, output):
 
 
 def _rotary_op_backward(ctx, dq, dk):
+    _bound().refuse_eager_nodes_in_capture("qk_norm_rotary" if ctx.normed else "rotary_embedding")
     if ctx.normed:
         positions, q, k, q_weight, k_weight = ctx.saved_tensors
         gq, gk, gwq, gwk = torch.ops.orda_b200.qk_norm_rotary_backward(dq, dk, q, k, positions, q_weight, k_weight,

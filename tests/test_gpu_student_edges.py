@@ -472,3 +472,39 @@ def test_custom_ops_keep_the_rules_of_custom_ops(which):
     """Schema, shapes without data, autograd registration, and tracing with dynamic shapes."""
     op, args = list(_custom_op_calls())[which]
     torch.library.opcheck(op, args)
+
+
+@pytest.mark.parametrize("which", ["glu", "rotary", "norm"])
+def test_captured_backward_of_a_recorded_call_is_refused_as_a_plain_one_is(which):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Pass(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x, wg, wu, q, k, wq, wk, pos = _block_inputs(4)
+    cfg = student.RotaryConfig(64)
+    call = {"glu": lambda t: student.gated_linear_unit(x, t, wu),
+            "rotary": lambda t: student.rotary_embedding(t, k, pos, cfg)[0],
+            "norm": lambda t: student.qk_norm_rotary(t, k, wq, wk, pos, cfg)[0]}[which]
+    leaf = (wg if which == "glu" else q).detach().requires_grad_(True)
+
+    def step():
+        with Pass():
+            y = call(leaf)
+            return torch.autograd.grad(y, leaf, torch.ones_like(y))[0]
+
+    want = step().clone()
+    eager = call(leaf)  # recorded on the default stream
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still lives"):
+        with torch.cuda.graph(graph):
+            step()
+    del eager, graph
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    assert torch.equal(got, want)
