@@ -14,7 +14,9 @@
 // up through distributed shared memory, in the blocks' order.
 //
 // Measured in bf16: 64 rows 4096 -> 11264 43 us (4.3 TB/s; the 512-row tiles of the pair GEMM 91, the 256-row
-// ones 60), 64 rows 1024 -> 2816 10.3 us with four blocks a tile, 14.4 with one.
+// ones 60), 64 rows 1024 -> 2816 10.3 us with four blocks a tile, 14.4 with one. Short calls are bound by latencies:
+// launch and cluster start, the few k blocks of a block, and after them the remote reads, which follow one another
+// (each block's `failed`, then each block's part of a token).
 //
 //   warp 0 : TMA producer    warp 1 : MMA issuer    warps 2..5 : epilogue
 //

@@ -99,9 +99,9 @@ def gated_linear_unit(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: tor
     ``x`` is ``[..., hidden]``, the weights ``[ffn, hidden]``; the result is ``[..., ffn]``. ``activation``
     is ``"silu"``, ``"gelu"`` (erf), ``"gelu_tanh"`` or ``"relu"``. The compute dtype follows the loss's rule
     (active autocast dtype, else bf16 if any input is bf16, else fp16, else fp32); products and the
-    activation are formed in fp32 and rounded once. fp32 runs on CUDA cores, exactly but without the tensor
-    cores' speed. Back-propagates into all three; the backward pass keeps the two products in the compute
-    dtype. Inputs with a hidden size that is no multiple of 8 are copied into padded rows first.
+    activation are formed in fp32 and rounded once. fp32 runs on CUDA cores, without the tensor cores' speed (and
+    slower than ``torch.nn.Linear``). Back-propagates into all three; the backward pass keeps the two products,
+    and multiplies their gradients, in the compute dtype. Inputs with a hidden size that is no multiple of 8 are copied into padded rows first.
     """
     h = None
     if not torch.compiler.is_compiling():
