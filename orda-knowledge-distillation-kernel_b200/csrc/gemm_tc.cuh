@@ -83,8 +83,8 @@ struct TcGemmParams {
   StoreEpiParams st;
 };
 
-// By one thread, after its block's own stores: of two blocks that write a marked value the one that ends last
-// has seen the status, or the other one has.
+// By one thread of a block whose own stores are done. Another block may still overwrite the mark, but it then
+// ends after this one, finds the status set and marks again.
 __device__ __forceinline__ void mark_timeout(const TcGemmParams& p) {
 #pragma unroll
   for (int i = 0; i < 2; ++i)

@@ -51,14 +51,13 @@ __device__ __forceinline__ void glu_act(float g, float& a, float& d) {
     a = g * cdf;
     d = cdf + g * e * 0.39894228040143268f;
   } else {
-    // 1/2 (1 + tanh z) = 1 / (1 + e^(-2z)), z = sqrt(2/pi) (g + 0.044715 g^3); z is taken within |g| <= 1e4, where s
-    // has long been 0 or 1: the square and the cube of a larger g may be infinite, and d inf * 0
+    // 1/2 (1 + tanh z) = 1 / (1 + e^(-2z)), z = sqrt(2/pi) (g + 0.044715 g^3). Where g^2 is infinite, s is 0 or 1 and
+    // d must not be inf * 0
     const float c = 0.79788456080286536f;
-    const float q = fabsf(g) > 1e4f ? copysignf(1e4f, g) : g;
-    const float z = c * (q + 0.044715f * q * q * q);
+    const float z = c * (g + 0.044715f * g * g * g);
     const float s = EXACT ? 1.f / (1.f + expf(-2.f * z)) : __fdividef(1.f, 1.f + fast_exp(-2.f * z));
     a = g * s;
-    d = s + q * (2.f * s * (1.f - s)) * c * (1.f + 0.134145f * q * q);
+    d = s + g * (2.f * s * (1.f - s)) * c * (1.f + 0.134145f * fminf(g * g, 1e30f));
   }
 }
 
