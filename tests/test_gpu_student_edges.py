@@ -508,3 +508,31 @@ def test_captured_backward_of_a_recorded_call_is_refused_as_a_plain_one_is(which
         got = step()
     graph.replay()
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------ results behind 2^31 elements
+@pytest.mark.parametrize("norm", [False, True])
+def test_rotary_results_and_gradients_behind_32_bits(norm):
+    """Tokens whose results, and whose gradients, lie behind 2^31 elements, against the same tokens alone."""
+    n, heads, d = 70_000, 256, 128
+    assert n * heads * d > 2 ** 31
+    cfg, pos = student.RotaryConfig(d), torch.arange(n, device="cuda")
+    w = [(1 + randn(d, seed=i, scale=0.1)).requires_grad_(norm) for i in range(2)]
+    rows = torch.tensor([0, 65_535, 65_536, n - 1], device="cuda")  # 65536 x 256 x 128 = 2^31
+    values, dys = randn(4, heads, d, seed=3, dtype=BF16), randn(4, heads, d, seed=4, dtype=BF16)
+
+    def run(q, k, p, dy):
+        q = q.requires_grad_(True)
+        out = (student.qk_norm_rotary(q, k, *w, p, cfg) if norm else student.rotary_embedding(q, k, p, cfg))[0]
+        return out.detach(), *torch.autograd.grad(out, [q, *w[:1]] if norm else [q], dy)
+
+    q = torch.ones(n, heads, d, device="cuda", dtype=BF16)
+    dy = torch.zeros_like(q)
+    q[rows], dy[rows] = values, dys
+    got = run(q, torch.ones(n, 1, d, device="cuda", dtype=BF16), pos, dy)
+    want = run(values, torch.ones(4, 1, d, device="cuda", dtype=BF16), pos[rows], dys)
+    assert torch.equal(got[0][rows], want[0]) and torch.equal(got[1][rows], want[1])
+    got[1][rows] = 0
+    assert not got[1].any()
+    if norm:  # the other tokens add zeros, in another order of the same terms
+        torch.testing.assert_close(got[2], want[2], rtol=0, atol=float(want[2].abs().max()) * 4 * heads * 2.0 ** -24)
